@@ -1,0 +1,383 @@
+"""Cases and plain forms of the token operators: atom types (or the ids of any vocabulary) looked up in a table and the
+gradient of that table, the log-probabilities of chosen ids, the preference loss over pairs of molecules and the clipped
+policy loss with a KL term, the last two with the gradient of the logits.
+
+``own`` False: elementary torch operations in 32 bits (64 for the chosen log-probabilities, one for each row, and what is
+made of them), rounded once at the end.
+``own`` True: the calls a user makes, diffusion_model_ligandmol_generation_amd.tokens."""
+import math
+
+import torch
+
+own = False
+
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+SIZES = {"fp32": 4, "bf16": 2, "fp16": 2}
+CLIP_LOW, CLIP_HIGH = 0.2, 0.28
+
+
+# ------------------------------------------------------------------------------------------------ cases
+def listed():
+    return [
+        # the 1024 x 29-atom batch of the headline workload: every atom's type looked up in the [119, 256] embedding
+        dict(name="embed_atoms", op="embed", tokens=29696, vocab=119, width=256, dtype="fp32", atoms=True),
+        # a vocabulary of the usual size, half precision
+        dict(name="embed_vocab", op="embed", tokens=65536, vocab=32000, width=1024, dtype="bf16", atoms=False),
+        # the gradient of the atom embedding for the same batch: five types hold nearly all rows
+        dict(name="embed_grad_atoms", op="embed_grad", tokens=29696, vocab=119, width=256, dtype="fp32", atoms=True),
+        # many rows of the table without a token, a few with very many
+        dict(name="embed_grad_vocab", op="embed_grad", tokens=65536, vocab=32000, width=1024, dtype="bf16", atoms=False),
+        # one ligand's types scored, as a sampler does between steps: latency
+        dict(name="logprob_ligand", op="logprob", tokens=29, vocab=119, dtype="fp32", atoms=True, ignored=0.0),
+        # scoring under a reference policy, rows of 64 KB
+        dict(name="logprob_vocab", op="logprob", tokens=8192, vocab=32000, dtype="bf16", atoms=False, ignored=0.05),
+        # 512 pairs of 29-atom ligands
+        dict(name="preference_atoms", op="preference", tokens=29696, vocab=119, pairs=512, ragged=False, dtype="fp32", atoms=True,
+             ignored=0.0, kind="sigmoid", average=False),
+        # 24 ragged pairs over a vocabulary of odd size, padding among them
+        dict(name="preference_vocab", op="preference", tokens=6007, vocab=32003, pairs=24, ragged=True, dtype="bf16", atoms=False,
+             ignored=0.1, kind="ipo", average=True),
+        # one ligand under its advantage: latency
+        dict(name="policy_ligand", op="policy", tokens=29, vocab=119, sequences=1, ragged=False, dtype="fp32", atoms=True,
+             ignored=0.0, per_sequence=True, aggregate="token"),
+        # 512 ragged ligands, as the training configuration with 10 to 64 atoms has them
+        dict(name="policy_atoms", op="policy", tokens=18944, vocab=119, sequences=512, ragged=True, dtype="fp32", atoms=True,
+             ignored=0.02, per_sequence=True, aggregate="sequence"),
+        # a rollout buffer of many ligands at once
+        dict(name="policy_rollout", op="policy", tokens=593920, vocab=119, sequences=20480, ragged=False, dtype="fp32", atoms=True,
+             ignored=0.0, per_sequence=True, aggregate="token"),
+        # token advantages over a vocabulary
+        dict(name="policy_vocab", op="policy", tokens=8192, vocab=32000, sequences=16, ragged=True, dtype="bf16", atoms=False,
+             ignored=0.05, per_sequence=False, aggregate="token"),
+    ]
+
+
+MOST_ROWS = 8192 * 32000   # values of the largest listed logits
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["embed", "embed_grad", "logprob", "preference", "policy"])
+    atoms = rng.random() < 0.4
+    dtype = rng.choice(["fp32", "fp32", "bf16", "fp16"]) if atoms else rng.choice(["fp32", "bf16", "bf16", "fp16"])
+    c = dict(op=op, dtype=dtype, atoms=atoms)
+    if op in ("embed", "embed_grad"):
+        c["vocab"] = 119 if atoms else _log_int(rng, 16, 100000)
+        c["width"] = 256 if atoms else _log_int(rng, 8, 2048)
+        most = 65536 * 1024 * 2 // SIZES[dtype] // c["width"]
+        c["vocab"] = max(16, min(c["vocab"], 32000 * 1024 * 2 // SIZES[dtype] // c["width"]))
+        c["tokens"] = _log_int(rng, 1, max(2, min(400000, most)))
+        return c
+    c["vocab"] = 119 if atoms else _log_int(rng, 16, 65536)
+    c["tokens"] = _log_int(rng, 1, max(2, min(590000, MOST_ROWS * 2 // SIZES[dtype] // c["vocab"] // 2)))
+    c["ignored"] = rng.choice([0.0, 0.0, 0.05, 0.3])
+    if op == "preference":
+        c.update(pairs=_log_int(rng, 1, max(1, min(4096, c["tokens"] // 2))), ragged=True,
+                 kind=rng.choice(["sigmoid", "ipo"]))
+        c["average"] = c["kind"] == "ipo" or rng.random() < 0.3
+    elif op == "policy":
+        c.update(sequences=_log_int(rng, 1, max(1, min(20480, c["tokens"]))), ragged=True,
+                 per_sequence=rng.random() < 0.6, aggregate=rng.choice(["token", "sequence"]))
+    return c
+
+
+def grad_scale(case):
+    """The loss scale of half-precision training: gradients of 1 / (number of tokens or pairs) would underflow in fp16."""
+    if case["dtype"] != "fp16":
+        return 1.0
+    n = case["pairs"] if case["op"] == "preference" and not case["average"] else case["tokens"]
+    return float(2 ** math.ceil(math.log2(n)))
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+def _ids(case, g):
+    """Types of drug-like ligands, or ids whose frequencies fall off as those of words do."""
+    T, V = case["tokens"], case["vocab"]
+    if case["atoms"]:
+        kinds = torch.tensor([1, 6, 7, 8, 9], device="cuda")
+        share = torch.tensor([0.30, 0.50, 0.09, 0.09, 0.02], device="cuda")
+        ids = kinds[torch.multinomial(share, T, replacement=True, generator=g)]
+    else:
+        u = torch.rand(T, device="cuda", generator=g, dtype=torch.float64)
+        ids = torch.exp(u * math.log(V)).long().clamp_(1, V) - 1
+        ids = (ids * 7919 + 13) % V   # the frequent ids lie anywhere in the table
+    p = case.get("ignored", 0.0)
+    if p:
+        ids = torch.where(torch.rand(T, device="cuda", generator=g) < p, torch.full_like(ids, -1), ids)
+    return ids
+
+
+def _seq_ptr(case, n, g):
+    T = case["tokens"]
+    if not case["ragged"]:
+        return (torch.arange(n + 1, device="cuda") * (T // n)).to(torch.int32)
+    cuts = torch.randint(0, T + 1, (n - 1,), device="cuda", generator=g).sort().values
+    ends = torch.tensor([0, T], device="cuda")
+    return torch.cat([ends[:1], cuts, ends[1:]]).to(torch.int32)
+
+
+def _row_logprobs(x, ids):
+    """log softmax of each row at its id, 0 where the id is ignored; rows in pieces, so that little memory is used."""
+    out = torch.zeros(x.shape[0], device=x.device)
+    step = max(1, (1 << 26) // x.shape[1])
+    for a in range(0, x.shape[0], step):
+        y = x[a:a + step].float()
+        i = ids[a:a + step]
+        lp = y.gather(1, i.clamp(min=0)[:, None])[:, 0] - torch.logsumexp(y, 1)
+        out[a:a + step] = torch.where(i >= 0, lp, torch.zeros_like(lp))
+    return out
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(int(seed))
+    dt = DTYPES[case["dtype"]]
+    T, V = case["tokens"], case["vocab"]
+    s = dict(case=case, ids=_ids(case, g))
+    if case["op"] in ("embed", "embed_grad"):
+        D = case["width"]
+        s["scale"] = math.sqrt(D)
+        s["table" if case["op"] == "embed" else "d_out"] = torch.randn(V if case["op"] == "embed" else T, D, device="cuda",
+                                                                       generator=g, dtype=dt) * 0.05
+        return s
+    logits = torch.randn(T, V, device="cuda", generator=g, dtype=dt).mul_(2.0)
+    if V > 40:   # some ids can not be chosen (types that no ligand has): their logits are -inf
+        first = int(torch.randint(20, V - 8, (1,), generator=torch.Generator().manual_seed(int(seed))))
+        logits[:, first:first + 4] = float("-inf")
+        s["ids"] = torch.where((s["ids"] >= first) & (s["ids"] < first + 4), torch.zeros_like(s["ids"]), s["ids"])
+    s["logits"] = logits
+    if case["op"] == "logprob":
+        return s
+    lp = _row_logprobs(logits, s["ids"])
+    noise = lambda k: k * torch.randn(T, device="cuda", generator=g)   # noqa: E731
+    moved = noise(0.1)
+    s["ref"] = lp + moved + 0.05 * moved.sign()   # a policy that has moved away from its reference
+    if case["op"] == "preference":
+        s["seq_ptr"] = _seq_ptr(case, 2 * case["pairs"], g)
+        return s
+    s["seq_ptr"] = _seq_ptr(case, case["sequences"], g)
+    old = lp + noise(0.15)
+    # a ratio next to a clip bound is moved off it: on which side it falls is no matter of accuracy
+    for bound in (1 - CLIP_LOW, 1 + CLIP_HIGH):
+        near = ((lp - old).exp() - bound).abs() < 1e-3
+        old = torch.where(near, old + 4e-3, old)
+    s["old"] = old
+    # rewards less the mean of earlier rollouts, which this one's is above
+    s["adv"] = torch.randn(case["sequences"] if case["per_sequence"] else T, device="cuda", generator=g) + 0.5
+    return s
+
+
+# ------------------------------------------------------------------------------------------------ plain forms
+def _segments(ptr, T):
+    """For each token the sequence it lies in."""
+    return torch.searchsorted(ptr[1:].contiguous(), torch.arange(T, device=ptr.device, dtype=ptr.dtype), right=True)
+
+
+def _sums(ptr, values):
+    """The sum of each sequence's values, in 64 bits."""
+    upto = torch.cat([torch.zeros(1, device=ptr.device, dtype=torch.float64), values.double().cumsum(0)])
+    ends = upto[ptr.long()]
+    return ends[1:] - ends[:-1]
+
+
+def _softmax_parts(x):
+    m = x.amax(1, keepdim=True)
+    e = (x - m).exp()
+    total = e.sum(1, keepdim=True)
+    return m, e, total
+
+
+def _chosen(x, m, total, ids):
+    """Each row's log-probability of its id, in 64 bits: differences of two policies' are small against them."""
+    return (x.gather(1, ids.clamp(min=0)[:, None]) - m)[:, 0].double() - total[:, 0].double().log()
+
+
+def _plain_embed(s):
+    t = s["table"]
+    return {"out": (t[s["ids"]].float() * s["scale"]).to(t.dtype)}
+
+
+def _plain_embed_grad(s):
+    d, ids, V = s["d_out"], s["ids"], s["case"]["vocab"]
+    T, D = d.shape
+    # long sums in 32 bits: added up in groups of tokens first
+    groups = max(1, min(64, T // (8 * V)))
+    where = (torch.arange(T, device=d.device) % groups) * V + ids
+    acc = torch.zeros(groups * V, D, device=d.device).index_add_(0, where, d.float())
+    return {"d_table": (acc.view(groups, V, D).sum(0) * s["scale"]).to(d.dtype)}
+
+
+def _plain_logprob(s):
+    x, ids = s["logits"].float(), s["ids"]
+    m, _, total = _softmax_parts(x)
+    lp = _chosen(x, m, total, ids)
+    return {"logp": torch.where(ids >= 0, lp, torch.zeros_like(lp)).float()}
+
+
+def _plain_d_logits(e, total, ids, coef, dtype):
+    """coef (onehot - softmax), 0 in the rows of ignored tokens (whose coef is 0)."""
+    d = e.div_(total).mul_(-coef[:, None])
+    d.scatter_add_(1, ids.clamp(min=0)[:, None], coef[:, None])
+    return d.to(dtype)
+
+
+def _plain_preference(s):
+    c, logits, ids, ptr = s["case"], s["logits"], s["ids"], s["seq_ptr"]
+    T, P, beta, smooth = c["tokens"], c["pairs"], 0.1, 0.1
+    x = logits.float()
+    m, e, total = _softmax_parts(x)
+    valid = ids >= 0
+    lp = _chosen(x, m, total, ids)
+    diff = torch.where(valid, lp - s["ref"], torch.zeros_like(lp))
+    seq = _segments(ptr, T)
+    ratio, length = _sums(ptr, diff), _sums(ptr, valid).clamp(min=1)
+    share = 1 / length if c["average"] else torch.ones_like(length)
+    ratio = ratio * share
+    gap = ratio[:P] - ratio[P:]
+    if c["kind"] == "sigmoid":
+        z = beta * gap
+        loss = (1 - smooth) * torch.log1p((-z).exp()) + smooth * torch.log1p(z.exp())
+        slope = beta * (torch.sigmoid(z) - (1 - smooth))
+    else:
+        z = gap - 1 / (2 * beta)
+        loss, slope = z * z, 2 * z
+    slope = torch.cat([slope, -slope]) / P * share
+    coef = torch.where(valid, slope[seq] * grad_scale(c), torch.zeros_like(lp)).float()
+    return {"loss": loss.mean().float(), "log_ratio": ratio.float(), "margin": gap.float(),
+            "d_logits": _plain_d_logits(e, total, ids, coef, logits.dtype)}
+
+
+def _plain_policy(s):
+    c, logits, ids, ptr = s["case"], s["logits"], s["ids"], s["seq_ptr"]
+    T, S, kl_coef = c["tokens"], c["sequences"], 0.05
+    x = logits.float()
+    m, e, total = _softmax_parts(x)
+    valid = ids >= 0
+    lp = _chosen(x, m, total, ids)
+    lp = torch.where(valid, lp, torch.zeros_like(lp))
+    seq = _segments(ptr, T)
+    adv = s["adv"][seq] if c["per_sequence"] else s["adv"]
+    if c["aggregate"] == "token":
+        weight = valid.double() / valid.sum().clamp(min=1)
+    else:
+        length = _sums(ptr, valid).clamp(min=1)
+        weight = valid.double() / (S * length[seq])
+    rho = (lp - s["old"]).exp()
+    clipped = ((adv > 0) & (rho > 1 + CLIP_HIGH)) | ((adv < 0) & (rho < 1 - CLIP_LOW))
+    gain = torch.minimum(rho * adv, rho.clamp(1 - CLIP_LOW, 1 + CLIP_HIGH) * adv)
+    q = s["ref"] - lp
+    kl = torch.expm1(q) - q
+    slope = torch.where(clipped, torch.zeros_like(rho), -adv * rho) - kl_coef * torch.expm1(q)
+    coef = (weight * slope * grad_scale(c)).float()
+    surrogate, kl = (weight * -gain).sum(), (weight * kl).sum()
+    return {"loss": (surrogate + kl_coef * kl).float(), "surrogate": surrogate.float(), "kl": kl.float(),
+            "clip_fraction": (weight * clipped).sum().float(), "logp": lp.float(),
+            "d_logits": _plain_d_logits(e, total, ids, coef, logits.dtype)}
+
+
+# ------------------------------------------------------------------------------------------------ one pass
+def run(s):
+    c = s["case"]
+    if own:
+        from diffusion_model_ligandmol_generation_amd import tokens as tk
+        if c["op"] == "embed":
+            return {"out": tk.embed_tokens(s["ids"], s["table"], s["scale"])}
+        if c["op"] == "embed_grad":
+            return {"d_table": tk.embed_tokens_grad(s["d_out"], s["ids"], c["vocab"], s["scale"])}
+        if c["op"] == "logprob":
+            return {"logp": tk.token_logprobs(s["logits"], s["ids"])}
+        if c["op"] == "preference":
+            r = tk.preference_loss_and_grad(s["logits"], s["ids"], s["seq_ptr"], s["ref"], beta=0.1, label_smoothing=0.1,
+                                            kind=c["kind"], average=c["average"], grad_scale=grad_scale(c))
+            return {"loss": r.loss, "log_ratio": r.log_ratio, "margin": r.margin, "d_logits": r.d_logits}
+        r = tk.policy_loss_and_grad(s["logits"], s["ids"], s["seq_ptr"], s["adv"], s["old"], s["ref"], clip_low=CLIP_LOW,
+                                    clip_high=CLIP_HIGH, kl_coef=0.05, aggregate=c["aggregate"],
+                                    grad_scale=grad_scale(c))
+        return {"loss": r.loss, "surrogate": r.surrogate, "kl": r.kl, "clip_fraction": r.clip_fraction, "logp": r.logp,
+                "d_logits": r.d_logits}
+    plain = {"embed": _plain_embed, "embed_grad": _plain_embed_grad, "logprob": _plain_logprob,
+             "preference": _plain_preference, "policy": _plain_policy}
+    return plain[c["op"]](s)
+
+
+def work(case):
+    T, V, z = case["tokens"], case["vocab"], SIZES[case["dtype"]]
+    if case["op"] == "embed":     # the rows that are read: no more than the table, no more than one for each token
+        D = case["width"]
+        return {"bytes": 8 * T + T * D * z + min(T, V) * D * z, "flops": T * D}
+    if case["op"] == "embed_grad":
+        D = case["width"]
+        return {"bytes": 8 * T + T * D * z + V * D * z, "flops": T * D}
+    live = 1 - case["ignored"]    # a row without a token is not read, its gradient is written
+    read, per = live * T * V * z, 8 * T
+    if case["op"] == "logprob":
+        return {"bytes": read + per + 4 * T, "flops": 4 * live * T * V}
+    if case["op"] == "preference":
+        return {"bytes": read + T * V * z + per + 4 * T + 16 * case["pairs"], "flops": 7 * live * T * V}
+    return {"bytes": read + T * V * z + per + 12 * T + 4 * len_adv(case), "flops": 7 * live * T * V}
+
+
+def len_adv(case):
+    return case["sequences"] if case["per_sequence"] else case["tokens"]
+
+
+# ------------------------------------------------------------------------------------------------ 64 bits
+def exact(case, seed):
+    s = prepare(case, seed)
+    ids, op = s["ids"], case["op"]
+    if op == "embed":
+        return {"out": torch.index_select(s["table"].double(), 0, ids) * s["scale"]}
+    if op == "embed_grad":
+        d = torch.zeros(case["vocab"], case["width"], device="cuda", dtype=torch.float64)
+        return {"d_table": d.index_add(0, ids, s["d_out"].double(), alpha=s["scale"])}
+    logits, T, V = s["logits"], case["tokens"], case["vocab"]
+    keep = ids.ge(0)
+    pieces = [slice(a, min(T, a + max(1, (1 << 25) // V))) for a in range(0, T, max(1, (1 << 25) // V))]
+
+    def rows(piece):
+        return torch.log_softmax(logits[piece].double(), -1)
+
+    logp = torch.cat([rows(p).take_along_dim(ids[p].clamp(min=0)[:, None], 1)[:, 0] for p in pieces]) * keep
+    if op == "logprob":
+        return {"logp": logp}
+    ptr = s["seq_ptr"].long()
+    owner = torch.repeat_interleave(torch.arange(ptr.numel() - 1, device="cuda"), ptr.diff())
+    count = torch.bincount(owner, weights=keep.double(), minlength=ptr.numel() - 1)
+    if op == "preference":
+        P = case["pairs"]
+        r = torch.bincount(owner, weights=(logp - s["ref"].double()) * keep, minlength=2 * P)
+        norm = count.clamp(min=1) if case["average"] else torch.ones_like(count)
+        r = (r / norm).requires_grad_()
+        gap = r[:P] - r[P:]
+        if case["kind"] == "sigmoid":
+            f = torch.nn.functional.softplus
+            loss = (0.9 * f(-0.1 * gap) + 0.1 * f(0.1 * gap)).mean()
+        else:
+            loss = ((gap - 5.0) ** 2).mean()
+        g, = torch.autograd.grad(loss, r)
+        coef = (g / norm)[owner] * keep
+        out = {"loss": loss.detach(), "log_ratio": r.detach(), "margin": gap.detach()}
+    else:
+        a = s["adv"].double()
+        a = a[owner] if case["per_sequence"] else a
+        w = keep / (keep.sum().clamp(min=1) if case["aggregate"] == "token" else case["sequences"] * count.clamp(min=1)[owner])
+        leaf = logp.clone().requires_grad_()
+        rho = torch.exp(leaf - s["old"].double())
+        lo, hi = 1 - CLIP_LOW, 1 + CLIP_HIGH
+        surrogate = -(w * torch.min(rho * a, rho.clamp(lo, hi) * a)).sum()
+        q = s["ref"].double() - leaf
+        kl = (w * (q.exp() - 1 - q)).sum()
+        loss = surrogate + 0.05 * kl
+        coef, = torch.autograd.grad(loss, leaf)
+        hit = torch.where(a > 0, rho > hi, (a < 0) & (rho < lo))
+        out = {"loss": loss.detach(), "surrogate": surrogate.detach(), "kl": kl.detach(),
+               "clip_fraction": (w * hit).sum().detach(), "logp": logp}
+    d = torch.empty(T, V, device="cuda", dtype=torch.float64)
+    for p in pieces:
+        y = rows(p).exp_().neg_()
+        y.scatter_add_(1, ids[p].clamp(min=0)[:, None], torch.ones_like(ids[p], dtype=torch.float64)[:, None])
+        d[p] = y * (coef[p] * grad_scale(case))[:, None]
+    out["d_logits"] = d
+    return out
