@@ -292,7 +292,8 @@ def run(s):
             r = tk.preference_loss_and_grad(s["logits"], s["ids"], s["seq_ptr"], s["ref"], beta=0.1, label_smoothing=0.1,
                                             kind=c["kind"], average=c["average"], grad_scale=grad_scale(c))
             return {"loss": r.loss, "log_ratio": r.log_ratio, "margin": r.margin, "d_logits": r.d_logits}
-        r = tk.policy_loss_and_grad(s["logits"], s["ids"], s["seq_ptr"], s["adv"], s["old"], s["ref"], clip_low=CLIP_LOW,
+        r = tk.policy_loss_and_grad(s["logits"], s["ids"], s["seq_ptr"], s["adv"], s["old"], s["ref"],
+                                    advantage_per="sequence" if c["per_sequence"] else "token", clip_low=CLIP_LOW,
                                     clip_high=CLIP_HIGH, kl_coef=0.05, aggregate=c["aggregate"],
                                     grad_scale=grad_scale(c))
         return {"loss": r.loss, "surrogate": r.surrogate, "kl": r.kl, "clip_fraction": r.clip_fraction, "logp": r.logp,
