@@ -289,8 +289,9 @@ def run(s):
         if c["op"] == "logprob":
             return {"logp": tk.token_logprobs(s["logits"], s["ids"])}
         if c["op"] == "preference":
-            r = tk.preference_loss_and_grad(s["logits"], s["ids"], s["seq_ptr"], s["ref"], beta=0.1, label_smoothing=0.1,
-                                            kind=c["kind"], average=c["average"], grad_scale=grad_scale(c))
+            r = tk.preference_loss_and_grad(s["logits"], s["ids"], s["seq_ptr"], s["ref"], beta=0.1,
+                                            label_smoothing=0.1 if c["kind"] == "sigmoid" else 0.0, kind=c["kind"],
+                                            average=c["average"], grad_scale=grad_scale(c))
             return {"loss": r.loss, "log_ratio": r.log_ratio, "margin": r.margin, "d_logits": r.d_logits}
         r = tk.policy_loss_and_grad(s["logits"], s["ids"], s["seq_ptr"], s["adv"], s["old"], s["ref"],
                                     advantage_per="sequence" if c["per_sequence"] else "token", clip_low=CLIP_LOW,
