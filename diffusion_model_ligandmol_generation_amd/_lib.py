@@ -78,6 +78,36 @@ class LossArgs(C.Structure):
                 ("workspace", C.c_void_p)]
 
 
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2                 # enum ligdiff_dtype
+PREFERENCE_KINDS = {"sigmoid": 0, "ipo": 1}                # enum ligdiff_preference_kind
+POLICY_MEANS = {"token": 0, "sequence": 1}                 # enum ligdiff_policy_mean
+
+
+class TokenArgs(C.Structure):
+    """struct ligdiff_token_args"""
+    _fields_ = [("logits", C.c_void_p), ("tokens", C.c_void_p), ("row_stride", C.c_int64), ("n_tokens", C.c_int64),
+                ("vocab", C.c_int32), ("dtype", C.c_int32), ("token_bytes", C.c_int32), ("temperature", C.c_float)]
+
+
+class PreferenceArgs(C.Structure):
+    """struct ligdiff_preference_args"""
+    _fields_ = [("seq_ptr", C.c_void_p), ("ref_logp", C.c_void_p), ("n_pairs", C.c_int32), ("kind", C.c_int32),
+                ("average", C.c_int32), ("beta", C.c_float), ("label_smoothing", C.c_float), ("denominator", C.c_float),
+                ("grad_scale", C.c_float), ("loss", C.c_void_p), ("log_ratio", C.c_void_p), ("margin", C.c_void_p),
+                ("slope", C.c_void_p), ("stats", C.c_void_p), ("row_seq", C.c_void_p), ("d_logits", C.c_void_p),
+                ("d_stride", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class PolicyArgs(C.Structure):
+    """struct ligdiff_policy_args"""
+    _fields_ = [("seq_ptr", C.c_void_p), ("advantage", C.c_void_p), ("old_logp", C.c_void_p), ("ref_logp", C.c_void_p),
+                ("n_seq", C.c_int32), ("advantage_per_token", C.c_int32), ("aggregate", C.c_int32), ("clip_low", C.c_float),
+                ("clip_high", C.c_float), ("kl_coef", C.c_float), ("denominator", C.c_float), ("grad_scale", C.c_float),
+                ("result", C.c_void_p), ("logp", C.c_void_p), ("stats", C.c_void_p), ("coef", C.c_void_p),
+                ("d_logits", C.c_void_p), ("d_stride", C.c_int64), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
 # name -> (restype, argtypes); every symbol include/ligdiff.h declares
 SIGNATURES = {
     "ligdiff_version": (C.c_int, []),
@@ -177,6 +207,19 @@ SIGNATURES = {
                                          C.c_void_p, C.c_void_p]),
     "ligdiff_full_edges": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p]),
     "ligdiff_prediction_gate": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
+    "ligdiff_embed": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_void_p, C.c_int32, C.c_int64,
+                                C.c_float, C.c_void_p, C.c_int64, C.c_void_p]),
+    "ligdiff_embed_grad_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int32]),
+    "ligdiff_embed_grad": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int32,
+                                     C.c_float, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_size_t,
+                                     C.c_void_p]),
+    "ligdiff_token_logprob": (C.c_int, [C.POINTER(TokenArgs), C.c_void_p, C.c_void_p, C.c_void_p]),
+    "ligdiff_token_logprob_grad": (C.c_int, [C.POINTER(TokenArgs), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_float,
+                                             C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "ligdiff_preference_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32]),
+    "ligdiff_preference_loss": (C.c_int, [C.POINTER(TokenArgs), C.POINTER(PreferenceArgs), C.c_void_p]),
+    "ligdiff_policy_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32, C.c_int32]),
+    "ligdiff_policy_loss": (C.c_int, [C.POINTER(TokenArgs), C.POINTER(PolicyArgs), C.c_void_p]),
     "ligdiff_validity_gate": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]),
 }
 

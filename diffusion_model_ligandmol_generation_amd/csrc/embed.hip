@@ -1,0 +1,475 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens.
+//   out[i, :] = scale W[tok_i, :]                       d_W[v, :] = scale sum_{i: tok_i = v} d_out[i, :]
+// Both are bound by HBM.  The gradient sorts the token positions (a stable radix sort of 8-byte records, small against the
+// rows) and then sums rows of equal tokens: every row of d_out is read once, in 32 bits and in a fixed order, no float
+// atomics, so the result does not change from run to run.  The tokens of a batch are very uneven (half of a ligand's atoms are
+// carbon), so the sorted positions are cut into chunks of equal length whatever the tokens are; a token whose positions
+// lie in several chunks leaves one partial row in each, and a second launch joins them.
+#include "embed.h"
+
+// ------------------------------------------------------------------ lookup
+// TPR lanes a row, four rows in flight per group: the token, then the row, then the store are dependent accesses.
+template <typename T, int TPR>
+__global__ __launch_bounds__(256) void k_embed(const T* __restrict__ table, int64_t row_stride, TokenView tok, int64_t n, int32_t D,
+                                               float scale, T* __restrict__ out, int64_t out_stride) {
+  constexpr int N = Pack<T>::N, RPB = 256 / TPR, RU = 4;
+  const int r = threadIdx.x % TPR, nb = D / N, tail = D - nb * N;
+  for (int64_t t0 = ((int64_t)blockIdx.x * RPB + threadIdx.x / TPR) * RU; t0 < n; t0 += (int64_t)gridDim.x * RPB * RU) {
+    int id[RU];
+#pragma unroll
+    for (int u = 0; u < RU; ++u) id[u] = t0 + u < n ? tok.at(t0 + u) : -1;
+    for (int i = r; i < nb; i += TPR) {
+      float v[RU][N];
+#pragma unroll
+      for (int u = 0; u < RU; ++u) {
+        if (id[u] >= 0) load_pack(table + id[u] * row_stride + (int64_t)i * N, v[u]);
+        else
+#pragma unroll
+          for (int j = 0; j < N; ++j) v[u][j] = 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < RU; ++u)
+        if (t0 + u < n) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) v[u][j] = id[u] >= 0 ? v[u][j] * scale : 0.f;
+          store_pack(out + (t0 + u) * out_stride + (int64_t)i * N, v[u]);
+        }
+    }
+    if (r < tail)
+#pragma unroll
+      for (int u = 0; u < RU; ++u)
+        if (t0 + u < n)
+          out[(t0 + u) * out_stride + nb * N + r] = id[u] >= 0 ? (T)((float)table[id[u] * row_stride + nb * N + r] * scale) : (T)0.f;
+  }
+}
+
+template <typename T>
+static void launch_embed(const void* table, int64_t row_stride, TokenView tok, int64_t n, int32_t D, float scale, void* out,
+                         int64_t out_stride, hipStream_t s) {
+  const int packs = D / Pack<T>::N;
+#define LAUNCH_EMBED(TPR)                                                                                                 \
+  do {                                                                                                                    \
+    const int64_t blocks = (n + 4 * (256 / TPR) - 1) / (4 * (256 / TPR));                                                 \
+    hipLaunchKernelGGL((k_embed<T, TPR>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, (const T*)table, \
+                       row_stride, tok, n, D, scale, (T*)out, out_stride);                                                \
+  } while (0)
+  if (packs <= 8) LAUNCH_EMBED(8);
+  else if (packs <= 16) LAUNCH_EMBED(16);
+  else if (packs <= 32) LAUNCH_EMBED(32);
+  else LAUNCH_EMBED(64);
+}
+
+static bool bad_embed(int dtype, int64_t n_rows, int32_t width, int token_bytes, int64_t n) {
+  return dtype < LIGDIFF_F32 || dtype > LIGDIFF_F16 || n_rows < 1 || n_rows > 0x7ffffffeLL || width < 1 ||
+         (token_bytes != 4 && token_bytes != 8) || n < 0 || n > 0x7fffffffLL;
+}
+
+extern "C" int ligdiff_embed(const void* table, int32_t dtype, int64_t n_rows, int32_t width, int64_t row_stride,
+                             const void* tokens, int32_t token_bytes, int64_t n_tokens, float scale, void* out,
+                             int64_t out_stride, void* stream) {
+  if (bad_embed(dtype, n_rows, width, token_bytes, n_tokens) || row_stride < width || out_stride < width || !table)
+    return LIGDIFF_ERR_ARG;
+  if (n_tokens == 0) return LIGDIFF_OK;
+  if (!tokens || !out) return LIGDIFF_ERR_ARG;
+  const TokenView tok{tokens, token_bytes, (int32_t)n_rows};
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == LIGDIFF_F32) launch_embed<float>(table, row_stride, tok, n_tokens, width, scale, out, out_stride, s);
+  else if (dtype == LIGDIFF_BF16) launch_embed<bf16_t>(table, row_stride, tok, n_tokens, width, scale, out, out_stride, s);
+  else launch_embed<f16_t>(table, row_stride, tok, n_tokens, width, scale, out, out_stride, s);
+  LD_CHECK_LAUNCH();
+  return LIGDIFF_OK;
+}
+
+// ------------------------------------------------------------------ stable radix sort of the positions by token
+#define SORT_NT 512
+#define SORT_WAVES (SORT_NT / 64)
+struct SortPass {
+  TokenView tok;                       // first pass: the key of position i is its token, tok.n_rows for tokens outside
+  const uint32_t* key_in; const int32_t* pos_in;   // later passes
+  uint32_t* key_out; int32_t* pos_out;
+  int64_t n;
+  int32_t shift, per_block;            // per_block: a multiple of SORT_NT
+  int32_t* hist;                       // [blocks][bins]
+  int32_t* row_ptr; int32_t rows;      // one-pass sorts: block 0 writes the first position of every token, [rows + 1]
+};
+template <bool FIRST> __device__ __forceinline__ uint32_t sort_key(const SortPass& a, int64_t i) {
+  if (!FIRST) return a.key_in[i];
+  const int id = a.tok.at(i);
+  return id < 0 ? (uint32_t)a.tok.n_rows : (uint32_t)id;
+}
+template <int BITS, bool FIRST>
+__global__ __launch_bounds__(SORT_NT) void k_sort_count(SortPass a) {
+  constexpr int NB = 1 << BITS;
+  __shared__ int cnt[NB];
+  for (int d = threadIdx.x; d < NB; d += SORT_NT) cnt[d] = 0;
+  __syncthreads();
+  const int64_t b0 = (int64_t)blockIdx.x * a.per_block;
+  for (int k = threadIdx.x; k < a.per_block; k += SORT_NT)
+    if (b0 + k < a.n) atomicAdd(&cnt[(sort_key<FIRST>(a, b0 + k) >> a.shift) & (NB - 1)], 1);
+  __syncthreads();
+  for (int d = threadIdx.x; d < NB; d += SORT_NT) a.hist[(int64_t)blockIdx.x * NB + d] = cnt[d];
+}
+// Each block finds its own offsets from the count table (no scan launch): total and preceding blocks' counts of every digit,
+// a prefix sum over the digits, then one over its waves; a wave ranks 64 positions at a time by the lanes that hold the
+// same digit, so positions of equal digits keep their order.
+template <int BITS, bool FIRST>
+__global__ __launch_bounds__(SORT_NT) void k_sort_scatter(SortPass a) {
+  constexpr int NB = 1 << BITS, K = NB > SORT_NT ? NB / SORT_NT : 1, LIVE = NB / K;
+  __shared__ int cnt[SORT_WAVES][NB];
+  __shared__ int wtot[SORT_WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int i = tid; i < SORT_WAVES * NB; i += SORT_NT) (&cnt[0][0])[i] = 0;
+  int total[K] = {}, before[K] = {};
+  if (tid < LIVE) {
+#pragma unroll 8
+    for (int b = 0; b < (int)gridDim.x; ++b)
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int h = a.hist[(int64_t)b * NB + tid * K + k];
+        total[k] += h;
+        before[k] += b < (int)blockIdx.x ? h : 0;
+      }
+  }
+  int own = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) own += total[k];
+  int scan = own;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(scan, o);
+    if (lane >= o) scan += u;
+  }
+  if (lane == 63) wtot[wave] = scan;
+  __syncthreads();
+  int excl = scan - own;
+  for (int w = 0; w < wave; ++w) excl += wtot[w];
+  // counts of this block's waves
+  const int64_t w0 = (int64_t)blockIdx.x * a.per_block + (int64_t)wave * (a.per_block / SORT_WAVES);
+  for (int k = lane; k < a.per_block / SORT_WAVES; k += 64)
+    if (w0 + k < a.n) atomicAdd(&cnt[wave][(sort_key<FIRST>(a, w0 + k) >> a.shift) & (NB - 1)], 1);
+  __syncthreads();
+  if (tid < LIVE) {
+    int start = excl;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int d = tid * K + k;
+      if (a.row_ptr && blockIdx.x == 0 && d <= a.rows) a.row_ptr[d] = start;
+      int run = start + before[k];
+      for (int w = 0; w < SORT_WAVES; ++w) {
+        const int c = cnt[w][d];
+        cnt[w][d] = run;
+        run += c;
+      }
+      start += total[k];
+    }
+  }
+  __syncthreads();
+  for (int k = 0; k < a.per_block / SORT_WAVES; k += 64) {
+    const int64_t i = w0 + k + lane;
+    const bool on = i < a.n;
+    uint32_t key = 0;
+    int32_t pos = 0;
+    if (on) { key = sort_key<FIRST>(a, i); pos = FIRST ? (int32_t)i : a.pos_in[i]; }
+    const int d = (int)(key >> a.shift) & (NB - 1);
+    uint64_t same = __ballot(on);
+    if (same == 0) break;
+#pragma unroll
+    for (int b = 0; b < BITS; ++b) {
+      const uint64_t set = __ballot((d >> b) & 1);
+      same &= (d >> b) & 1 ? set : ~set;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1));
+    int at = 0;
+    if (on) at = cnt[wave][d];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (on && rank == 0) cnt[wave][d] = at + __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (on) {
+      a.key_out[at + rank] = key;
+      a.pos_out[at + rank] = pos;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ sums of rows of equal tokens
+struct SegIn {
+  const void* d_out; int64_t d_stride;
+  const uint32_t* key; const int32_t* pos;   // sorted
+  int64_t n;
+  int32_t* row_ptr; bool have_ptr;
+  int32_t rows, D, R, n_chunks, n_tiles;
+  float scale;
+  float* part;                               // [n_chunks][2][D]
+  void* d_table; int64_t t_stride;
+  bool accumulate;
+  int32_t zero_blocks;
+};
+#define ZERO_ROWS 64   // rows of the table a block of the first part looks after
+
+template <typename TO> __device__ __forceinline__ void put(TO* p, float v, bool add) { *p = (TO)(add ? (float)*p + v : v); }
+// the first `live` of N columns
+template <typename TO, int N> __device__ __forceinline__ void put_columns(TO* p, const float (&v)[N], float scale, int live, bool add) {
+  if (live == N && !add) {
+    typedef TO Raw __attribute__((ext_vector_type(N), aligned(sizeof(TO))));
+    Raw r;
+#pragma unroll
+    for (int j = 0; j < N; ++j) r[j] = (TO)(v[j] * scale);
+    *reinterpret_cast<Raw*>(p) = r;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (j < live) put(p + j, v[j] * scale, add);
+}
+
+// Blocks [0, zero_blocks): find where each token's positions start (bisection, unless the sort wrote it) and write the rows
+// of tokens that do not occur.  The other blocks: one wave a chunk of R sorted positions and 64 packs of columns.
+template <typename T, typename TO>
+__global__ __launch_bounds__(256) void k_segment_sums(SegIn a) {
+  constexpr int N = Pack<T>::N, U = 8;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if ((int)blockIdx.x < a.zero_blocks) {
+    __shared__ int ptr[ZERO_ROWS + 1];
+    const int v0 = blockIdx.x * ZERO_ROWS;
+    for (int k = threadIdx.x; k <= ZERO_ROWS; k += 256) {
+      const int64_t v = (int64_t)v0 + k;
+      if (v > a.rows) continue;
+      int p;
+      if (a.have_ptr) p = a.row_ptr[v];
+      else {
+        int64_t lo = 0, hi = a.n;   // the number of keys below v
+        while (lo < hi) {
+          const int64_t mid = (lo + hi) >> 1;
+          if ((int64_t)a.key[mid] < v) lo = mid + 1; else hi = mid;
+        }
+        p = (int)lo;
+        if (k < ZERO_ROWS || v == a.rows) a.row_ptr[v] = p;
+      }
+      ptr[k] = p;
+    }
+    __syncthreads();
+    if (a.accumulate) return;
+    for (int k = wave; k < ZERO_ROWS && v0 + k < a.rows; k += 4) {
+      if (ptr[k + 1] != ptr[k]) continue;
+      TO* row = reinterpret_cast<TO*>(a.d_table) + (int64_t)(v0 + k) * a.t_stride;
+      constexpr int M = Pack<TO>::N;
+      const float z[M] = {};
+      const int nb = a.D / M;
+      for (int i = lane; i < nb; i += 64) store_pack(row + (int64_t)i * M, z);
+      if (lane < a.D - nb * M) row[nb * M + lane] = (TO)0.f;
+    }
+    return;
+  }
+  const int64_t unit = (int64_t)(blockIdx.x - a.zero_blocks) * 4 + wave;
+  const int chunk = (int)(unit / a.n_tiles), tile = (int)(unit % a.n_tiles);
+  if (chunk >= a.n_chunks) return;
+  const int64_t c0 = (int64_t)chunk * a.R;
+  const int rows = (int)(a.n - c0 < a.R ? a.n - c0 : a.R);
+  const int col = tile * 64 * N + lane * N;
+  const int live = a.D - col < 0 ? 0 : a.D - col < N ? a.D - col : N;   // columns of this lane
+  const uint32_t limit = (uint32_t)a.rows;
+  uint32_t cur = a.key[c0];
+  if (cur >= limit) return;
+  const bool head_open = c0 > 0 && a.key[c0 - 1] == cur;
+  const bool tail_open = c0 + rows < a.n && a.key[c0 + rows] == a.key[c0 + rows - 1];
+  float acc[N] = {};
+  bool first = true;
+  const auto flush = [&](bool open) {
+    if (open) {
+      put_columns<float, N>(a.part + ((int64_t)chunk * 2 + (first ? 0 : 1)) * a.D + col, acc, 1.0f, live, false);
+    } else {
+      put_columns<TO, N>(reinterpret_cast<TO*>(a.d_table) + (int64_t)cur * a.t_stride + col, acc, a.scale, live, a.accumulate);
+    }
+  };
+  const T* base = reinterpret_cast<const T*>(a.d_out) + col;
+  bool done = false;
+  for (int b = 0; b < rows && !done; b += 64) {
+    const int left = rows - b < 64 ? rows - b : 64;
+    uint32_t kv = 0xffffffffu;
+    int32_t pv = 0;
+    if (lane < left) { kv = a.key[c0 + b + lane]; pv = a.pos[c0 + b + lane]; }
+    for (int g = 0; g < left && !done; g += U) {
+      float v[U][N];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (g + u >= left) continue;
+        const int64_t p = __builtin_amdgcn_readlane(pv, g + u);
+        if (live == N) load_pack(base + p * a.d_stride, v[u]);
+        else
+#pragma unroll
+          for (int j = 0; j < N; ++j) v[u][j] = j < live ? (float)base[p * a.d_stride + j] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (g + u >= left || done) continue;
+        const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)kv, g + u);
+        if (key != cur) {
+          flush(first && head_open);
+          first = false;
+          cur = key;
+#pragma unroll
+          for (int j = 0; j < N; ++j) acc[j] = 0.f;
+          if (key >= limit) { done = true; continue; }   // tokens without a row are sorted last
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += v[u][j];
+      }
+    }
+  }
+  if (!done) flush((first && head_open) || tail_open);
+}
+
+#define JOIN_WAVES 8
+// One block a chunk and tile; it joins the partial rows of the token that starts in this chunk and goes on in the next.
+template <typename TO>
+__global__ __launch_bounds__(JOIN_WAVES * 64) void k_segment_join(SegIn a) {
+  const int chunk = blockIdx.x / a.n_tiles, tile = blockIdx.x % a.n_tiles;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c0 = (int64_t)chunk * a.R;
+  const int64_t end = a.n - c0 < a.R ? a.n : c0 + a.R;
+  const uint32_t key = a.key[end - 1];
+  if (key >= (uint32_t)a.rows) return;
+  const int s = a.row_ptr[key], e = a.row_ptr[key + 1];
+  if (s < c0 || e <= end) return;
+  const int last = (e - 1) / a.R, count = last - chunk + 1;
+  const int slot = s == c0 ? 0 : 1;
+  __shared__ float sh[JOIN_WAVES][4][64];
+  // 256 columns a block: 64 lanes x 4
+  const int col = tile * 256 + lane * 4;
+  const int live = a.D - col < 0 ? 0 : a.D - col < 4 ? a.D - col : 4;
+  float acc[4] = {};
+  if (live > 0)
+#pragma unroll 8
+    for (int k = wave; k < count; k += JOIN_WAVES) {
+      const float* p = a.part + ((int64_t)(chunk + k) * 2 + (k == 0 ? slot : 0)) * a.D + col;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] += j < live ? p[j] : 0.f;
+    }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sh[wave][j][lane] = acc[j];
+  __syncthreads();
+  if (wave != 0) return;
+  TO* out = reinterpret_cast<TO*>(a.d_table) + (int64_t)key * a.t_stride + col;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float v = sh[0][j][lane];
+#pragma unroll
+    for (int w = 1; w < JOIN_WAVES; ++w) v += sh[w][j][lane];
+    if (j < live) put(out + j, v * a.scale, a.accumulate);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+// Sort: one pass of 8 bits for up to 255 rows (the token outside is one more key), else passes of 11 bits.
+static int sort_bits(int32_t n_rows) { return n_rows < 256 ? 8 : 11; }
+static int sort_passes(int32_t n_rows, int bits) {
+  int p = 1;
+  while (p * bits < 31 && (n_rows >> (p * bits)) != 0) ++p;
+  return p;
+}
+// Blocks of a sort pass: 1024 positions or more each; every block reads the whole count table, so there are at most 64 blocks
+// with 2048 bins and 512 with 256.
+static int sort_per_block(int64_t n, int bits) {
+  const int64_t most = bits == 8 ? 512 : 64;
+  const int64_t per = (n + most - 1) / most;
+  return (int)((per < 1024 ? 1024 : per + SORT_NT - 1) / SORT_NT * SORT_NT);
+}
+// Positions of a chunk: about 4096 waves over the chip, at least 16 positions (a chunk leaves up to one partial row).
+static int chunk_rows(int64_t n, int tiles) {
+  int r = 16;
+  while (r < 512 && n * tiles > (int64_t)r * 4096) r *= 2;
+  return r;
+}
+struct EmbedWs { uint32_t* key[2]; int32_t* pos[2]; int32_t* hist; int32_t* row_ptr; float* part; size_t bytes; };
+static EmbedWs embed_ws(void* base, int64_t n, int32_t rows, int32_t width) {
+  char* p = (char*)base;
+  size_t used = 0;
+  const auto take = [&](size_t bytes) { char* r = p + used; used += align_up(bytes, 256); return r; };
+  EmbedWs w;
+  for (int k = 0; k < 2; ++k) { w.key[k] = (uint32_t*)take((size_t)n * 4); w.pos[k] = (int32_t*)take((size_t)n * 4); }
+  const int bits = sort_bits(rows);
+  const int64_t blocks = n ? (n + sort_per_block(n, bits) - 1) / sort_per_block(n, bits) : 0;
+  w.hist = (int32_t*)take((size_t)blocks * (1 << bits) * 4);
+  w.row_ptr = (int32_t*)take(((size_t)rows + 1) * 4);
+  // (half-precision tiles are the widest: fewest tiles, shortest chunks, most partial rows)
+  const int64_t r = chunk_rows(n, (width + 511) / 512);
+  w.part = (float*)take((size_t)((n + r - 1) / r) * 2 * (size_t)width * 4);
+  w.bytes = used;
+  return w;
+}
+size_t embed_grad_workspace(int64_t n, int32_t rows, int32_t width) { return embed_ws(nullptr, n, rows, width).bytes; }
+
+template <int BITS> static int sort_tokens(const EmbedGrad& g, const EmbedWs& w, hipStream_t s) {
+  SortPass a;
+  a.tok = g.tok; a.n = g.n; a.per_block = sort_per_block(g.n, BITS); a.hist = w.hist; a.rows = g.rows;
+  const int blocks = (int)((g.n + a.per_block - 1) / a.per_block);
+  const int passes = sort_passes(g.tok.n_rows, BITS);
+  for (int p = 0; p < passes; ++p) {
+    a.shift = p * BITS;
+    a.key_in = w.key[(p + 1) & 1]; a.pos_in = w.pos[(p + 1) & 1];
+    a.key_out = w.key[p & 1]; a.pos_out = w.pos[p & 1];
+    a.row_ptr = passes == 1 && g.rows < (1 << BITS) ? w.row_ptr : nullptr;
+    if (p == 0) {
+      hipLaunchKernelGGL((k_sort_count<BITS, true>), dim3(blocks), dim3(SORT_NT), 0, s, a);
+      hipLaunchKernelGGL((k_sort_scatter<BITS, true>), dim3(blocks), dim3(SORT_NT), 0, s, a);
+    } else {
+      hipLaunchKernelGGL((k_sort_count<BITS, false>), dim3(blocks), dim3(SORT_NT), 0, s, a);
+      hipLaunchKernelGGL((k_sort_scatter<BITS, false>), dim3(blocks), dim3(SORT_NT), 0, s, a);
+    }
+  }
+  return passes;
+}
+
+template <typename T, typename TO> static void segment_sums(SegIn a, hipStream_t s) {
+  a.n_tiles = (a.D + 64 * Pack<T>::N - 1) / (64 * Pack<T>::N);
+  a.R = chunk_rows(a.n, a.n_tiles);
+  a.n_chunks = (int)((a.n + a.R - 1) / a.R);
+  a.zero_blocks = (a.rows + ZERO_ROWS - 1) / ZERO_ROWS;
+  const int64_t waves = (int64_t)a.n_chunks * a.n_tiles;
+  hipLaunchKernelGGL((k_segment_sums<T, TO>), dim3((unsigned)(a.zero_blocks + (waves + 3) / 4)), dim3(256), 0, s, a);
+  if (a.n_chunks > 1) {
+    SegIn j = a;
+    j.n_tiles = (a.D + 255) / 256;
+    hipLaunchKernelGGL((k_segment_join<TO>), dim3((unsigned)((int64_t)j.n_chunks * j.n_tiles)), dim3(JOIN_WAVES * 64), 0, s, j);
+  }
+}
+
+void embed_grad(const EmbedGrad& g, void* workspace, hipStream_t s) {
+  const EmbedWs w = embed_ws(workspace, g.n, g.rows, g.width);
+  SegIn a;
+  a.have_ptr = false;
+  int passes = 1;
+  if (g.n > 0) {
+    const int bits = sort_bits(g.rows);
+    passes = bits == 8 ? sort_tokens<8>(g, w, s) : sort_tokens<11>(g, w, s);
+    a.have_ptr = passes == 1 && g.rows < (1 << bits);
+  }
+  a.d_out = g.d_out; a.d_stride = g.d_stride; a.key = w.key[(passes - 1) & 1]; a.pos = w.pos[(passes - 1) & 1]; a.n = g.n;
+  a.row_ptr = w.row_ptr; a.rows = g.rows; a.D = g.width; a.scale = g.scale; a.part = w.part;
+  a.d_table = g.d_table; a.t_stride = g.t_stride; a.accumulate = g.accumulate;
+  const bool wide = g.grad_dtype == LIGDIFF_F32;
+  if (g.dtype == LIGDIFF_F32) segment_sums<float, float>(a, s);
+  else if (g.dtype == LIGDIFF_BF16) { if (wide) segment_sums<bf16_t, float>(a, s); else segment_sums<bf16_t, bf16_t>(a, s); }
+  else { if (wide) segment_sums<f16_t, float>(a, s); else segment_sums<f16_t, f16_t>(a, s); }
+}
+
+extern "C" size_t ligdiff_embed_grad_workspace_bytes(int64_t n_tokens, int64_t n_rows, int32_t width) {
+  if (bad_embed(LIGDIFF_F32, n_rows, width, 4, n_tokens)) return 0;
+  return embed_grad_workspace(n_tokens, (int32_t)n_rows, width);
+}
+
+extern "C" int ligdiff_embed_grad(const void* d_out, int32_t dtype, int64_t d_stride, const void* tokens, int32_t token_bytes,
+                                  int64_t n_tokens, int64_t n_rows, int32_t width, float scale, void* d_table,
+                                  int32_t grad_dtype, int64_t table_stride, int32_t accumulate, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  if (bad_embed(dtype, n_rows, width, token_bytes, n_tokens) || (grad_dtype != dtype && grad_dtype != LIGDIFF_F32) ||
+      d_stride < width || table_stride < width || !d_table || !workspace)
+    return LIGDIFF_ERR_ARG;
+  if (n_tokens > 0 && (!d_out || !tokens)) return LIGDIFF_ERR_ARG;
+  if (workspace_bytes < embed_grad_workspace(n_tokens, (int32_t)n_rows, width)) return LIGDIFF_ERR_WORKSPACE;
+  EmbedGrad g{d_out, dtype, d_stride, TokenView{tokens, token_bytes, (int32_t)n_rows}, n_tokens, (int32_t)n_rows, width, scale,
+              d_table, grad_dtype, table_stride, accumulate != 0};
+  embed_grad(g, workspace, (hipStream_t)stream);
+  LD_CHECK_LAUNCH();
+  return LIGDIFF_OK;
+}

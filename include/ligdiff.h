@@ -580,6 +580,121 @@ int ligdiff_prediction_gate(const float* eps_x, const float* eps_pos, const int3
 int ligdiff_validity_gate(const float* x, const float* pos, const int32_t* mol_ptr, int32_t n_mols,
                           int32_t* accept, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Ids and the log-probabilities a network gives them: atom types (the 119 classes of atom_pred, of which
+ * model1.py:991-997 takes the types and generation.py:162-233 the softmax) or the tokens of any vocabulary.
+ * Embedding lookup and its gradient, log-probabilities of chosen ids, and two losses on them for fine-tuning: on
+ * pairs of molecules of which one is preferred, and on rewards (clipped policy loss with a KL term).  No counterpart
+ * in the reference, which takes one-hot types and has no loss on atom_pred's distribution.
+ * Ids are int32 or int64 (token_bytes 4 or 8).  An id outside [0, vocab) is an ignored position (padding), not an
+ * error: it looks up a row of zeros, has log-probability 0 and takes no part in a loss or gradient.  Sums, softmax
+ * statistics and gradients are formed in 32 bits or more and rounded once to the element type.  Nothing is accumulated
+ * by atomics: results do not change from run to run.
+ * ------------------------------------------------------------------------------- */
+enum ligdiff_dtype { LIGDIFF_F32 = 0, LIGDIFF_BF16 = 1, LIGDIFF_F16 = 2 };
+
+/* out[i, :] = scale * table[tokens[i], :].  table [n_rows, width] and out [n_tokens, width] of `dtype`, rows
+ * row_stride / out_stride elements apart (>= width, any alignment). */
+int ligdiff_embed(const void* table, int32_t dtype, int64_t n_rows, int32_t width, int64_t row_stride,
+                  const void* tokens, int32_t token_bytes, int64_t n_tokens, float scale, void* out,
+                  int64_t out_stride, void* stream);
+
+/* d_table[v, :] = scale * sum of d_out[i, :] over the positions with tokens[i] == v, zeros where there is none (with
+ * accumulate != 0 the sums are added to d_table and other rows left alone).  The positions are sorted by token (stably)
+ * and summed in that order in 32 bits.  grad_dtype: dtype or LIGDIFF_F32. */
+size_t ligdiff_embed_grad_workspace_bytes(int64_t n_tokens, int64_t n_rows, int32_t width);
+int ligdiff_embed_grad(const void* d_out, int32_t dtype, int64_t d_stride, const void* tokens, int32_t token_bytes,
+                       int64_t n_tokens, int64_t n_rows, int32_t width, float scale, void* d_table,
+                       int32_t grad_dtype, int64_t table_stride, int32_t accumulate, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+typedef struct ligdiff_token_args {
+  const void* logits;       /* [n_tokens, vocab] of dtype, rows row_stride elements apart   */
+  const void* tokens;       /* [n_tokens] chosen ids                                        */
+  int64_t row_stride;
+  int64_t n_tokens;         /* < 2^31                                                       */
+  int32_t vocab;
+  int32_t dtype;
+  int32_t token_bytes;
+  float temperature;        /* > 0: the distribution is softmax(logits / temperature)       */
+} ligdiff_token_args;
+
+/* logp [n_tokens] = log softmax(logits / temperature)[t, tokens[t]].  stats (may be NULL) [n_tokens, 2]: what the gradient
+ * needs of a row, its maximum and 1 / sum.  An id whose logit is -inf has logp -inf; a row of -inf only has no
+ * distribution: logp -inf and no gradient. */
+int ligdiff_token_logprob(const ligdiff_token_args* args, float* logp, float* stats, void* stream);
+
+/* d_logits[t, v] = c_t * mult * (*upstream) / temperature * ((v == tokens[t]) - p[t, v]), stats from the forward call.
+ * c_t = coef[t], or coef[coef_index[t]] when an index is given (entries outside [0, n_coef): 0).  upstream: device
+ * float or NULL (1).  Rows with c_t == 0 are written as zeros without being read. */
+int ligdiff_token_logprob_grad(const ligdiff_token_args* args, const float* stats, const float* coef,
+                               const int32_t* coef_index, int64_t n_coef, float mult, const float* upstream,
+                               void* d_logits, int64_t d_stride, void* stream);
+
+/* Preference loss over pairs of sequences (molecules): sequence p of the batch is preferred over sequence n_pairs + p.
+ *   r_s = sum over sequence s of (logp_t - ref_logp_t)   (divided by its number of positions with average != 0)
+ *   d_p = r_p - r_{n_pairs + p}
+ *   sigmoid: -(1 - e) log sigmoid(beta d) - e log sigmoid(-beta d)  (e = label_smoothing);  ipo: (d - 1 / (2 beta))^2
+ *   loss = sum over pairs / denominator
+ * seq_ptr [2 n_pairs + 1] int32, ascending, first position of each sequence (mol_ptr of a packed batch); a sequence may
+ * be empty (r = 0); positions outside every sequence take no part. */
+enum ligdiff_preference_kind { LIGDIFF_PREFERENCE_SIGMOID = 0, LIGDIFF_PREFERENCE_IPO = 1 };
+typedef struct ligdiff_preference_args {
+  const int32_t* seq_ptr;
+  const float* ref_logp;    /* [n_tokens] log-probabilities under the reference, or NULL (0) */
+  int32_t n_pairs;
+  int32_t kind;
+  int32_t average;
+  float beta;               /* > 0                                                           */
+  float label_smoothing;    /* [0, 0.5)                                                      */
+  float denominator;        /* <= 0: n_pairs; data parallel: the pairs of all ranks          */
+  float grad_scale;         /* factor of the gradient (loss scaling)                         */
+  float* loss;              /* [1]                                                           */
+  float* log_ratio;         /* [2 n_pairs] r_s                                               */
+  float* margin;            /* [n_pairs] d_p                                                 */
+  float* slope;             /* [2 n_pairs] grad_scale * d loss / d logp of a sequence's rows */
+  float* stats;             /* [n_tokens, 2]                                                 */
+  int32_t* row_seq;         /* [n_tokens] sequence of each position, -1: takes no part       */
+  void* d_logits;           /* [n_tokens, vocab] of dtype, or NULL: later, by                */
+  int64_t d_stride;         /* ligdiff_token_logprob_grad(stats, slope, row_seq, 2 n_pairs)  */
+  void* workspace;
+  size_t workspace_bytes;
+} ligdiff_preference_args;
+size_t ligdiff_preference_workspace_bytes(int64_t n_tokens, int32_t n_pairs);
+int ligdiff_preference_loss(const ligdiff_token_args* args, const ligdiff_preference_args* q, void* stream);
+
+/* Clipped policy loss with a KL term: with rho = exp(logp_t - old_logp_t), A the advantage of position t (or of its
+ * sequence) and k = ref_logp_t - logp_t,
+ *   l_t = -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(k) - k - 1)
+ * token mean: sum of l_t / number of positions that take part; sequence mean: mean over the sequences (empty ones count) of
+ * the mean over their positions.  denominator > 0 takes the place of the number of positions / sequences.  The loss and the
+ * gradient of the logits come from one pass over them. */
+enum ligdiff_policy_mean { LIGDIFF_POLICY_TOKEN_MEAN = 0, LIGDIFF_POLICY_SEQUENCE_MEAN = 1 };
+typedef struct ligdiff_policy_args {
+  const int32_t* seq_ptr;   /* [n_seq + 1] ascending, or NULL: one sequence (n_seq = 1)      */
+  const float* advantage;   /* [n_seq], or [n_tokens] with advantage_per_token               */
+  const float* old_logp;    /* [n_tokens], or NULL: the policy itself (rho = 1)              */
+  const float* ref_logp;    /* [n_tokens], or NULL: no KL term                               */
+  int32_t n_seq;
+  int32_t advantage_per_token;
+  int32_t aggregate;
+  float clip_low;           /* [0, 1]                                                        */
+  float clip_high;          /* >= 0                                                          */
+  float kl_coef;            /* >= 0                                                          */
+  float denominator;
+  float grad_scale;
+  float* result;            /* [4] loss, -min term, KL term, share of clipped positions      */
+  float* logp;              /* [n_tokens] or NULL                                            */
+  float* stats;             /* [n_tokens, 2] or NULL                                         */
+  float* coef;              /* [n_tokens] d loss / d logp_t or NULL: with stats, for a later */
+  void* d_logits;           /* gradient; d_logits [n_tokens, vocab] or NULL                  */
+  int64_t d_stride;
+  void* workspace;
+  size_t workspace_bytes;
+} ligdiff_policy_args;
+size_t ligdiff_policy_workspace_bytes(int64_t n_tokens, int32_t n_seq, int32_t aggregate);
+int ligdiff_policy_loss(const ligdiff_token_args* args, const ligdiff_policy_args* q, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

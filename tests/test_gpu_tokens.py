@@ -1,0 +1,582 @@
+"""GPU: the token operators against plain 64-bit implementations.
+
+Tolerances, fixed before the first run.  u = 2^-24 is half a step of fp32.
+* A sum of n fp32 terms in any order is off by at most (n - 1) u sum |term|.
+* logp = (x_t - m) - log S: an exponential exp2(c (x - m)) is off by u (|c (x - m)| ln 2 + 4) relative (argument rounded
+  twice, instruction good to one step), which weighted by the probabilities is at most 2 u (log V + 4); the sum over at
+  most 64 + 40 serial adds per lane and tree adds 104 u.  With V <= 2^17: (2 * 16 + 104) u = 136 u, call it LOGP = 9e-6;
+  the fp32 output adds u |logp|.
+* d = g ([v = id] - p): p carries the relative error of the same exponentials and of the sum, 2 LOGP of g p in all; g of
+  the policy loss carries exp(logp - old), LOGP + 4 u relative; the result is rounded to its type (half a step, eps / 2,
+  and half the smallest subnormal of fp16)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+LOGP = 9e-6
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def tk():
+    from diffusion_model_ligandmol_generation_amd import tokens
+    return tokens
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def half_step(t):
+    """Half a step of the type relative, and half its smallest subnormal."""
+    return torch.finfo(t).eps / 2, {torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126}[t]
+
+
+def within(got, want, slack, what):
+    """|got - want| <= half a step of got's type + slack (a number or a tensor); equal infinities and NaNs agree."""
+    rel, sub = half_step(got.dtype)
+    got, want = got.double(), want.double()
+    ok = (got == want) | (got.isnan() & want.isnan()) | ((got - want).abs() <= rel * 1.01 * want.abs() + sub + slack)
+    assert bool(ok.all()), (what, int((~ok).sum()), float((got - want).abs().nan_to_num().max()))
+
+
+def ids_of(T, V, g, ignored=0.0, dtype=torch.int64):
+    ids = torch.randint(0, V, (T,), device="cuda", generator=g)
+    if ignored:
+        off = torch.rand(T, device="cuda", generator=g) < ignored
+        bad = torch.tensor([-1, -100, V, V + 7], device="cuda")[torch.randint(0, 4, (T,), device="cuda", generator=g)]
+        ids = torch.where(off, bad, ids)
+    return ids.to(dtype)
+
+
+def strided(t, pad, lead=0):
+    """The same rows, ``pad`` elements apart more and ``lead`` elements into a larger buffer: (view, buffer)."""
+    buf = torch.full((t.shape[0], t.shape[1] + pad), 7.0, dtype=t.dtype, device=t.device)
+    view = buf[:, lead:lead + t.shape[1]]
+    view.copy_(t)
+    return view, buf
+
+
+# ------------------------------------------------------------------------------------------------ embedding
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("T,V,D", [(1, 1, 1), (29, 119, 256), (3, 7, 5), (1000, 119, 29), (517, 33, 64), (100, 9, 1030),
+                                   (2050, 300, 257), (64, 5, 2048), (5, 4, 131), (1, 70000, 12)])
+def test_embed(tk, dtype, T, V, D):
+    g = gen(T + V + D)
+    table = torch.randn(V, D, device="cuda", generator=g, dtype=DTYPES[dtype])
+    for ids, view, scale in ((ids_of(T, V, g, 0.2), table, 16.0), (ids_of(T, V, g, 0.2, torch.int32), strided(table, 3, 2)[0], 0.37)):
+        got = tk.embed_tokens(ids, view, scale)
+        on = (ids >= 0) & (ids < V)
+        want = torch.where(on[:, None], table.double()[ids.long().clamp(0, V - 1)] * scale, 0.0)
+        assert got.dtype == table.dtype and got.shape == (T, D)
+        within(got, want, U * 2 * want.abs(), "embed")     # the product, and the scale as fp32
+
+
+def test_embed_shapes(tk):
+    table = torch.randn(11, 6, device="cuda")
+    ids = torch.arange(12, device="cuda").view(3, 4) - 1
+    got = tk.embed_tokens(ids, table)
+    assert got.shape == (3, 4, 6) and torch.equal(got[0, 1:], table[:3]) and not got[0, 0].any()
+    assert tk.embed_tokens(ids[:0], table).shape == (0, 4, 6)
+    assert torch.equal(tk.embed_tokens(ids.t(), table), got.transpose(0, 1))
+
+
+def grad_oracle(d, ids, V, scale):
+    on = (ids >= 0) & (ids < V)
+    d, ids = d.double()[on], ids.long()[on]
+    z = torch.zeros(V, d.shape[1], device="cuda", dtype=torch.float64)
+    want, mass = z.index_add(0, ids, d) * scale, z.index_add(0, ids, d.abs()) * scale
+    n = torch.bincount(ids, minlength=V).double()[:, None]
+    return want, (n + 2) * U * mass      # any order of n terms, the scaling
+
+
+EMBED_GRADS = [(1, 1, 1), (29, 119, 256), (1000, 119, 29), (4097, 255, 64), (4096, 256, 33), (3000, 257, 7), (5000, 2047, 16),
+               (2111, 2048, 40), (700, 5000, 300), (40000, 3, 130), (300, 100000, 8), (16384, 119, 513), (33, 5000000, 1)]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("T,V,D", EMBED_GRADS)
+def test_embed_grad(tk, dtype, T, V, D):
+    g = gen(T + V + D)
+    d = torch.randn(T, D, device="cuda", generator=g, dtype=DTYPES[dtype])
+    one = torch.full((T,), V // 2, device="cuda")
+    for name, ids in (("uniform", ids_of(T, V, g, 0.1)), ("one token", one), ("all ignored", one - V - 1),
+                      ("sorted", ids_of(T, V, g).sort().values), ("int32", ids_of(T, V, g, 0.1, torch.int32))):
+        got = tk.embed_tokens_grad(d, ids, V, 0.5)
+        want, slack = grad_oracle(d, ids, V, 0.5)
+        assert got.dtype == d.dtype
+        within(got, want, slack, name)
+        assert torch.equal(got, tk.embed_tokens_grad(d, ids, V, 0.5))      # the same bits every time
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_embed_grad_outputs_and_strides(tk, dtype):
+    g = gen(3)
+    T, V, D = 3000, 300, 70
+    d = torch.randn(T, D, device="cuda", generator=g, dtype=DTYPES[dtype])
+    ids = ids_of(T, V // 2, g, 0.1)       # half the table without a token
+    want, slack = grad_oracle(d, ids, V, 2.0)
+    out, buf = strided(torch.full((V, D), 5.0, device="cuda"), 3, 1)
+    got = tk.embed_tokens_grad(strided(d, 5, 3)[0], ids, V, 2.0, out=out)
+    assert got is out
+    within(out, want, slack, "fp32, strided")
+    assert (buf[:, 0] == 7).all() and (buf[:, -2:] == 7).all()             # what lies between the rows is left alone
+    start = torch.randn(V, D, device="cuda", generator=g)
+    acc = start.clone()
+    tk.embed_tokens_grad(d, ids, V, 2.0, out=acc, accumulate=True)
+    within(acc, start.double() + want, slack + U * (start.abs().double() + want.abs()), "accumulate")
+    assert torch.equal(acc[V // 2 + 10:], start[V // 2 + 10:])             # rows without a token as they were
+    empty = tk.embed_tokens_grad(d[:0], ids[:0], V)
+    assert empty.shape == (V, D) and not empty.any()
+    assert torch.equal(tk.embed_tokens_grad(d[:0], ids[:0], V, out=start.clone(), accumulate=True), start)
+
+
+def test_embed_autograd(tk):
+    g = gen(4)
+    table = torch.randn(119, 256, device="cuda", generator=g, requires_grad=True)
+    ids = ids_of(900, 119, g, 0.1).view(30, 30)
+    up = torch.randn(30, 30, 256, device="cuda", generator=g)
+    out = tk.embed_tokens(ids, table, 3.0)
+    out.backward(up)
+    want, slack = grad_oracle(up.view(900, 256), ids.view(-1), 119, 3.0)
+    within(table.grad, want, slack, "autograd")
+    # a broadcast incoming gradient (zero strides), as that of out.sum()
+    table.grad = None
+    tk.embed_tokens(ids, table, 3.0).sum().backward()
+    want, slack = grad_oracle(torch.ones(900, 256, device="cuda"), ids.view(-1), 119, 3.0)
+    within(table.grad, want, slack, "expanded gradient")
+
+
+# ------------------------------------------------------------------------------------------------ log-probabilities
+def logp_oracle(x, ids, temperature=1.0):
+    """(logp, p) in 64 bits; rows of -inf only and ignored rows have p = 0."""
+    z = x.double() / temperature
+    V = x.shape[1]
+    on = (ids >= 0) & (ids < V)
+    m = z.amax(1, keepdim=True)
+    m = torch.where(m == float("-inf"), torch.zeros_like(m), m)
+    e = (z - m).exp()
+    S = e.sum(1, keepdim=True)
+    lp = (z - m).gather(1, ids.long().clamp(0, V - 1)[:, None])[:, 0] - S[:, 0].log()
+    lp = torch.where(S[:, 0] == 0, torch.full_like(lp, float("-inf")), lp)
+    p = torch.where(S == 0, torch.zeros_like(e), e / S)
+    return torch.where(on, lp, torch.zeros_like(lp)), torch.where(on[:, None], p, torch.zeros_like(p)), on
+
+
+def d_logits_oracle(p, ids, on, g):
+    """g ([v = id] - p) row by row, 0 where g is 0."""
+    d = -p
+    d[torch.arange(len(ids), device="cuda")[on], ids.long()[on]] += 1
+    return torch.where((g == 0)[:, None], torch.zeros_like(d), d * g[:, None])
+
+
+# one size on either side of every border between the kernel's forms: 16, 32, 64, 128 ... 8192 packs of 4 or 8
+VOCABS = [1, 2, 7, 63, 64, 67, 119, 128, 131, 259, 300, 512, 515, 1030, 2048, 2055, 4100, 8192, 8199, 16387, 32768, 32771, 65539, 70001]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("V", VOCABS)
+def test_logprobs(tk, dtype, V):
+    g = gen(V)
+    T = 37 if V < 20000 else 5
+    x = (torch.randn(T, V, device="cuda", generator=g) * 3).to(DTYPES[dtype])
+    ids = ids_of(T, V, g, 0.15)
+    for view, tokens, tau in ((x, ids, 1.0), (strided(x, 3, 1)[0], ids.int(), 0.7)):
+        got = tk.token_logprobs(view, tokens, tau)
+        lp, p, on = logp_oracle(x, ids, tau)
+        within(got, lp, LOGP / tau, "logp")
+        leaf = view.detach().requires_grad_()
+        up = torch.randn(T, device="cuda", generator=g)
+        tk.token_logprobs(leaf, tokens, tau).backward(up)
+        want = d_logits_oracle(p, ids, on, up.double() / tau * on)
+        within(leaf.grad, want, (3 * LOGP / tau * (up.abs().double() / tau)[:, None] * (p + 1e-3)) + 4 * U * want.abs(), "d_logits")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("V", [5, 119, 515, 5000, 20000, 70001])
+def test_logprobs_masks(tk, dtype, V):
+    """-inf and lowest-value masks, empty rows, infinities and NaN."""
+    g = gen(V)
+    t = DTYPES[dtype]
+    low = torch.finfo(t).min
+    x = torch.randn(12, V, device="cuda", generator=g).to(t)
+    ids = torch.full((12,), 2, device="cuda")
+    x[0] = float("-inf")                                  # nothing left: logp -inf, no gradient
+    x[1] = float("-inf"); x[1, 2] = 0.5                   # only the chosen id
+    x[2] = float("-inf"); x[2, V - 1] = -3.0              # only another one: logp -inf
+    x[3] = low                                            # all at the lowest value: uniform
+    x[4] = low; x[4, 2] = 1.0
+    x[5, V // 2] = float("nan")                           # NaN reaches its row only
+    x[6, V - 1] = float("nan"); ids[6] = -1               # and not that of an ignored position
+    x[7, :3] = float("inf")
+    x[8, ::2] = float("-inf"); x[8, 2] = 0.0
+    got = tk.token_logprobs(x, ids)
+    assert got[0] == float("-inf") and got[2] == float("-inf") and got[6] == 0 and got[5].isnan() and got[7].isnan()
+    lp, p, on = logp_oracle(x, ids)
+    rows = [0, 1, 2, 3, 4, 6, 8, 9, 10, 11]
+    within(got[rows], lp[rows], LOGP, "logp")
+    leaf = x.clone().requires_grad_()
+    tk.token_logprobs(leaf, ids).backward(torch.ones(12, device="cuda"))
+    assert not leaf.grad[0].any() and not leaf.grad[6].any() and leaf.grad[5].isnan().any()
+    want = d_logits_oracle(p, ids, on, on.double())
+    want[0] = 0
+    # (row 0: a row without a distribution has p = 0 and sends no gradient at the chosen id either)
+    within(leaf.grad[rows], want[rows], 3 * LOGP * (p[rows] + 1e-3), "d_logits")
+
+
+def test_logprobs_shapes(tk):
+    x = torch.randn(4, 6, 9, device="cuda")
+    ids = torch.randint(0, 9, (4, 6), device="cuda")
+    want = torch.log_softmax(x.double(), -1).gather(-1, ids[..., None])[..., 0]
+    within(tk.token_logprobs(x, ids), want, LOGP, "3-D")
+    within(tk.token_logprobs(x.transpose(0, 1), ids.t()), want.t(), LOGP, "transposed")
+    y = torch.randn(9, 30, device="cuda").t()             # columns of unit stride
+    within(tk.token_logprobs(y, ids.view(-1)[:20].repeat(2)[:30]), torch.log_softmax(y.double(), -1).gather(
+        1, ids.view(-1)[:20].repeat(2)[:30, None])[:, 0], LOGP, "column-major")
+    z = torch.randn(1, 9, device="cuda").expand(5, 9)     # rows that are one row
+    within(tk.token_logprobs(z, torch.arange(5, device="cuda")), torch.log_softmax(z.double(), -1)[0, :5], LOGP, "expanded")
+    assert tk.token_logprobs(x[:0], ids[:0]).shape == (0, 6)
+
+
+# ------------------------------------------------------------------------------------------------ losses
+def cuts(T, S, g):
+    c = torch.randint(0, T + 1, (S - 1,), device="cuda", generator=g).sort().values if S > 1 else torch.zeros(0, device="cuda")
+    return torch.cat([torch.zeros(1, device="cuda"), c, torch.full((1,), T, device="cuda")]).to(torch.int32)
+
+
+def owner_of(ptr, T):
+    t = torch.arange(T, device="cuda")
+    s = torch.searchsorted(ptr.long().contiguous(), t, right=True) - 1
+    return torch.where((s >= 0) & (s < len(ptr) - 1), s, torch.full_like(s, -1))
+
+
+def seq_sum(values, owner, S):
+    return torch.zeros(S + 1, dtype=torch.float64, device="cuda").index_add(0, owner + 1, values.double())[1:]
+
+
+def preference_oracle(x, ids, ptr, ref, beta, e, kind, average, tau, denominator):
+    T, S = len(ids), len(ptr) - 1
+    P = S // 2
+    lp, p, on = logp_oracle(x, ids, tau)
+    owner = owner_of(ptr, T)
+    on = on & (owner >= 0)
+    diff = torch.where(on, lp - (ref.double() if ref is not None else 0.0), torch.zeros_like(lp))
+    n = seq_sum(on, owner, S)
+    share = torch.where(n > 0, 1 / n.clamp(min=1), torch.ones_like(n)) if average else torch.ones_like(n)
+    r = (seq_sum(diff, owner, S) * share).requires_grad_()
+    gap = r[:P] - r[P:]
+    sp = torch.nn.functional.softplus
+    each = (1 - e) * sp(-beta * gap) + e * sp(beta * gap) if kind == "sigmoid" else (gap - 0.5 / beta) ** 2
+    loss = each.sum() / (denominator or P)
+    slope, = torch.autograd.grad(loss, r)
+    g = torch.where(on, (slope * share)[owner.clamp(min=0)], torch.zeros_like(lp)) / tau
+    return dict(loss=loss.detach(), log_ratio=r.detach(), margin=gap.detach(), d=d_logits_oracle(p, ids, on, g), g=g, p=p, n=n, share=share,
+                each=each.detach())
+
+
+PREFS = [  # T, V, P, beta, e, kind, average, tau, denominator, whole (sequences cover all positions)
+    (2, 119, 1, 0.1, 0.0, "sigmoid", False, 1.0, None, True), (29 * 64, 119, 32, 0.5, 0.1, "sigmoid", False, 1.0, None, True),
+    (5000, 119, 700, 0.1, 0.0, "sigmoid", True, 0.8, 12.5, False), (9000, 21, 1, 0.02, 0.2, "sigmoid", False, 1.0, None, True),
+    (9001, 21, 3, 0.3, 0.0, "ipo", True, 1.3, None, False), (1023, 515, 4, 0.1, 0.0, "ipo", True, 1.0, 100.0, True),
+    (1025, 33, 5000, 0.1, 0.0, "sigmoid", False, 1.0, None, True), (40, 20001, 2, 0.1, 0.05, "sigmoid", True, 1.0, None, False)]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("case", PREFS)
+def test_preference(tk, dtype, case):
+    T, V, P, beta, e, kind, average, tau, denominator, whole = case
+    g = gen(T + V)
+    x = (torch.randn(T, V, device="cuda", generator=g) * 2).to(DTYPES[dtype])
+    ids = ids_of(T, V, g, 0.1)
+    ptr = cuts(T, 2 * P, g)
+    if not whole:       # some positions lie before the first sequence, some behind the last
+        ptr = ptr.clamp(7, T - 9)
+    lp = logp_oracle(x, ids, tau)[0]
+    ref = (lp + 0.1 * torch.randn(T, device="cuda", generator=g)).float()
+    scale = 256.0 if dtype == "fp16" else 1.0
+    got = tk.preference_loss_and_grad(strided(x, 5, 2)[0], ids, ptr, ref, beta, e, kind, average, tau, denominator, scale)
+    want = preference_oracle(x, ids, ptr, ref, beta, e, kind, average, tau, denominator)
+    ratio_slack = (want["n"] + 1) * (LOGP / tau + U) * want["share"]                  # every position's difference
+    gap_slack = ratio_slack[:P] + ratio_slack[P:]
+    within(got.log_ratio, want["log_ratio"], ratio_slack, "log_ratio")
+    within(got.margin, want["margin"], gap_slack, "margin")
+    D = denominator or P
+    gap = want["margin"]
+    lip = beta * torch.ones_like(gap) if kind == "sigmoid" else 2 * (gap - 0.5 / beta).abs() + gap_slack
+    within(got.loss, want["loss"], (lip * gap_slack).sum() / D + 1e-12, "loss")
+    curve = (beta ** 2 / 4 if kind == "sigmoid" else 2.0) / D * gap_slack             # how far a slope can be off
+    owner = owner_of(ptr, T).clamp(min=0) % P
+    g_off = torch.where(want["g"] != 0, curve[owner] / tau * want["share"][owner_of(ptr, T).clamp(min=0)], 0.0) + 4 * U * want["g"].abs()
+    slack = scale * (g_off[:, None] + 3 * LOGP / tau * want["g"].abs()[:, None] * (want["p"] + 1e-3))
+    within(got.d_logits, want["d"] * scale, slack, "d_logits")
+    assert got.d_logits.dtype == x.dtype
+    again = tk.preference_loss_and_grad(x, ids.int(), ptr.long(), ref, beta, e, kind, average, tau, denominator, scale)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))                         # strides and id types change no bit
+    # the differentiable form, its gradient scaled by what comes in
+    leaf = x.clone().requires_grad_()
+    r = tk.preference_loss(leaf, ids, ptr, ref, beta, e, kind, average, tau, denominator)
+    (r.loss * scale).backward()
+    assert torch.equal(r.loss, got.loss) and torch.equal(r.log_ratio, got.log_ratio) and torch.equal(r.margin, got.margin)
+    within(leaf.grad, want["d"] * scale, slack, "autograd")
+
+
+def test_preference_empty(tk):
+    """Sequences and batches without a position: the margin is 0."""
+    x, ids = torch.randn(6, 119, device="cuda"), torch.full((6,), -1, device="cuda")
+    z = torch.zeros(5, dtype=torch.int32, device="cuda")
+    for args in ((x[:0], ids[:0], z), (x, ids, torch.tensor([0, 2, 4, 5, 6], device="cuda")), (x, ids * 0, z)):
+        for average in (False, True):
+            r = tk.preference_loss_and_grad(*args, average=average)
+            within(r.loss, torch.log(torch.tensor(2.0, dtype=torch.float64, device="cuda")), 0.0, "log 2")
+            assert not r.margin.any() and not r.log_ratio.any() and not r.d_logits.any()
+
+
+def policy_oracle(x, ids, ptr, adv, per_token, old, ref, lo, hi, kl_coef, aggregate, tau, denominator):
+    T = len(ids)
+    S = len(ptr) - 1 if ptr is not None else 1
+    lp, p, on = logp_oracle(x, ids, tau)
+    owner = owner_of(ptr, T) if ptr is not None else torch.zeros(T, dtype=torch.int64, device="cuda")
+    on = on & (owner >= 0)
+    n = seq_sum(on, owner, S)
+    A = adv.double() if per_token else adv.double()[owner.clamp(min=0)]
+    if aggregate == "token":
+        w = on.double() / (denominator or float(on.sum().clamp(min=1)))
+    else:
+        w = torch.where(on, 1 / ((denominator or S) * n.clamp(min=1)[owner.clamp(min=0)]), 0.0)
+    leaf = lp.clone().requires_grad_()
+    rho = (leaf - (old.double() if old is not None else leaf.detach())).exp()
+    gain = torch.where(A == 0, torch.zeros_like(rho), torch.minimum(rho * A, rho.clamp(1 - lo, 1 + hi) * A))
+    q = ref.double() - leaf if ref is not None else leaf * 0
+    kl_t = q.exp() - 1 - q
+    sur, kl = -(w * gain)[on].sum(), (w * kl_t)[on].sum()
+    loss = sur + kl_coef * kl
+    c, = torch.autograd.grad(loss, leaf)
+    hit = ((A > 0) & (rho > 1 + hi)) | ((A < 0) & (rho < 1 - lo))
+    g = torch.where(on, c, torch.zeros_like(c)) / tau
+    rho = rho.detach()
+    return dict(loss=loss.detach(), surrogate=sur.detach(), kl=kl.detach(), clip_fraction=(w * hit)[on].sum().detach(),
+                logp=lp, d=d_logits_oracle(p, ids, on, g), g=g, p=p, on=on, w=w,
+                # the error of logp, LOGP, reaches the slope A rho + kl_coef exp(q) once, the two terms themselves once
+                dg=w * (A.abs() * rho + kl_coef * q.exp()).detach(), ds=w * A.abs() * rho, dk=w * (q.exp() - 1).abs().detach(),
+                mass=(w * (gain.abs() + kl_coef * kl_t))[on].sum().detach())
+
+
+POLICIES = [  # T, V, S (None: no seq_ptr), per token, old, ref, lo, hi, kl_coef, aggregate, tau, denominator, whole
+    (1, 119, 1, False, True, True, 0.2, 0.2, 0.1, "token", 1.0, None, True),
+    (29, 119, 1, False, True, True, 0.2, 0.28, 0.05, "sequence", 1.0, None, True),
+    (1900, 119, 64, False, True, False, 0.2, 0.2, 0.0, "sequence", 0.9, None, False),
+    (5000, 119, 6000, False, True, True, 0.1, 0.3, 0.2, "sequence", 1.0, 77.0, True),
+    (9000, 21, 2, False, False, True, 0.2, 0.2, 0.5, "sequence", 1.0, None, True),
+    (3001, 515, 9, True, True, True, 0.2, 0.2, 0.1, "token", 1.2, None, False),
+    (2048, 64, 2048, True, True, True, 0.2, 0.2, 0.1, "token", 1.0, 5000.0, True),
+    (70, 20001, None, True, True, False, 1.0, 0.0, 0.1, "token", 1.0, None, True),
+    (40000, 119, 1300, False, False, False, 0.0, 0.2, 0.0, "token", 1.0, None, True)]
+
+
+def policy_inputs(case, dtype, seed=0):
+    T, V, S, per_token, use_old, use_ref, lo, hi, kl_coef, aggregate, tau, denominator, whole = case
+    g = gen(T + V + seed)
+    x = (torch.randn(T, V, device="cuda", generator=g) * 2).to(DTYPES[dtype])
+    ids = ids_of(T, V, g, 0.1 if T > 1 else 0.0)
+    ptr = None if S is None else cuts(T, S, g)
+    if not whole:
+        ptr = ptr.clamp(7, T - 9)
+    lp = logp_oracle(x, ids, tau)[0]
+    move = 0.3 * torch.randn(T, device="cuda", generator=g)
+    for bound in (1 - lo, 1 + hi):          # no ratio within the error of a clip bound
+        if bound > 0:
+            edge = -torch.log(torch.tensor(bound))
+            move = torch.where((move - edge).abs() < 1e-3, edge + 2e-3, move)
+    old = (lp + move).float() if use_old else None
+    ref = (lp + 0.3 * torch.randn(T, device="cuda", generator=g)).float() if use_ref else None
+    adv = torch.randn(T if per_token else (S or 1), device="cuda", generator=g)
+    adv[::7] = 0.0
+    return x, ids, ptr, adv, old, ref
+
+
+def policy_slack(want, scale, tau):
+    slack = scale * (3 * LOGP / tau * (want["g"].abs()[:, None] * (want["p"] + 1e-3))
+                     + (2 * LOGP / tau + 16 * U) * (want["dg"] / tau)[:, None])
+    return slack
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("case", POLICIES)
+def test_policy(tk, dtype, case):
+    T, V, S, per_token, use_old, use_ref, lo, hi, kl_coef, aggregate, tau, denominator, whole = case
+    x, ids, ptr, adv, old, ref = policy_inputs(case, dtype)
+    scale = 1024.0 if dtype == "fp16" else 1.0
+    per = "token" if per_token else "sequence"
+    got = tk.policy_loss_and_grad(strided(x, 3, 1)[0], ids, ptr, adv, old, ref, per, lo, hi, kl_coef, aggregate, tau, denominator, scale)
+    want = policy_oracle(x, ids, ptr, adv, per_token, old, ref, lo, hi, kl_coef, aggregate, tau, denominator)
+    within(got.logp[want["on"]], want["logp"][want["on"]], LOGP / tau, "logp")
+    assert not got.logp[~want["on"]].any()
+    e = LOGP / tau + 16 * U
+    s_off, k_off = (e * want["ds"]).sum(), (e * want["dk"] + 8 * U * want["w"]).sum()
+    within(got.surrogate, want["surrogate"], s_off, "surrogate")
+    within(got.kl, want["kl"], k_off, "kl")
+    within(got.loss, want["loss"], s_off + kl_coef * k_off, "loss")
+    within(got.clip_fraction, want["clip_fraction"], 1e-9, "clip_fraction")
+    slack = policy_slack(want, scale, tau)
+    within(got.d_logits, want["d"] * scale, slack, "d_logits")
+    again = tk.policy_loss_and_grad(x, ids.int(), ptr, adv, old, ref, per, lo, hi, kl_coef, aggregate, tau, denominator, scale)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    leaf = x.clone().requires_grad_()
+    r = tk.policy_loss(leaf, ids, ptr, adv, old, ref, per, lo, hi, kl_coef, aggregate, tau, denominator)
+    (r.loss * scale).backward()
+    assert all(torch.equal(a, b) for a, b in zip(r, got[:5]))
+    within(leaf.grad, want["d"] * scale, slack, "autograd")
+
+
+def test_policy_empty(tk):
+    x, ids = torch.randn(6, 119, device="cuda"), torch.full((6,), -1, device="cuda")
+    x[2] = float("nan")
+    z, adv = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.ones(2, device="cuda")
+    for args in ((x[:0], ids[:0], z, adv), (x, ids, torch.tensor([0, 2, 6], device="cuda"), adv), (x, ids * 0, z, adv)):
+        for aggregate in ("token", "sequence"):
+            r = tk.policy_loss_and_grad(*args, kl_coef=0.1, aggregate=aggregate)
+            assert r.loss == 0 and r.kl == 0 and r.surrogate == 0 and r.clip_fraction == 0 and not r.d_logits.any() and not r.logp.any()
+
+
+def test_nan_stays_in_its_row(tk):
+    """A NaN logit at a position that takes no part reaches nothing; at one that does, its row's gradient and the loss."""
+    g = gen(8)
+    x = torch.randn(100, 119, device="cuda", generator=g)
+    ids, ptr = ids_of(100, 119, g), torch.tensor([10, 50, 90], device="cuda")
+    ids[20] = -1
+    adv = torch.ones(2, device="cuda")
+    clean = tk.policy_loss_and_grad(x, ids, ptr, adv, kl_coef=0.0)
+    clean_pref = tk.preference_loss_and_grad(x, ids, ptr)
+    x[3], x[20], x[95] = float("nan"), float("nan"), float("nan")
+    assert all(torch.equal(a, b) for a, b in zip(tk.policy_loss_and_grad(x, ids, ptr, adv, kl_coef=0.0), clean))
+    assert all(torch.equal(a, b) for a, b in zip(tk.preference_loss_and_grad(x, ids, ptr), clean_pref))
+    x[30, 5] = float("nan")
+    r = tk.policy_loss_and_grad(x, ids, ptr, adv, kl_coef=0.0)
+    assert r.loss.isnan() and r.d_logits[30].isnan().all()
+    rest = [i for i in range(100) if i != 30]
+    assert torch.equal(r.d_logits[rest], clean.d_logits[rest])
+
+
+def test_gradients_against_differences(tk):
+    """Central differences of the 64-bit loss along a direction, step 1e-5: their own error, h^2 and 1e-16 / h, is below
+    1e-9 of the terms' size; the gradients are fp32, off by a few LOGP of each term."""
+    g = gen(9)
+    case = (60, 31, 6, False, True, True, 0.2, 0.2, 0.3, "sequence", 0.8, None, True)
+    x, ids, ptr, adv, old, ref = policy_inputs(case, "fp32")
+    v = torch.randn(x.shape, device="cuda", generator=g, dtype=torch.float64)
+    h = 1e-5
+    f = lambda y: policy_oracle(y, ids, ptr, adv, False, old, ref, 0.2, 0.2, 0.3, "sequence", 0.8, None)["loss"]   # noqa: E731
+    want = (f(x.double() + h * v) - f(x.double() - h * v)) / (2 * h)
+    got = tk.policy_loss_and_grad(x, ids, ptr, adv, old, ref, "sequence", 0.2, 0.2, 0.3, "sequence", 0.8).d_logits
+    size = (got.double().abs() * v.abs()).sum()
+    assert abs((got.double() * v).sum() - want) <= 4 * LOGP / 0.8 * size
+    f = lambda y: preference_oracle(y, ids, ptr, ref, 0.5, 0.1, "sigmoid", False, 0.8, None)["loss"]   # noqa: E731
+    want = (f(x.double() + h * v) - f(x.double() - h * v)) / (2 * h)
+    got = tk.preference_loss_and_grad(x, ids, ptr, ref, 0.5, 0.1, temperature=0.8).d_logits
+    size = (got.double().abs() * v.abs()).sum()
+    assert abs((got.double() * v).sum() - want) <= 4 * LOGP / 0.8 * size
+
+
+# ------------------------------------------------------------------------------------------------ how they are called
+def test_two_backwards_of_one_graph(tk):
+    g = gen(10)
+    x = torch.randn(64, 119, device="cuda", generator=g, requires_grad=True)
+    ids, ptr, adv = ids_of(64, 119, g), cuts(64, 4, g), torch.ones(4, device="cuda")
+    for loss in (tk.policy_loss(x, ids, ptr, adv).loss, tk.preference_loss(x, ids, ptr).loss, tk.token_logprobs(x, ids).sum()):
+        a, = torch.autograd.grad(loss, x, retain_graph=True)
+        b, = torch.autograd.grad(loss * 2, x)
+        within(b, 2 * a.double(), 2 * U * a.abs().double(), "second backward")
+    loss = tk.policy_loss(x, ids, ptr, adv).loss
+    with torch.no_grad():
+        x.mul_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_captured_and_replayed(tk):
+    """All operators in one graph, replayed on new inputs with eager work in between: every replay has the eager bits."""
+    g = gen(11)
+    T, V, S = 3000, 119, 80
+    x, ids, ptr = torch.randn(T, V, device="cuda", generator=g), ids_of(T, V, g, 0.1), cuts(T, S, g)
+    adv, old = torch.randn(S, device="cuda", generator=g), -4 + torch.randn(T, device="cuda", generator=g)
+    table, up = torch.randn(V, 256, device="cuda", generator=g), torch.randn(T, 256, device="cuda", generator=g)
+
+    def step():
+        p = tk.policy_loss_and_grad(x, ids, ptr, adv, old, old, kl_coef=0.1, aggregate="sequence")
+        q = tk.preference_loss_and_grad(x, ids, ptr, old)
+        return [*p, *q, tk.embed_tokens(ids, table, 2.0), tk.embed_tokens_grad(up, ids, V, 2.0), tk.embed_tokens_grad(up, ids, 5000),
+                tk.token_logprobs(x, ids)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for k in range(4):
+        for t in (x, adv, table, up):
+            t.copy_(torch.randn(t.shape, device="cuda", generator=g))
+        ids.copy_(ids_of(T, V, g, 0.1))
+        ptr.copy_(cuts(T, S, g))
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        for i, (a, b) in enumerate(zip(outs, eager)):
+            assert torch.equal(a, b), (k, i)
+
+
+def test_two_calls_at_once(tk):
+    """Calls that overlap on two streams share nothing."""
+    g = gen(12)
+    sets = [(torch.randn(20000, 119, device="cuda", generator=g), ids_of(20000, 119, g, 0.1), cuts(20000, 600, g),
+             torch.randn(600, device="cuda", generator=g), torch.randn(20000, 256, device="cuda", generator=g)) for _ in range(2)]
+
+    def step(x, ids, ptr, adv, up):
+        return [*tk.policy_loss_and_grad(x, ids, ptr, adv, kl_coef=0.0), *tk.preference_loss_and_grad(x, ids, ptr),
+                tk.embed_tokens_grad(up, ids, 119)]
+
+    alone = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(5):
+        for i, (st, s) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(st):
+                got[i].append(step(*s))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, alone[i]))
+
+
+def test_refusals(tk):
+    x, ids = torch.randn(6, 119, device="cuda"), torch.zeros(6, dtype=torch.int64, device="cuda")
+    ptr, adv = torch.tensor([0, 3, 6], device="cuda"), torch.ones(2, device="cuda")
+    for call in (
+            lambda: tk.token_logprobs(x.double(), ids), lambda: tk.token_logprobs(x, ids.float()), lambda: tk.token_logprobs(x, ids[:5]),
+            lambda: tk.token_logprobs(x, ids.cpu()), lambda: tk.token_logprobs(x, ids, 0.0), lambda: tk.token_logprobs(x, ids, float("nan")),
+            lambda: tk.token_logprobs(x[0], ids[0]), lambda: tk.token_logprobs(x[:, :0], ids),
+            lambda: tk.preference_loss(x, ids, ptr[:2]), lambda: tk.preference_loss(x, ids, ptr[:1]), lambda: tk.preference_loss(x, ids, ptr.cpu()),
+            lambda: tk.preference_loss(x, ids, ptr.float()), lambda: tk.preference_loss(x, ids, ptr, beta=0.0),
+            lambda: tk.preference_loss(x, ids, ptr, label_smoothing=0.6), lambda: tk.preference_loss(x, ids, ptr, kind="hinge"),
+            lambda: tk.preference_loss(x, ids, ptr, kind="ipo", label_smoothing=0.1), lambda: tk.preference_loss(x, ids, ptr, adv),
+            lambda: tk.preference_loss(x, ids, ptr, denominator=0), lambda: tk.preference_loss(x, ids, ptr, x[:, 0].cpu()),
+            lambda: tk.preference_loss(x, ids, ptr, ids), lambda: tk.preference_loss_and_grad(x, ids, ptr, grad_scale=float("inf")),
+            lambda: tk.policy_loss(x, ids, ptr, adv[:1]), lambda: tk.policy_loss(x, ids, ptr, adv, advantage_per="token"),
+            lambda: tk.policy_loss(x, ids, ptr, adv, advantage_per="atom"), lambda: tk.policy_loss(x, ids, None, adv),
+            lambda: tk.policy_loss(x, ids, ptr, adv, adv), lambda: tk.policy_loss(x, ids, ptr, adv, clip_low=1.1),
+            lambda: tk.policy_loss(x, ids, ptr, adv, clip_high=-0.1), lambda: tk.policy_loss(x, ids, ptr, adv, kl_coef=-1),
+            lambda: tk.policy_loss(x, ids, ptr, adv, aggregate="mean"), lambda: tk.policy_loss(x, ids, ptr, adv, denominator=-1),
+            lambda: tk.embed_tokens(ids, x[0]), lambda: tk.embed_tokens(ids.float(), x), lambda: tk.embed_tokens(ids, x, float("nan")),
+            lambda: tk.embed_tokens(ids, x[:0]), lambda: tk.embed_tokens(ids.cpu(), x), lambda: tk.embed_tokens_grad(x, ids[:5], 3),
+            lambda: tk.embed_tokens_grad(x, ids, 0), lambda: tk.embed_tokens_grad(x, ids, 3, accumulate=True),
+            lambda: tk.embed_tokens_grad(x, ids, 3, out=torch.empty(4, 119, device="cuda")),
+            lambda: tk.embed_tokens_grad(x, ids, 3, out=torch.empty(3, 119, device="cuda", dtype=torch.bfloat16)),
+            lambda: tk.embed_tokens_grad(x, ids, 3, out=torch.empty(119, 3, device="cuda").t()),
+            lambda: tk.embed_tokens_grad(x, ids, 3, out=torch.empty(1, 119, device="cuda").expand(3, 119))):
+        with pytest.raises(ValueError):
+            call()
