@@ -7,7 +7,9 @@ pids=()
 for f in chain_dit_mol_heads chain_dit_mol chain_dit_row_heads chain_dit_row forward backward chain_e3 sampler api pack loss consistency optim embed tokens; do
   if [ -f $f.hip ]; then
     MORE=""
-    case $f in embed|tokens) MORE="-Xclang -target-feature -Xclang -packed-fp32-ops" ;; esac   # no packed fp32 arithmetic
+    # no packed fp32 arithmetic; constants of the per-row 64-bit part are not hoisted into registers for the whole row loop
+    # (k_token_rows: 20 to 30 registers, two waves a SIMD)
+    case $f in embed|tokens) MORE="-Xclang -target-feature -Xclang -packed-fp32-ops -mllvm -disable-machine-licm" ;; esac
     hipcc $FLAGS $MORE -c $f.hip -o $f.o &
     pids+=($!)
   fi

@@ -17,6 +17,14 @@ struct TokenRows {
   double inv_t;        // 1 / temperature
 };
 
+// exp((x - m) / temperature) of a row with maximum m is exp2(c x - mc), mc = c m: one fused multiply-add, rounded once, also
+// for logits far from 0.  mc is a rounded number, but the same one in every element and in logp, where it cancels exactly;
+// so does c, whose rounding only means a temperature that is off by 2^-25.  A maximum near the end of the fp32 range (rows
+// masked with the type's lowest value) would overflow mc: such a row is shifted by m first, and its mc is 0.
+__device__ __forceinline__ bool far_out(float m) { return !(fabsf(m) < 1e38f); }
+__device__ __forceinline__ float shifted(float x, float m) { return x == m ? 0.f : x - m; }   // (+inf - +inf is not asked for)
+
+
 // log(s) of the softmax sum, in 64 bits: losses use differences of log-probabilities of two policies, which are small
 // against the log-probabilities.  s = 2^k f with f in [sqrt(1/2), sqrt(2)), z = (f - 1) / (f + 1),
 // log f = 2 (z + z^3/3 + z^5/5 + ...): |z| < 0.172, six terms leave 5e-11 (the fp32 sum itself is good to ~1e-7).
@@ -69,9 +77,7 @@ struct PolicyIn {
   const float* old_logp;     // may be null: the policy itself
   const float* ref_logp;     // may be null: no KL term
   float clip_lo, clip_hi, kl_coef, grad_scale;
-  double* partial;           // [gridDim.x][3]
-  uint32_t* counter;
-  float* result;             // loss, surrogate, kl, clip fraction
+  double* partial;           // [gridDim.x][3]: surrogate, kl, share of clipped rows
 };
 struct RowOut {
   float* logp;               // [n] or null
@@ -80,38 +86,61 @@ struct RowOut {
   float* coef;               // [n] d loss / d logp (TK_POLICY); may be null
   void* d;                   // gradient of the logits or null
   int64_t d_stride;
-  uint32_t* clear;           // a counter of a later launch to set to 0, or null
 };
 
 // What a row contributes once its maximum M and sum S are known, the same in every lane of the row; returns the gradient's
 // factor d loss / d logp * grad_scale / temperature.
+// What is known of a row besides its logits; loaded one row ahead, so that a row costs one memory latency.
+struct RowScalars { int id, seq; float old, ref; };
+// A value that all lanes of the wave share, in a scalar register.
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ double uniform(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int MODE> __device__ __forceinline__ RowScalars row_scalars(const TokenRows& a, const PolicyIn& p, const RowOut& o, int64_t t) {
+  RowScalars r{-1, 0, 0.f, 0.f};
+  if (t >= a.n) return r;
+  r.id = a.tok.at(t);
+  if constexpr (MODE == TK_POLICY) {
+    r.seq = p.seq_of[t];
+    if (p.old_logp) r.old = p.old_logp[t];
+    if (p.ref_logp) r.ref = p.ref_logp[t];
+  } else if (o.minus) r.ref = o.minus[t];
+  return r;
+}
+
 template <int MODE>
-__device__ __forceinline__ float row_epilogue(const TokenRows& a, const PolicyIn& p, const RowOut& o, int64_t t, int id, int seq,
-                                              float xt, float M, float S, float inv_s, bool writer, double w, double (&acc)[3]) {
+__device__ __forceinline__ float row_epilogue(const TokenRows& a, const PolicyIn& p, const RowOut& o, int64_t t, const RowScalars& c,
+                                              float xt, float M, float S, float inv_s, bool writer, float A, double w, double* acc) {
   // a row of -inf only has no distribution: S = 0, logp = -inf, no gradient
-  const double lp = S == 0.f ? -__builtin_inf() : ((double)xt - (double)M) * a.inv_t - log_of_sum(S);
+  const double z = far_out(M) ? ((double)xt - (double)M) * a.c : fma((double)xt, (double)a.c, -(double)(M * a.c));
+  const double lp = S == 0.f ? -__builtin_inf() : fma(z, 0.69314718055994530942, -log_of_sum(S));
   float g = 0.f, coef = 0.f;
   if constexpr (MODE == TK_POLICY) {
-    const float A = p.adv[p.adv_per_token ? t : (int64_t)seq];
-    const float rho = p.old_logp ? expf((float)(lp - (double)p.old_logp[t])) : lp == lp ? 1.0f : (float)lp;
+    const float rho = p.old_logp ? expf((float)(lp - (double)c.old)) : lp == lp ? 1.0f : (float)lp;
     const float hi = 1.0f + p.clip_hi, lo = 1.0f - p.clip_lo;
     const bool clipped = (A > 0.f && rho > hi) || (A < 0.f && rho < lo);
     const float gain = A == 0.f ? 0.f : fminf(rho * A, fminf(fmaxf(rho, lo), hi) * A);
     float slope = clipped || A == 0.f ? 0.f : -A * rho;
     float em1 = 0.f, kl = 0.f;
     if (p.ref_logp) {
-      kl_terms((float)((double)p.ref_logp[t] - lp), em1, kl);
+      kl_terms((float)((double)c.ref - lp), em1, kl);
       slope -= p.kl_coef * em1;
     }
     if (rho != rho) slope = rho;   // fminf drops a NaN
-    acc[0] -= w * (double)(rho != rho ? rho : gain);
-    acc[1] += w * (double)kl;
-    acc[2] += clipped ? w : 0.0;
+    if (writer) {
+      acc[0] -= w * (double)(rho != rho ? rho : gain);
+      acc[1] += w * (double)kl;
+      acc[2] += clipped ? w : 0.0;
+    }
     coef = (float)(w * (double)slope);
     if (S != 0.f) g = (float)(w * (double)slope * (double)p.grad_scale * a.inv_t);
   }
   if (writer) {
-    if (o.logp) o.logp[t] = (float)(o.minus ? lp - (double)o.minus[t] : lp);
+    if (o.logp) o.logp[t] = (float)(MODE == TK_LOGP ? lp - (double)c.ref : lp);
     if (o.stats) { o.stats[2 * t] = M; o.stats[2 * t + 1] = inv_s; }
     if (o.coef) o.coef[t] = coef;
   }
@@ -152,124 +181,238 @@ template <int NT> __device__ __forceinline__ double inverse_total(const PolicyIn
   }
   return total > 0.0 ? 1.0 / total : 0.0;
 }
-// Per-block sums to memory; the last block adds them up in block order.
-template <int NT> __device__ __forceinline__ void policy_finish(const PolicyIn& p, double (&acc)[3], double* red) {
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    const double v = block_sum<NT>(acc[k], red);
-    if (threadIdx.x == 0) p.partial[(int64_t)blockIdx.x * 3 + k] = v;
-  }
-  if (!last_block(p.counter)) return;
-  double v[3] = {0.0, 0.0, 0.0};
-  for (int b = threadIdx.x; b < (int)gridDim.x; b += NT)
-#pragma unroll
-    for (int k = 0; k < 3; ++k) v[k] += p.partial[(int64_t)b * 3 + k];
-#pragma unroll
-  for (int k = 0; k < 3; ++k) v[k] = block_sum<NT>(v[k], red);
-  if (threadIdx.x == 0) {
-    p.result[0] = (float)(v[0] + (double)p.kl_coef * v[1]);
-    p.result[1] = (float)v[0];
-    p.result[2] = (float)v[1];
-    p.result[3] = (float)v[2];
+// Per-block sums to memory; k_policy_final adds them up in block order.  (A last block that did it inside this launch would
+// need a release fence in every block, which writes back its XCD's L2: 30 us for 1200 blocks against 3 for a launch.)
+template <int RPB> __device__ __forceinline__ void policy_partial(const PolicyIn& p, const double (&acc)[RPB][3]) {
+  __syncthreads();
+  if (threadIdx.x < 3) {
+    double v = acc[0][threadIdx.x];
+    for (int g = 1; g < RPB; ++g) v += acc[g][threadIdx.x];
+    p.partial[(int64_t)blockIdx.x * 3 + threadIdx.x] = v;
   }
 }
+__global__ __launch_bounds__(256) void k_policy_final(const double* __restrict__ partial, int blocks, double kl_coef, float* __restrict__ result) {
+  __shared__ double red[4];
+  double v[3] = {0.0, 0.0, 0.0};
+#pragma unroll 4
+  for (int b = threadIdx.x; b < blocks; b += 256)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) v[k] += partial[(int64_t)b * 3 + k];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) v[k] = block_sum<256>(v[k], red);
+  if (threadIdx.x == 0) {
+    result[0] = (float)(v[0] + kl_coef * v[1]);
+    result[1] = (float)v[0];
+    result[2] = (float)v[1];
+    result[3] = (float)v[2];
+  }
+}
+
+// What a wave's sum, relative to its own maximum m, counts in a row with maximum M.
+__device__ __forceinline__ float part_factor(float m, float M, float c) {
+#pragma clang fp contract(off)   // both products are the rounded numbers that the exponentials used
+  if (m == -__builtin_inff()) return 0.f;
+  const float mc = m * c, Mc = M * c;
+  return __builtin_amdgcn_exp2f(far_out(m) || far_out(M) ? shifted(m, M) * c : mc - Mc);
+}
+// The maximum and sum of a row from those of its 4 or 16 waves (0 and 0 for a row of -inf only).
+template <int NW> __device__ __forceinline__ void join_waves(const float2* sh, float c, float& M, float& S) {
+  const float2 v = sh[threadIdx.x & (NW - 1)];
+  M = v.x;
+  M = fmaxf(M, dpp_move<0xB1>(M));
+  M = fmaxf(M, dpp_move<0x4E>(M));
+  if (NW == 16) { M = fmaxf(M, dpp_move<0x141>(M)); M = fmaxf(M, dpp_move<0x140>(M)); }
+  if (M == -__builtin_inff()) M = 0.f;
+  S = v.y * part_factor(v.x, M, c);
+  S += dpp_move<0xB1>(S);
+  S += dpp_move<0x4E>(S);
+  if (NW == 16) { S += dpp_move<0x141>(S); S += dpp_move<0x140>(S); }
+}
+// exp2(c x - mc) of a lane's packs, handed on one pack at a time.  Half-precision packs stay packed until then (the compiler
+// would keep the values that it unpacked for the maximum, twice the registers): the policy loss exponentiates them a second
+// time for its gradient rather than hold 32-bit results, which halves the rows in flight.
+__device__ __forceinline__ void set_pack(u32x4& x, const float (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = __float_as_uint(v[j]);
+}
+template <typename T, int NV, typename F>
+__device__ __forceinline__ void exponentials(u32x4 (&x)[NV], float m, float mc, float c, bool far, F&& take) {
+  constexpr int N = Pack<T>::N;
+  if (__builtin_expect(far, 0)) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (sizeof(T) == 2) asm volatile("" : "+v"(x[k]));
+      float e[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) e[j] = __builtin_amdgcn_exp2f(shifted(raw_get<T>(x[k], j), m) * c);
+      take(k, e);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (sizeof(T) == 2) asm volatile("" : "+v"(x[k]));
+      float e[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(raw_get<T>(x[k], j), c, -mc));
+      take(k, e);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+// Waves a SIMD holds at once: what the registers of a row allow.
+#define ROW_WAVES(TPR, REGS, MODE) ((MODE) == TK_LOGP ? ((REGS) <= 16 ? 8 : 6) : (TPR) == 1024 ? ((REGS) <= 16 ? 8 : 4) : (REGS) <= 8 ? 6 : (REGS) <= 16 ? 5 : 4)
 
 // Rows that fit the registers of TPR lanes, NV packs a lane: the logits are read once, exponentiated once, and the policy
 // loss writes its gradient from the same registers.  TPR = 16 / 64: several rows a block and no barrier; 256 / 1024: one
 // row a block, whose waves take the maximum and sum of their own part and exchange the pair once.
 template <typename T, int TPR, int NV, int MODE>
-__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_token_rows(TokenRows a, PolicyIn p, RowOut o) {
-  constexpr int N = Pack<T>::N, NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR, NW = TPR / 64;
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)) void k_token_rows(TokenRows a, PolicyIn p, RowOut o) {
+  constexpr int N = Pack<T>::N, NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR, NW = TPR / 64, GRP = TPR < 64 ? TPR : 64;
+  constexpr bool KEEP = MODE == TK_POLICY && sizeof(T) == 4;   // the exponentials take the logits' registers
   __shared__ float2 sh[2][NW > 1 ? NW : 1];
   __shared__ double red[NT / 64];
-  const int r = threadIdx.x % TPR;
+  __shared__ double acc[MODE == TK_POLICY ? RPB : 1][3];
+  const int r = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x;
+  const int mine = TPR < 64 ? threadIdx.x / TPR : TPR == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0;
   const int V = a.V, nb = V / N, tail = V - nb * N;
-  double inv_total = 0.0, acc[3] = {0.0, 0.0, 0.0};
-  if constexpr (MODE == TK_POLICY) inv_total = inverse_total<NT>(p, red);
-  if (o.clear && blockIdx.x == 0 && threadIdx.x == 0) *o.clear = 0;
+  double inv_total = 0.0;
+  if constexpr (MODE == TK_POLICY) {
+    if (threadIdx.x < RPB * 3) acc[threadIdx.x / 3][threadIdx.x % 3] = 0.0;
+    inv_total = uniform(inverse_total<NT>(p, red));
+    __syncthreads();
+  }
   int parity = 0;
-  for (int64_t base = (int64_t)blockIdx.x * RPB; base < a.n; base += (int64_t)gridDim.x * RPB) {
-    const int64_t t = base + threadIdx.x / TPR;
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  RowScalars next = row_scalars<MODE>(a, p, o, (int64_t)blockIdx.x * RPB + mine);
+  for (int64_t base = (int64_t)blockIdx.x * RPB; base < a.n; base += step) {
+    const int64_t t = base + mine;
+    RowScalars c = next;
+    if constexpr (TPR >= 64) c = RowScalars{uniform(c.id), uniform(c.seq), uniform(c.old), uniform(c.ref)};
+    next = row_scalars<MODE>(a, p, o, t + step);
     if (TPR <= 64 && t >= a.n) continue;
-    int id = a.tok.at(t), seq = 0;
-    if constexpr (MODE == TK_POLICY) {
-      seq = p.seq_of[t];
-      if (seq < 0) id = -1;
-    }
-    if (id < 0) {
+    const int id = c.id;
+    if (id < 0 || c.seq < 0) {
       row_skip<T>(o, t, V, r, TPR, r == 0);
       continue;
     }
     const T* row = reinterpret_cast<const T*>(a.x) + t * a.stride;
-    float e[NV][N], et = -__builtin_inff();
+    u32x4 x[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if (r + k * TPR < nb) load_pack(row + (int64_t)(r + k * TPR) * N, e[k]);
-      else
-#pragma unroll
-        for (int j = 0; j < N; ++j) e[k][j] = -__builtin_inff();
+      x[k] = raw_minus_inf<T>();
+      if (r + k * TPR < nb) x[k] = load_raw(row + (int64_t)(r + k * TPR) * N);
     }
+    float et = -__builtin_inff();
     if (r < tail) et = (float)row[nb * N + r];
-    const float xt = (float)row[id];
+    float xt = (float)row[id];
     double w = 0.0;
-    if constexpr (MODE == TK_POLICY) w = row_weight(p, seq, inv_total);
+    float A = 0.f;
+    if constexpr (MODE == TK_POLICY) {
+      A = p.adv[p.adv_per_token ? t : (int64_t)c.seq];
+      w = row_weight(p, c.seq, inv_total);
+    }
     float m = et;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
-      for (int j = 0; j < N; ++j) m = fmaxf(m, e[k][j]);
-    m = group_max<(TPR < 64 ? TPR : 64)>(m);
-    const float mm = m == -__builtin_inff() ? 0.f : m;
-    float s = et = __builtin_amdgcn_exp2f((et - mm) * a.c);
+      for (int j = 0; j < N; ++j) m = fmaxf(m, raw_get<T>(x[k], j));
+    m = group_max<GRP>(m);
+    // this wave's own part: e = exp2(c x - mc)
+    const bool none = m == -__builtin_inff(), far = !none && far_out(m);
+    const float mc = none || far ? 0.f : m * a.c;
+    float s;
+    if (__builtin_expect(far, 0)) s = et = __builtin_amdgcn_exp2f(shifted(et, m) * a.c);
+    else s = et = __builtin_amdgcn_exp2f(fmaf(et, a.c, -mc));
+    exponentials<T, NV>(x, m, mc, a.c, far, [&](int k, float (&e)[N]) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int j = 0; j < N; ++j) s += e[k][j] = __builtin_amdgcn_exp2f((e[k][j] - mm) * a.c);
-    s = group_sum<(TPR < 64 ? TPR : 64)>(s);
-    float M = mm, S = s, f = 1.0f;
+      for (int j = 0; j < N; ++j) s += e[j];
+      if constexpr (KEEP) set_pack(x[k], e);
+    });
+    s = group_sum<GRP>(s);
+    float M = none ? 0.f : m, S = s, f = 1.0f;
     if constexpr (NW > 1) {
       // (the buffers alternate between rows: a wave that runs ahead writes the other one)
       if ((threadIdx.x & 63) == 0) sh[parity][threadIdx.x >> 6] = make_float2(m, s);
       __syncthreads();
-      M = -__builtin_inff();
-#pragma unroll
-      for (int i = 0; i < NW; ++i) M = fmaxf(M, sh[parity][i].x);
-      if (M == -__builtin_inff()) M = 0.f;
-      S = 0.f;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) S += sh[parity][i].y * __builtin_amdgcn_exp2f((sh[parity][i].x - M) * a.c);
-      f = __builtin_amdgcn_exp2f((mm - M) * a.c);
-      if (m == -__builtin_inff()) f = 0.f;
+      join_waves<NW>(sh[parity], a.c, M, S);
+      f = part_factor(m, M, a.c);
       parity ^= 1;
     }
-    const float inv_s = S == 0.f ? 0.f : 1.0f / S;
-    const float g = row_epilogue<MODE>(a, p, o, t, id, seq, xt, M, S, inv_s, r == 0, w, acc);
+    float inv_s = S == 0.f ? 0.f : 1.0f / S;
+    if constexpr (TPR >= 64) {
+      inv_s = uniform(inv_s);
+      xt = uniform(xt); M = uniform(M); S = uniform(S);
+      if constexpr (MODE == TK_POLICY) { A = uniform(A); w = uniform(w); }
+    }
+    float g = row_epilogue<MODE>(a, p, o, t, c, xt, M, S, inv_s, r == 0, A, w, acc[MODE == TK_POLICY ? mine : 0]);
+    if constexpr (TPR >= 64) g = uniform(g);
     if constexpr (MODE == TK_POLICY) {
       if (o.d == nullptr) continue;
       T* d = reinterpret_cast<T*>(o.d) + t * o.d_stride;
-      // a factor of 0 sends no gradient, also where the row holds a NaN
-      const float q = g == 0.f ? 0.f : -g * f * inv_s;
-      const int it = id / N;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int i = r + k * TPR;
-        if (i < nb) {
-          float v[N];
-#pragma unroll
-          for (int j = 0; j < N; ++j) v[j] = g == 0.f ? 0.f : q * e[k][j];
-          if (i == it) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] += j == id - it * N ? g : 0.f;
-          }
-          store_pack(d + (int64_t)i * N, v);
-        }
+      if (g == 0.f) {   // sends no gradient, also where the row holds a NaN
+        row_skip<T>(RowOut{nullptr, nullptr, nullptr, nullptr, o.d, o.d_stride}, t, V, r, TPR, false);
+        continue;
       }
-      if (r < tail) d[nb * N + r] = (T)((g == 0.f ? 0.f : q * et) + (nb * N + r == id ? g : 0.f));
+      const float q = -g * f * inv_s;
+      const int it = id / N;
+      const auto out = [&](int k, float (&e)[N]) {
+        const int i = r + k * TPR;
+#pragma unroll
+        for (int j = 0; j < N; ++j) e[j] *= q;
+        if (i == it) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) e[j] += j == id - it * N ? g : 0.f;
+        }
+        if (i < nb) store_pack(d + (int64_t)i * N, e);
+      };
+      if constexpr (KEEP) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          float e[N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) e[j] = raw_get<T>(x[k], j);
+          out(k, e);
+        }
+      } else {
+        exponentials<T, NV>(x, m, mc, a.c, far, out);
+      }
+      if (r < tail) d[nb * N + r] = (T)(q * et + (nb * N + r == id ? g : 0.f));
     }
   }
-  if constexpr (MODE == TK_POLICY) {
-    if (r != 0) acc[0] = acc[1] = acc[2] = 0.0;
-    policy_finish<NT>(p, acc, red);
+  if constexpr (MODE == TK_POLICY) policy_partial<RPB>(p, acc);
+}
+
+// One row's gradient from its logits, maximum and 1 / sum, by TPR lanes: g ([v = id] - p[v]).  A factor of 0 sends no
+// gradient, also where the row holds a NaN, and a row of -inf only (1 / sum is 0) has none.
+template <typename T, int TPR>
+__device__ __forceinline__ void row_gradient(const TokenRows& a, const T* row, T* d, int id, int r, float M, float inv_s, float g) {
+  constexpr int N = Pack<T>::N;
+  const int V = a.V, nb = V / N, tail = V - nb * N;
+  const bool off = g == 0.f || inv_s == 0.f, far = far_out(M);
+  const float mc = far ? 0.f : M * a.c, q = -g * inv_s;
+  const int it = id / N;
+  if (off) {
+    const float z[N] = {};
+    for (int i = r; i < nb; i += TPR) store_pack(d + (int64_t)i * N, z);
+    if (r < tail) d[nb * N + r] = (T)0.f;
+    return;
+  }
+#pragma unroll 4
+  for (int i = r; i < nb; i += TPR) {
+    float v[N];
+    load_pack(row + (int64_t)i * N, v);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = q * __builtin_amdgcn_exp2f(fmaf(far ? shifted(v[j], M) : v[j], a.c, -mc));
+    if (i == it) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] += j == id - it * N ? g : 0.f;
+    }
+    store_pack(d + (int64_t)i * N, v);
+  }
+  if (r < tail) {
+    const int v = nb * N + r;
+    const float x = (float)row[v];
+    d[v] = (T)(q * __builtin_amdgcn_exp2f(fmaf(far ? shifted(x, M) : x, a.c, -mc)) + (v == id ? g : 0.f));
   }
 }
 
@@ -281,78 +424,64 @@ __global__ __launch_bounds__(1024) void k_token_rows_long(TokenRows a, PolicyIn 
   __shared__ double red[NW];
   const int r = threadIdx.x;
   const int V = a.V, nb = V / N, tail = V - nb * N;
-  double inv_total = 0.0, acc[3] = {0.0, 0.0, 0.0};
-  if constexpr (MODE == TK_POLICY) inv_total = inverse_total<NT>(p, red);
-  if (o.clear && blockIdx.x == 0 && threadIdx.x == 0) *o.clear = 0;
+  __shared__ double acc[1][3];
+  double inv_total = 0.0;
+  if constexpr (MODE == TK_POLICY) {
+    if (threadIdx.x < 3) acc[0][threadIdx.x] = 0.0;
+    inv_total = uniform(inverse_total<NT>(p, red));
+    __syncthreads();
+  }
   int parity = 0;
   for (int64_t t = blockIdx.x; t < a.n; t += gridDim.x) {
-    int id = a.tok.at(t), seq = 0;
-    if constexpr (MODE == TK_POLICY) {
-      seq = p.seq_of[t];
-      if (seq < 0) id = -1;
-    }
-    if (id < 0) {
+    const RowScalars c = row_scalars<MODE>(a, p, o, t);
+    const int id = c.id;
+    if (id < 0 || c.seq < 0) {
       row_skip<T>(o, t, V, r, NT, r == 0);
       continue;
     }
     const T* row = reinterpret_cast<const T*>(a.x) + t * a.stride;
     const float xt = (float)row[id];
     double w = 0.0;
-    if constexpr (MODE == TK_POLICY) w = row_weight(p, seq, inv_total);
-    float m = -__builtin_inff(), s = 0.f;
-    const auto take = [&](float mx, const float* v, int n) {
-      const float nm = fmaxf(m, mx), z = nm == -__builtin_inff() ? 0.f : nm;
-      if (m != -__builtin_inff()) s *= __builtin_amdgcn_exp2f((m - z) * a.c);
-      for (int j = 0; j < n; ++j) s += __builtin_amdgcn_exp2f((v[j] - z) * a.c);
-      m = nm;
-    };
-    for (int i = r; i < nb; i += NT) {
+    float A = 0.f;
+    if constexpr (MODE == TK_POLICY) {
+      A = p.adv[p.adv_per_token ? t : (int64_t)c.seq];
+      w = row_weight(p, c.seq, inv_total);
+    }
+    float m = -__builtin_inff(), s = 0.f;   // of this lane: s relative to m
+    for (int i = r; i < nb + (r < tail ? NT : 0); i += NT) {
       float v[N];
-      load_pack(row + (int64_t)i * N, v);
+      if (i < nb) load_pack(row + (int64_t)i * N, v);
+      else {   // one element of the tail
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = -__builtin_inff();
+        v[0] = (float)row[nb * N + r];
+      }
       float mx = v[0];
 #pragma unroll
       for (int j = 1; j < N; ++j) mx = fmaxf(mx, v[j]);
-      take(mx, v, N);
+      if (mx > m) {
+        s *= part_factor(m, mx, a.c);
+        m = mx;
+      }
+      const bool none = m == -__builtin_inff(), far = !none && far_out(m);
+      const float mc = none || far ? 0.f : m * a.c;
+#pragma unroll
+      for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f(fmaf(far ? shifted(v[j], m) : v[j], a.c, -mc));
     }
-    if (r < tail) {
-      const float v = (float)row[nb * N + r];
-      take(v, &v, 1);
-    }
-    const float wm = group_max<64>(m), wmm = wm == -__builtin_inff() ? 0.f : wm;
-    s = group_sum<64>(m == -__builtin_inff() ? s : s * __builtin_amdgcn_exp2f((m - wmm) * a.c));
+    const float wm = group_max<64>(m);
+    s = group_sum<64>(s * part_factor(m, wm == -__builtin_inff() ? 0.f : wm, a.c));
     if ((threadIdx.x & 63) == 0) sh[parity][threadIdx.x >> 6] = make_float2(wm, s);
     __syncthreads();
-    float M = -__builtin_inff(), S = 0.f;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) M = fmaxf(M, sh[parity][i].x);
-    if (M == -__builtin_inff()) M = 0.f;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) S += sh[parity][i].y * __builtin_amdgcn_exp2f((sh[parity][i].x - M) * a.c);
+    float M, S;
+    join_waves<NW>(sh[parity], a.c, M, S);
     parity ^= 1;
     const float inv_s = S == 0.f ? 0.f : 1.0f / S;
-    const float g = row_epilogue<MODE>(a, p, o, t, id, seq, xt, M, S, inv_s, r == 0, w, acc);
+    const float g = row_epilogue<MODE>(a, p, o, t, c, xt, M, S, inv_s, r == 0, A, w, acc[0]);
     if constexpr (MODE == TK_POLICY) {
-      if (o.d == nullptr) continue;
-      T* d = reinterpret_cast<T*>(o.d) + t * o.d_stride;
-      const float q = -g * inv_s;
-      for (int i = r; i < nb; i += NT) {
-        float v[N];
-        load_pack(row + (int64_t)i * N, v);
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          v[j] = g == 0.f ? 0.f : q * __builtin_amdgcn_exp2f((v[j] - M) * a.c) + (i * N + j == id ? g : 0.f);
-        store_pack(d + (int64_t)i * N, v);
-      }
-      if (r < tail) {
-        const int v = nb * N + r;
-        d[v] = (T)(g == 0.f ? 0.f : q * __builtin_amdgcn_exp2f(((float)row[v] - M) * a.c) + (v == id ? g : 0.f));
-      }
+      if (o.d) row_gradient<T, NT>(a, row, reinterpret_cast<T*>(o.d) + t * o.d_stride, id, r, M, inv_s, g);
     }
   }
-  if constexpr (MODE == TK_POLICY) {
-    if (r != 0) acc[0] = acc[1] = acc[2] = 0.0;
-    policy_finish<NT>(p, acc, red);
-  }
+  if constexpr (MODE == TK_POLICY) policy_partial<1>(p, acc);
 }
 
 // d_logits[t, v] = coef mult upstream / temperature ([v = id_t] - p[t, v]) from the saved maximum and 1 / sum: no reduction,
@@ -360,77 +489,98 @@ __global__ __launch_bounds__(1024) void k_token_rows_long(TokenRows a, PolicyIn 
 template <typename T, int TPR>
 __global__ __launch_bounds__(256) void k_token_grad(TokenRows a, const float* __restrict__ stats, const float* __restrict__ coef,
                                                     const int32_t* __restrict__ index, int64_t n_coef, float mult, const float* __restrict__ upstream, T* __restrict__ d, int64_t d_stride) {
-  constexpr int N = Pack<T>::N, RPB = 256 / TPR;
+  constexpr int RPB = 256 / TPR;
   const int r = threadIdx.x % TPR;
-  const int V = a.V, nb = V / N, tail = V - nb * N;
   const double k = (double)mult * a.inv_t * (upstream ? (double)*upstream : 1.0);
   for (int64_t t = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; t < a.n; t += (int64_t)gridDim.x * RPB) {
     const int id = a.tok.at(t);
     const int64_t ci = index ? (int64_t)index[t] : t;
     const float g = id < 0 || ci < 0 || ci >= n_coef ? 0.f : (float)((double)coef[ci] * k);
-    T* out = d + t * d_stride;
-    if (g == 0.f || stats[2 * t + 1] == 0.f) {   // sends no gradient, also where the row holds a NaN; or -inf only
-      row_skip<T>(RowOut{nullptr, nullptr, nullptr, nullptr, d, d_stride, nullptr}, t, V, r, TPR, false);
-      continue;
-    }
-    const float M = stats[2 * t], q = -g * stats[2 * t + 1];
-    const T* row = reinterpret_cast<const T*>(a.x) + t * a.stride;
-    const int it = id / N;
-#pragma unroll 4
-    for (int i = r; i < nb; i += TPR) {
-      float v[N];
-      load_pack(row + (int64_t)i * N, v);
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = q * __builtin_amdgcn_exp2f((v[j] - M) * a.c);
-      if (i == it) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] += j == id - it * N ? g : 0.f;
-      }
-      store_pack(out + (int64_t)i * N, v);
-    }
-    if (r < tail) {
-      const int v = nb * N + r;
-      out[v] = (T)(q * __builtin_amdgcn_exp2f(((float)row[v] - M) * a.c) + (v == id ? g : 0.f));
-    }
+    row_gradient<T, TPR>(a, reinterpret_cast<const T*>(a.x) + t * a.stride, d + t * d_stride, id, r, stats[2 * t],
+                         g == 0.f ? 0.f : stats[2 * t + 1], g);
   }
 }
 
-// Rows in chunks of SEG_ROWS, one block a chunk: the sequence of each row by bisection of seq_ptr (bounded whatever
-// seq_ptr holds; -1 for ignored rows and rows outside every sequence), the chunk's number of taking rows, and for every
+// Rows in chunks of SEG_ROWS, one block a chunk: the sequence of each row (-1 for ignored rows and rows outside every
+// sequence), the chunk's number of taking rows, and for every
 // sequence that meets the chunk the sum and the number of its rows in it, from prefix sums in 64 bits.  What sequence s has
 // in chunk c goes to place c + s: both grow along the rows, so no two parts share a place.  A sequence of any length is
 // then the sum of its parts, and no block waits for one long sequence.
 #define SEG_ROWS 1024
-__device__ __forceinline__ int seq_at(const int32_t* __restrict__ seq_ptr, int lo, int hi, int64_t t) {
-  // the last s in [lo, hi] with seq_ptr[s] <= t, lo - 1 if there is none
-  while (lo <= hi) {
-    const int mid = (int)(((int64_t)lo + hi) >> 1);
-    if ((int64_t)seq_ptr[mid] <= t) lo = mid + 1; else hi = mid - 1;
+// The number of seq_ptr[0 .. n) that are <= t, by a whole wave: 64 probes a step.  (In 32 bits: n <= 2^31, a probe lies
+// below 2^31 + 2^25.  The compiler's scalar code for the 64-bit form selects by a stale condition bit.)
+__device__ __forceinline__ uint32_t wave_count_upto(const int32_t* __restrict__ seq_ptr, uint32_t n, int32_t t) {
+  uint32_t lo = 0, hi = n;     // the answer lies in [lo, hi], which shrinks to 1/64 a step whatever seq_ptr holds
+  while (lo < hi) {
+    const uint32_t step = (hi - lo + 63) >> 6, at = lo + ((threadIdx.x & 63) + 1) * step - 1;
+    const uint64_t below = __ballot(at < hi && seq_ptr[at < hi ? at : lo] <= t);
+    const uint32_t k = (uint32_t)__popcll(below), next = lo + (k + 1) * step - 1;
+    lo += k * step;
+    hi = next < hi ? next : hi;
+    hi = hi < lo ? lo : hi;
   }
-  return hi;
+  return lo;
 }
 template <bool SUM>
 __global__ __launch_bounds__(256) void k_row_segments(TokenView tok, int64_t n, const int32_t* __restrict__ seq_ptr, int32_t S,
                                                       const float* __restrict__ diff, int32_t* __restrict__ seq_of,
                                                       double* __restrict__ part_sum, int32_t* __restrict__ part_len,
-                                                      int32_t* __restrict__ chunk_len, uint32_t* __restrict__ clear) {
+                                                      int32_t* __restrict__ chunk_len) {
   __shared__ double pre[SUM ? SEG_ROWS + 1 : 1];
   __shared__ int cnt[SEG_ROWS + 1];
   __shared__ double wsum[4];
-  __shared__ int wcnt[4];
+  __shared__ int wcnt[4], wmax[4], ends[2];
+  int* const mark = cnt;   // (the counts replace the marks once every thread has read its own)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (clear && blockIdx.x == 0 && tid == 0) *clear = 0;
   const int64_t c = blockIdx.x, c0 = c * SEG_ROWS;
   const int rows = (int)(n - c0 < SEG_ROWS ? n - c0 : SEG_ROWS);
-  const int64_t first = seq_ptr ? seq_ptr[0] : 0, last = seq_ptr ? seq_ptr[S] : n;
-  double v[4];
+  bool on[4];
+  float d[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {   // (loads of a place that exists, so that all of them are under way at once)
+    const int i = tid * 4 + j;
+    const int64_t at = c0 + (i < rows ? i : rows - 1);
+    on[j] = (tok.at(at) >= 0) & (i < rows);
+    d[j] = SUM ? diff[at] : 0.f;
+  }
+  // sequences of the chunk's first and last row (-1: before the first, S: behind the last)
+  if (seq_ptr && wave < 2) {
+    const int k = (int)wave_count_upto(seq_ptr, (uint32_t)S + 1u, (int32_t)(wave ? c0 + rows - 1 : c0)) - 1;
+    if (lane == 0) ends[wave] = k;
+  }
+  if (!seq_ptr && tid < 2) ends[tid] = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) mark[tid * 4 + j] = -1;
+  __syncthreads();
+  const int s0 = ends[0], s1 = ends[1], sa = s0 < 0 ? 0 : s0;
+  // a row's sequence is the last that starts at or before it: starts are marked, then a running maximum
+  if (seq_ptr)
+    for (int64_t s = (int64_t)sa + tid; s <= s1; s += 256) {
+      const int64_t at = seq_ptr[s] - c0;
+      if (at >= 0 && at < rows) atomicMax(&mark[at], (int)s);
+    }
+  __syncthreads();
+  int m[4], top = s0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { const int v = mark[tid * 4 + j]; top = v > top ? v : top; m[j] = top; }
+  int run = top;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(run, o); if (lane >= o && u > run) run = u; }
+  if (lane == 63) wmax[wave] = run;
+  int before = __shfl_up(run, 1);
+  if (lane == 0) before = s0;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) before = wmax[w] > before ? wmax[w] : before;
   int k[4];
+  double v[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
+    m[j] = before > m[j] ? before : m[j];
+    if (!on[j] || m[j] >= S) m[j] = -1;
+    k[j] = m[j] >= 0;
+    v[j] = SUM && k[j] ? (double)d[j] : 0.0;
     const int i = tid * 4 + j;
-    const int64_t t = c0 + i;
-    k[j] = i < rows && t >= first && t < last && tok.at(t) >= 0;
-    v[j] = SUM && k[j] ? (double)diff[t] : 0.0;
+    if (i < rows) seq_of[c0 + i] = m[j];
   }
   int ci = (k[0] + k[1]) + (k[2] + k[3]);
   double vi = (v[0] + v[1]) + (v[2] + v[3]);
@@ -456,17 +606,8 @@ __global__ __launch_bounds__(256) void k_row_segments(TokenView tok, int64_t n, 
   }
   __syncthreads();
   if (tid == 0 && chunk_len) chunk_len[c] = cnt[rows];
-  const int s0 = seq_ptr ? seq_at(seq_ptr, 0, S, c0) : 0, s1 = seq_ptr ? seq_at(seq_ptr, 0, S, c0 + rows - 1) : 0;
-  for (int i = tid; i < rows; i += 256) {
-    int s = -1;
-    if (cnt[i + 1] != cnt[i]) {
-      s = seq_ptr ? seq_at(seq_ptr, s0 < 0 ? 0 : s0, s1, c0 + i) : 0;
-      if (s >= S) s = -1;
-    }
-    seq_of[c0 + i] = s;
-  }
   if (!part_len) return;
-  for (int64_t s = (int64_t)(s0 < 0 ? 0 : s0) + tid; s <= s1 && s < S; s += 256) {
+  for (int64_t s = (int64_t)sa + tid; s <= s1 && s < S; s += 256) {
     const int64_t t0 = seq_ptr ? seq_ptr[s] : 0, t1 = seq_ptr ? seq_ptr[s + 1] : n;
     const int a = t0 <= c0 ? 0 : t0 - c0 < rows ? (int)(t0 - c0) : rows;
     const int b = t1 <= c0 ? 0 : t1 - c0 < rows ? (int)(t1 - c0) : rows;
@@ -511,12 +652,11 @@ struct PrefIn {
   float beta, smooth;
   int32_t kind, average;
   double denom, grad_scale;
-  float* loss; float* log_ratio; float* margin; float* slope;
+  float* log_ratio; float* margin; float* slope;
   double* partial;          // [gridDim.x]
-  uint32_t* counter;
 };
 // Pairs: sequence p is preferred over sequence P + p.  A wave joins both sequences' differences (a margin is what two long
-// sums leave: 64 bits), forms the loss and d loss / d logp of either sequence's rows; the last block adds the losses.
+// sums leave: 64 bits), forms the loss and d loss / d logp of either sequence's rows.
 __global__ __launch_bounds__(256) void k_preference(PrefIn a) {
   __shared__ double red[4];
   const int lane = threadIdx.x & 63;
@@ -555,15 +695,17 @@ __global__ __launch_bounds__(256) void k_preference(PrefIn a) {
   }
   total = block_sum<256>(total, red);
   if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
-  if (!last_block(a.counter)) return;
+}
+__global__ __launch_bounds__(256) void k_preference_final(const double* __restrict__ partial, int blocks, double denom, float* __restrict__ loss) {
+  __shared__ double red[4];
   double v = 0.0;
-  for (int b = threadIdx.x; b < (int)gridDim.x; b += 256) v += a.partial[b];
+#pragma unroll 4
+  for (int b = threadIdx.x; b < blocks; b += 256) v += partial[b];
   v = block_sum<256>(v, red);
-  if (threadIdx.x == 0) a.loss[0] = (float)(v / a.denom);
+  if (threadIdx.x == 0) *loss = (float)(v / denom);
 }
 
 // An empty batch: no row kernel runs.
-__global__ void k_clear(uint32_t* counter) { if (threadIdx.x == 0) *counter = 0; }
 __global__ void k_empty_policy(float* result) { if (threadIdx.x < 4) result[threadIdx.x] = 0.f; }
 
 // ------------------------------------------------------------------ host side
@@ -571,35 +713,38 @@ __global__ void k_empty_policy(float* result) { if (threadIdx.x < 4) result[thre
 // added up by one block.
 static int row_grid(int64_t groups, int most) { return (int)(groups < most ? groups : most); }
 
-template <typename T, int TPR, int NV, int MODE>
-static void launch_rows_as(const TokenRows& a, const PolicyIn& p, const RowOut& o, int grid_cap, hipStream_t s) {
-  constexpr int NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR;
-  const int grid = row_grid((a.n + RPB - 1) / RPB, grid_cap);
-  hipLaunchKernelGGL((k_token_rows<T, TPR, NV, MODE>), dim3(grid), dim3(NT), 0, s, a, p, o);
-}
 #define TK_GRID_CAP 2048
-// The least lanes whose registers hold a row: 16 lanes up to 64 packs, a wave up to 512, 256 lanes up to 2048, 1024 up to
-// 8192 (32768 fp32 or 65536 half-precision logits); beyond that the row is read twice.
-template <typename T, int MODE>
-static void launch_rows(const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
-  const int packs = a.V / Pack<T>::N;
-  if (packs <= 16) launch_rows_as<T, 16, 1, MODE>(a, p, o, TK_GRID_CAP, s);
-  else if (packs <= 32) launch_rows_as<T, 16, 2, MODE>(a, p, o, TK_GRID_CAP, s);
-  else if (packs <= 64) launch_rows_as<T, 16, 4, MODE>(a, p, o, TK_GRID_CAP, s);
-  else if (packs <= 128) launch_rows_as<T, 64, 2, MODE>(a, p, o, TK_GRID_CAP, s);
-  else if (packs <= 256) launch_rows_as<T, 64, 4, MODE>(a, p, o, TK_GRID_CAP, s);
-  else if (packs <= 512) launch_rows_as<T, 64, 8, MODE>(a, p, o, TK_GRID_CAP, s);
-  else if (packs <= 1024) launch_rows_as<T, 256, 4, MODE>(a, p, o, TK_GRID_CAP, s);
-  else if (packs <= 2048) launch_rows_as<T, 256, 8, MODE>(a, p, o, TK_GRID_CAP, s);
-  else if (packs <= 4096) launch_rows_as<T, 1024, 4, MODE>(a, p, o, TK_GRID_CAP, s);
-  else if (packs <= 8192) launch_rows_as<T, 1024, 8, MODE>(a, p, o, TK_GRID_CAP, s);
-  else hipLaunchKernelGGL((k_token_rows_long<T, MODE>), dim3(row_grid(a.n, TK_GRID_CAP)), dim3(1024), 0, s, a, p, o);
+template <typename T, int TPR, int NV, int MODE>
+static int launch_rows_as(const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
+  constexpr int NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR;
+  const int grid = row_grid((a.n + RPB - 1) / RPB, TK_GRID_CAP * 256 / NT);
+  hipLaunchKernelGGL((k_token_rows<T, TPR, NV, MODE>), dim3(grid), dim3(NT), 0, s, a, p, o);
+  return grid;
 }
-template <int MODE> static void launch_rows_dtype(int dtype, const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
-  if (a.n == 0) return;
-  if (dtype == LIGDIFF_F32) launch_rows<float, MODE>(a, p, o, s);
-  else if (dtype == LIGDIFF_BF16) launch_rows<bf16_t, MODE>(a, p, o, s);
-  else launch_rows<f16_t, MODE>(a, p, o, s);
+// The least lanes whose registers hold a row: 16 lanes up to 64 packs, a wave up to 512, 256 lanes up to 2048, 1024 up to
+// 8192 (32768 fp32 or 65536 half-precision logits); beyond that the row is read twice.  Returns the number of blocks.
+template <typename T, int MODE>
+static int launch_rows(const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
+  const int packs = a.V / Pack<T>::N;
+  if (packs <= 16) return launch_rows_as<T, 16, 1, MODE>(a, p, o, s);
+  if (packs <= 32) return launch_rows_as<T, 16, 2, MODE>(a, p, o, s);
+  if (packs <= 64) return launch_rows_as<T, 16, 4, MODE>(a, p, o, s);
+  if (packs <= 128) return launch_rows_as<T, 64, 2, MODE>(a, p, o, s);
+  if (packs <= 256) return launch_rows_as<T, 64, 4, MODE>(a, p, o, s);
+  if (packs <= 512) return launch_rows_as<T, 64, 8, MODE>(a, p, o, s);
+  if (packs <= 1024) return launch_rows_as<T, 256, 4, MODE>(a, p, o, s);
+  if (packs <= 2048) return launch_rows_as<T, 256, 8, MODE>(a, p, o, s);
+  if (packs <= 4096) return launch_rows_as<T, 1024, 4, MODE>(a, p, o, s);
+  if (packs <= 8192) return launch_rows_as<T, 1024, 8, MODE>(a, p, o, s);
+  const int grid = row_grid(a.n, TK_GRID_CAP);
+  hipLaunchKernelGGL((k_token_rows_long<T, MODE>), dim3(grid), dim3(1024), 0, s, a, p, o);
+  return grid;
+}
+template <int MODE> static int launch_rows_dtype(int dtype, const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
+  if (a.n == 0) return 0;
+  if (dtype == LIGDIFF_F32) return launch_rows<float, MODE>(a, p, o, s);
+  if (dtype == LIGDIFF_BF16) return launch_rows<bf16_t, MODE>(a, p, o, s);
+  return launch_rows<f16_t, MODE>(a, p, o, s);
 }
 template <typename T>
 static void launch_grad(const TokenRows& a, const float* stats, const float* coef, const int32_t* index, int64_t n_coef, float mult, const float* up, void* d,
@@ -639,7 +784,7 @@ extern "C" int ligdiff_token_logprob(const ligdiff_token_args* args, float* logp
   const int rc = fill_rows(&a, args);
   if (rc) return rc;
   if (a.n > 0 && !logp) return LIGDIFF_ERR_ARG;
-  launch_rows_dtype<TK_LOGP>(args->dtype, a, PolicyIn{}, RowOut{logp, nullptr, stats, nullptr, nullptr, 0, nullptr}, (hipStream_t)stream);
+  launch_rows_dtype<TK_LOGP>(args->dtype, a, PolicyIn{}, RowOut{logp, nullptr, stats, nullptr, nullptr, 0}, (hipStream_t)stream);
   LD_CHECK_LAUNCH();
   return LIGDIFF_OK;
 }
@@ -668,12 +813,11 @@ struct Pieces {
   }
 };
 #define PREF_BLOCKS 1024
-struct PrefWs { uint32_t* counter; double* partial; float* diff; double* part_sum; int32_t* part_len; size_t bytes; };
+struct PrefWs { double* partial; float* diff; double* part_sum; int32_t* part_len; size_t bytes; };
 static PrefWs pref_ws(void* base, int64_t n, int32_t P) {
   Pieces w{(char*)base};
   const size_t parts = (size_t)(seg_chunks(n) + 2 * (int64_t)P);
   PrefWs r;
-  r.counter = w.take<uint32_t>(1);
   r.partial = w.take<double>(PREF_BLOCKS);
   r.diff = w.take<float>((size_t)n);
   r.part_sum = w.take<double>(parts);
@@ -701,31 +845,30 @@ extern "C" int ligdiff_preference_loss(const ligdiff_token_args* args, const lig
   if (q->workspace_bytes < w.bytes) return LIGDIFF_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   if (a.n > 0) {
-    launch_rows_dtype<TK_LOGP>(args->dtype, a, PolicyIn{}, RowOut{w.diff, q->ref_logp, q->stats, nullptr, nullptr, 0, w.counter}, s);
+    launch_rows_dtype<TK_LOGP>(args->dtype, a, PolicyIn{}, RowOut{w.diff, q->ref_logp, q->stats, nullptr, nullptr, 0}, s);
     hipLaunchKernelGGL((k_row_segments<true>), dim3((unsigned)seg_chunks(a.n)), dim3(256), 0, s, a.tok, a.n, q->seq_ptr,
-                       2 * q->n_pairs, w.diff, q->row_seq, w.part_sum, w.part_len, (int32_t*)nullptr, (uint32_t*)nullptr);
-  } else {
-    hipLaunchKernelGGL(k_clear, dim3(1), dim3(64), 0, s, w.counter);
+                       2 * q->n_pairs, w.diff, q->row_seq, w.part_sum, w.part_len, (int32_t*)nullptr);
   }
   PrefIn p;
   p.n = a.n; p.seq_ptr = q->seq_ptr; p.P = q->n_pairs; p.part_sum = w.part_sum; p.part_len = w.part_len;
   p.beta = q->beta; p.smooth = q->label_smoothing; p.kind = q->kind; p.average = q->average != 0;
   p.denom = q->denominator > 0.f ? (double)q->denominator : (double)q->n_pairs;
   p.grad_scale = (double)q->grad_scale;
-  p.loss = q->loss; p.log_ratio = q->log_ratio; p.margin = q->margin; p.slope = q->slope;
-  p.partial = w.partial; p.counter = w.counter;
-  hipLaunchKernelGGL(k_preference, dim3(row_grid(((int64_t)q->n_pairs + 3) / 4, PREF_BLOCKS)), dim3(256), 0, s, p);
+  p.log_ratio = q->log_ratio; p.margin = q->margin; p.slope = q->slope;
+  p.partial = w.partial;
+  const int blocks = row_grid(((int64_t)q->n_pairs + 3) / 4, PREF_BLOCKS);
+  hipLaunchKernelGGL(k_preference, dim3(blocks), dim3(256), 0, s, p);
+  hipLaunchKernelGGL(k_preference_final, dim3(1), dim3(256), 0, s, w.partial, blocks, p.denom, q->loss);
   if (q->d_logits)
     launch_grad_dtype(args->dtype, a, q->stats, q->slope, q->row_seq, 2 * (int64_t)q->n_pairs, 1.0f, nullptr, q->d_logits, q->d_stride, s);
   LD_CHECK_LAUNCH();
   return LIGDIFF_OK;
 }
 
-struct PolicyWs { uint32_t* counter; double* partial; int32_t* chunk_len; int32_t* seq_of; int32_t* part_len; int32_t* seq_len; size_t bytes; };
+struct PolicyWs { double* partial; int32_t* chunk_len; int32_t* seq_of; int32_t* part_len; int32_t* seq_len; size_t bytes; };
 static PolicyWs policy_ws(void* base, int64_t n, int32_t S, bool per_seq) {
   Pieces w{(char*)base};
   PolicyWs r;
-  r.counter = w.take<uint32_t>(1);
   r.partial = w.take<double>(TK_GRID_CAP * 3);
   r.chunk_len = w.take<int32_t>((size_t)seg_chunks(n));
   r.seq_of = w.take<int32_t>((size_t)n);
@@ -760,7 +903,7 @@ extern "C" int ligdiff_policy_loss(const ligdiff_token_args* args, const ligdiff
   }
   const int chunks = (int)seg_chunks(a.n);
   hipLaunchKernelGGL((k_row_segments<false>), dim3(chunks), dim3(256), 0, s, a.tok, a.n, q->seq_ptr, q->n_seq, (const float*)nullptr,
-                     w.seq_of, (double*)nullptr, per_seq ? w.part_len : nullptr, w.chunk_len, w.counter);
+                     w.seq_of, (double*)nullptr, per_seq ? w.part_len : nullptr, w.chunk_len);
   if (per_seq)
     hipLaunchKernelGGL(k_sequence_lengths, dim3(ceil_div(q->n_seq, 4)), dim3(256), 0, s, q->seq_ptr, a.n, q->n_seq, w.part_len, w.seq_len);
   PolicyIn p;
@@ -769,8 +912,9 @@ extern "C" int ligdiff_policy_loss(const ligdiff_token_args* args, const ligdiff
   p.adv = q->advantage; p.adv_per_token = q->advantage_per_token != 0;
   p.old_logp = q->old_logp; p.ref_logp = q->ref_logp;
   p.clip_lo = q->clip_low; p.clip_hi = q->clip_high; p.kl_coef = q->kl_coef; p.grad_scale = q->grad_scale;
-  p.partial = w.partial; p.counter = w.counter; p.result = q->result;
-  launch_rows_dtype<TK_POLICY>(args->dtype, a, p, RowOut{q->logp, nullptr, q->stats, q->coef, q->d_logits, q->d_stride, nullptr}, s);
+  p.partial = w.partial;
+  const int blocks = launch_rows_dtype<TK_POLICY>(args->dtype, a, p, RowOut{q->logp, nullptr, q->stats, q->coef, q->d_logits, q->d_stride}, s);
+  hipLaunchKernelGGL(k_policy_final, dim3(1), dim3(256), 0, s, w.partial, blocks, (double)q->kl_coef, q->result);
   LD_CHECK_LAUNCH();
   return LIGDIFF_OK;
 }
