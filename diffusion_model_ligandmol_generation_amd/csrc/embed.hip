@@ -19,20 +19,19 @@ __global__ __launch_bounds__(256) void k_embed(const T* __restrict__ table, int6
 #pragma unroll
     for (int u = 0; u < RU; ++u) id[u] = t0 + u < n ? tok.at(t0 + u) : -1;
     for (int i = r; i < nb; i += TPR) {
-      float v[RU][N];
+      u32x4 v[RU];
 #pragma unroll
       for (int u = 0; u < RU; ++u) {
-        if (id[u] >= 0) load_pack(table + id[u] * row_stride + (int64_t)i * N, v[u]);
-        else
-#pragma unroll
-          for (int j = 0; j < N; ++j) v[u][j] = 0.f;
+        v[u] = u32x4{0, 0, 0, 0};
+        if (id[u] >= 0) v[u] = load_raw(table + id[u] * row_stride + (int64_t)i * N);
       }
 #pragma unroll
       for (int u = 0; u < RU; ++u)
         if (t0 + u < n) {
+          float f[N];
 #pragma unroll
-          for (int j = 0; j < N; ++j) v[u][j] = id[u] >= 0 ? v[u][j] * scale : 0.f;
-          store_pack(out + (t0 + u) * out_stride + (int64_t)i * N, v[u]);
+          for (int j = 0; j < N; ++j) f[j] = raw_get<T>(v[u], j) * scale;
+          store_pack(out + (t0 + u) * out_stride + (int64_t)i * N, f);
         }
     }
     if (r < tail)
@@ -199,11 +198,12 @@ struct SegIn {
   int32_t* row_ptr; bool have_ptr;
   int32_t rows, D, R, n_chunks, n_tiles;
   float scale;
-  float* part;                               // [n_chunks][2][D]
+  float* part;                               // [n_chunks][2][D], a chunk here SUM_WAVES * R positions
   void* d_table; int64_t t_stride;
   bool accumulate;
   int32_t zero_blocks;
 };
+#define SUM_WAVES 8
 #define ZERO_ROWS 64   // rows of the table a block of the first part looks after
 
 template <typename TO> __device__ __forceinline__ void put(TO* p, float v, bool add) { *p = (TO)(add ? (float)*p + v : v); }
@@ -223,15 +223,17 @@ template <typename TO, int N> __device__ __forceinline__ void put_columns(TO* p,
 }
 
 // Blocks [0, zero_blocks): find where each token's positions start (bisection, unless the sort wrote it) and write the rows
-// of tokens that do not occur.  The other blocks: one wave a chunk of R sorted positions and 64 packs of columns.
+// of tokens that do not occur.  The other blocks: SUM_WAVES chunks of R sorted positions and 64 packs of columns, a wave a chunk.  A wave
+// writes the tokens that lie inside its chunk; the first and the last, which may go on in the neighbours', meet in LDS, and
+// only what goes on beyond the block's chunks leaves it as a partial row: slot 0 the block's first token, slot 1 its last.
 template <typename T, typename TO>
-__global__ __launch_bounds__(256) void k_segment_sums(SegIn a) {
-  constexpr int N = Pack<T>::N, U = 8;
+__global__ __launch_bounds__(SUM_WAVES * 64) void k_segment_sums(SegIn a) {
+  constexpr int N = Pack<T>::N, U = 8, NT = SUM_WAVES * 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((int)blockIdx.x < a.zero_blocks) {
     __shared__ int ptr[ZERO_ROWS + 1];
     const int v0 = blockIdx.x * ZERO_ROWS;
-    for (int k = threadIdx.x; k <= ZERO_ROWS; k += 256) {
+    for (int k = threadIdx.x; k <= ZERO_ROWS; k += NT) {
       const int64_t v = (int64_t)v0 + k;
       if (v > a.rows) continue;
       int p;
@@ -249,7 +251,7 @@ __global__ __launch_bounds__(256) void k_segment_sums(SegIn a) {
     }
     __syncthreads();
     if (a.accumulate) return;
-    for (int k = wave; k < ZERO_ROWS && v0 + k < a.rows; k += 4) {
+    for (int k = wave; k < ZERO_ROWS && v0 + k < a.rows; k += SUM_WAVES) {
       if (ptr[k + 1] != ptr[k]) continue;
       TO* row = reinterpret_cast<TO*>(a.d_table) + (int64_t)(v0 + k) * a.t_stride;
       constexpr int M = Pack<TO>::N;
@@ -260,91 +262,127 @@ __global__ __launch_bounds__(256) void k_segment_sums(SegIn a) {
     }
     return;
   }
-  const int64_t unit = (int64_t)(blockIdx.x - a.zero_blocks) * 4 + wave;
-  const int chunk = (int)(unit / a.n_tiles), tile = (int)(unit % a.n_tiles);
-  if (chunk >= a.n_chunks) return;
-  const int64_t c0 = (int64_t)chunk * a.R;
-  const int rows = (int)(a.n - c0 < a.R ? a.n - c0 : a.R);
+  const int chunk = (int)((blockIdx.x - a.zero_blocks) / a.n_tiles), tile = (int)((blockIdx.x - a.zero_blocks) % a.n_tiles);
+  __shared__ float sum[SUM_WAVES][2][64 * N];
+  __shared__ uint32_t key0[SUM_WAVES], key1[SUM_WAVES];   // a wave's first and last token
+  const int64_t b0 = (int64_t)chunk * a.R * SUM_WAVES, c0 = b0 + (int64_t)wave * a.R;
+  const int64_t left_of = a.n - c0;
+  const int rows = left_of <= 0 ? 0 : (int)(left_of < a.R ? left_of : a.R);
   const int col = tile * 64 * N + lane * N;
   const int live = a.D - col < 0 ? 0 : a.D - col < N ? a.D - col : N;   // columns of this lane
-  const uint32_t limit = (uint32_t)a.rows;
-  uint32_t cur = a.key[c0];
-  if (cur >= limit) return;
-  const bool head_open = c0 > 0 && a.key[c0 - 1] == cur;
-  const bool tail_open = c0 + rows < a.n && a.key[c0 + rows] == a.key[c0 + rows - 1];
+  const uint32_t limit = (uint32_t)a.rows, none = 0xffffffffu;
   float acc[N] = {};
-  bool first = true;
-  const auto flush = [&](bool open) {
-    if (open) {
-      put_columns<float, N>(a.part + ((int64_t)chunk * 2 + (first ? 0 : 1)) * a.D + col, acc, 1.0f, live, false);
+  uint32_t cur = none, head = none;
+  const T* base = reinterpret_cast<const T*>(a.d_out) + col;
+  const auto flush = [&]() {   // token `cur` ends inside the chunk
+    if (cur == head) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) sum[wave][0][lane * N + j] = acc[j];
     } else {
       put_columns<TO, N>(reinterpret_cast<TO*>(a.d_table) + (int64_t)cur * a.t_stride + col, acc, a.scale, live, a.accumulate);
     }
   };
-  const T* base = reinterpret_cast<const T*>(a.d_out) + col;
   bool done = false;
   for (int b = 0; b < rows && !done; b += 64) {
     const int left = rows - b < 64 ? rows - b : 64;
-    uint32_t kv = 0xffffffffu;
+    uint32_t kv = none;
     int32_t pv = 0;
     if (lane < left) { kv = a.key[c0 + b + lane]; pv = a.pos[c0 + b + lane]; }
+    if (b == 0) {
+      cur = head = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv);
+      if (cur >= limit) { cur = head = none; break; }
+    }
     for (int g = 0; g < left && !done; g += U) {
-      float v[U][N];
+      u32x4 v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (g + u >= left) continue;
         const int64_t p = __builtin_amdgcn_readlane(pv, g + u);
-        if (live == N) load_pack(base + p * a.d_stride, v[u]);
-        else
-#pragma unroll
-          for (int j = 0; j < N; ++j) v[u][j] = j < live ? (float)base[p * a.d_stride + j] : 0.f;
+        if (live == N) v[u] = load_raw(base + p * a.d_stride);
+        else v[u] = load_raw_part(base + p * a.d_stride, live);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (g + u >= left || done) continue;
         const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)kv, g + u);
+        if (key >= limit) { done = true; continue; }   // tokens without a row are sorted last
         if (key != cur) {
-          flush(first && head_open);
-          first = false;
+          flush();
           cur = key;
 #pragma unroll
           for (int j = 0; j < N; ++j) acc[j] = 0.f;
-          if (key >= limit) { done = true; continue; }   // tokens without a row are sorted last
         }
 #pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] += v[u][j];
+        for (int j = 0; j < N; ++j) acc[j] += raw_get<T>(v[u], j);
       }
     }
   }
-  if (!done) flush((first && head_open) || tail_open);
+  // the last token: slot 1, or slot 0 when the chunk holds one token only
+#pragma unroll
+  for (int j = 0; j < N; ++j) sum[wave][cur == head ? 0 : 1][lane * N + j] = acc[j];
+  if (lane == 0) { key0[wave] = head; key1[wave] = cur; }
+  __syncthreads();
+  // join: a thread a column, the chunks in order
+  const int64_t b1 = a.n < b0 + (int64_t)a.R * SUM_WAVES ? a.n : b0 + (int64_t)a.R * SUM_WAVES;
+  const uint32_t in = b0 > 0 ? a.key[b0 - 1] : none, out = b1 < a.n ? a.key[b1] : none;   // the neighbours' tokens
+  float* part = a.part + (int64_t)chunk * 2 * a.D;
+  for (int k = threadIdx.x; k < 64 * N; k += NT) {
+    const int c = tile * 64 * N + k;
+    if (c >= a.D) continue;
+    uint32_t open = none;   // the token that is being added up
+    float v = 0.f;
+    const auto close = [&](bool goes_on) {
+      if (open == none) return;
+      const bool first = open == key0[0];
+      if ((first && open == in) || goes_on) part[(first ? 0 : 1) * a.D + c] = v;
+      else put(reinterpret_cast<TO*>(a.d_table) + (int64_t)open * a.t_stride + c, v * a.scale, a.accumulate);
+    };
+#pragma unroll
+    for (int w = 0; w < SUM_WAVES; ++w) {
+      if (key0[w] == none) continue;
+      if (key0[w] == open) v += sum[w][0][k];
+      else { close(false); open = key0[w]; v = sum[w][0][k]; }
+      if (key1[w] != key0[w]) { close(false); open = key1[w]; v = sum[w][1][k]; }
+    }
+    close(open != none && open == out);
+  }
 }
 
 #define JOIN_WAVES 8
-// One block a chunk and tile; it joins the partial rows of the token that starts in this chunk and goes on in the next.
+// One block for each block of the sums; it joins the partial rows of the token that starts there and goes on in the next.
 template <typename TO>
 __global__ __launch_bounds__(JOIN_WAVES * 64) void k_segment_join(SegIn a) {
   const int chunk = blockIdx.x / a.n_tiles, tile = blockIdx.x % a.n_tiles;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c0 = (int64_t)chunk * a.R;
-  const int64_t end = a.n - c0 < a.R ? a.n : c0 + a.R;
+  const int64_t per = (int64_t)a.R * SUM_WAVES, c0 = chunk * per;
+  const int64_t end = a.n - c0 < per ? a.n : c0 + per;
   const uint32_t key = a.key[end - 1];
   if (key >= (uint32_t)a.rows) return;
   const int s = a.row_ptr[key], e = a.row_ptr[key + 1];
   if (s < c0 || e <= end) return;
-  const int last = (e - 1) / a.R, count = last - chunk + 1;
+  const int last = (int)((e - 1) / per), count = last - chunk + 1;
   const int slot = s == c0 ? 0 : 1;
   __shared__ float sh[JOIN_WAVES][4][64];
   // 256 columns a block: 64 lanes x 4
   const int col = tile * 256 + lane * 4;
   const int live = a.D - col < 0 ? 0 : a.D - col < 4 ? a.D - col : 4;
   float acc[4] = {};
-  if (live > 0)
+  const auto add = [&](auto whole) {
 #pragma unroll 8
     for (int k = wave; k < count; k += JOIN_WAVES) {
       const float* p = a.part + ((int64_t)(chunk + k) * 2 + (k == 0 ? slot : 0)) * a.D + col;
+      float v[4] = {};
+      if (decltype(whole)::value) load_pack(p, v);
+      else
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] += j < live ? p[j] : 0.f;
+        for (int j = 0; j < 4; ++j)
+          if (j < live) v[j] = p[j];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] += v[j];
     }
+  };
+  if (live == 4) add(std::true_type());
+  else if (live > 0) add(std::false_type());
 #pragma unroll
   for (int j = 0; j < 4; ++j) sh[wave][j][lane] = acc[j];
   __syncthreads();
@@ -360,8 +398,10 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void k_segment_join(SegIn a) {
 }
 
 // ------------------------------------------------------------------ host side
-// Sort: one pass of 8 bits for up to 255 rows (the token outside is one more key), else passes of 11 bits.
-static int sort_bits(int32_t n_rows) { return n_rows < 256 ? 8 : 11; }
+// Sort: passes of 8 bits while they take no more passes than 11 bits would (a pass of 2048 bins costs twice one of 256: each
+// block reads the whole count table): one pass for up to 255 rows (the token outside is one more key), two below 65536 rows;
+// from there two passes of 11 bits up to 2^22 rows, three beyond.
+static int sort_bits(int32_t rows) { return rows < 65536 ? 8 : 11; }
 static int sort_passes(int32_t n_rows, int bits) {
   int p = 1;
   while (p * bits < 31 && (n_rows >> (p * bits)) != 0) ++p;
@@ -374,10 +414,10 @@ static int sort_per_block(int64_t n, int bits) {
   const int64_t per = (n + most - 1) / most;
   return (int)((per < 1024 ? 1024 : per + SORT_NT - 1) / SORT_NT * SORT_NT);
 }
-// Positions of a chunk: about 4096 waves over the chip, at least 16 positions (a chunk leaves up to one partial row).
+// Positions of a wave: about 8192 waves over the chip, at least 16 positions.
 static int chunk_rows(int64_t n, int tiles) {
   int r = 16;
-  while (r < 512 && n * tiles > (int64_t)r * 4096) r *= 2;
+  while (r < 512 && n * tiles > (int64_t)r * 8192) r *= 2;
   return r;
 }
 struct EmbedWs { uint32_t* key[2]; int32_t* pos[2]; int32_t* hist; int32_t* row_ptr; float* part; size_t bytes; };
@@ -392,7 +432,7 @@ static EmbedWs embed_ws(void* base, int64_t n, int32_t rows, int32_t width) {
   w.hist = (int32_t*)take((size_t)blocks * (1 << bits) * 4);
   w.row_ptr = (int32_t*)take(((size_t)rows + 1) * 4);
   // (half-precision tiles are the widest: fewest tiles, shortest chunks, most partial rows)
-  const int64_t r = chunk_rows(n, (width + 511) / 512);
+  const int64_t r = (int64_t)chunk_rows(n, (width + 511) / 512) * SUM_WAVES;
   w.part = (float*)take((size_t)((n + r - 1) / r) * 2 * (size_t)width * 4);
   w.bytes = used;
   return w;
@@ -423,10 +463,11 @@ template <int BITS> static int sort_tokens(const EmbedGrad& g, const EmbedWs& w,
 template <typename T, typename TO> static void segment_sums(SegIn a, hipStream_t s) {
   a.n_tiles = (a.D + 64 * Pack<T>::N - 1) / (64 * Pack<T>::N);
   a.R = chunk_rows(a.n, a.n_tiles);
-  a.n_chunks = (int)((a.n + a.R - 1) / a.R);
+  const int64_t per = (int64_t)a.R * SUM_WAVES;
+  a.n_chunks = (int)((a.n + per - 1) / per);
   a.zero_blocks = (a.rows + ZERO_ROWS - 1) / ZERO_ROWS;
-  const int64_t waves = (int64_t)a.n_chunks * a.n_tiles;
-  hipLaunchKernelGGL((k_segment_sums<T, TO>), dim3((unsigned)(a.zero_blocks + (waves + 3) / 4)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((k_segment_sums<T, TO>), dim3((unsigned)(a.zero_blocks + (int64_t)a.n_chunks * a.n_tiles)), dim3(SUM_WAVES * 64),
+                     0, s, a);
   if (a.n_chunks > 1) {
     SegIn j = a;
     j.n_tiles = (a.D + 255) / 256;

@@ -31,6 +31,15 @@ template <typename T> __device__ __forceinline__ u32x4 raw_minus_inf() {
   const uint32_t v = sizeof(T) == 4 ? 0xff800000u : __builtin_bit_cast(uint16_t, (typename std::conditional<sizeof(T) == 4, bf16_t, T>::type)-__builtin_inff()) * 0x10001u;
   return u32x4{v, v, v, v};
 }
+// The first `live` elements of a pack, zeros behind them.
+template <typename T> __device__ __forceinline__ u32x4 load_raw_part(const T* p, int live) {
+  typedef typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type Bits;
+  u32x4 r = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < Pack<T>::N; ++j)
+    if (j < live) r[j / Pack<T>::PER] |= (uint32_t)reinterpret_cast<const Bits*>(p)[j] << (j % Pack<T>::PER * 16);
+  return r;
+}
 template <typename T> __device__ __forceinline__ void load_pack(const T* p, float (&v)[Pack<T>::N]) {
   const u32x4 r = load_raw(p);
 #pragma unroll
