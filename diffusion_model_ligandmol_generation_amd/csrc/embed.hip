@@ -117,6 +117,17 @@ __global__ __launch_bounds__(SORT_NT) void k_sort_scatter(SortPass a) {
   __shared__ int cnt[SORT_WAVES][NB];
   __shared__ int wtot[SORT_WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // this wave's first keys are on their way while the count table is read
+  constexpr int PRE = 2;
+  const int64_t w0 = (int64_t)blockIdx.x * a.per_block + (int64_t)wave * (a.per_block / SORT_WAVES);
+  uint32_t pre_key[PRE];
+  int32_t pre_pos[PRE];
+#pragma unroll
+  for (int k = 0; k < PRE; ++k) {
+    const int64_t i = w0 + k * 64 + lane;   // (a wave's part is at least PRE * 64 positions)
+    pre_key[k] = 0; pre_pos[k] = 0;
+    if (i < a.n) { pre_key[k] = sort_key<FIRST>(a, i); pre_pos[k] = FIRST ? (int32_t)i : a.pos_in[i]; }
+  }
   for (int i = tid; i < SORT_WAVES * NB; i += SORT_NT) (&cnt[0][0])[i] = 0;
   int total[K] = {}, before[K] = {};
   if (tid < LIVE) {
@@ -143,8 +154,10 @@ __global__ __launch_bounds__(SORT_NT) void k_sort_scatter(SortPass a) {
   int excl = scan - own;
   for (int w = 0; w < wave; ++w) excl += wtot[w];
   // counts of this block's waves
-  const int64_t w0 = (int64_t)blockIdx.x * a.per_block + (int64_t)wave * (a.per_block / SORT_WAVES);
-  for (int k = lane; k < a.per_block / SORT_WAVES; k += 64)
+#pragma unroll
+  for (int k = 0; k < PRE; ++k)
+    if (w0 + k * 64 + lane < a.n) atomicAdd(&cnt[wave][(pre_key[k] >> a.shift) & (NB - 1)], 1);
+  for (int k = PRE * 64 + lane; k < a.per_block / SORT_WAVES; k += 64)
     if (w0 + k < a.n) atomicAdd(&cnt[wave][(sort_key<FIRST>(a, w0 + k) >> a.shift) & (NB - 1)], 1);
   __syncthreads();
   if (tid < LIVE) {
@@ -163,15 +176,9 @@ __global__ __launch_bounds__(SORT_NT) void k_sort_scatter(SortPass a) {
     }
   }
   __syncthreads();
-  for (int k = 0; k < a.per_block / SORT_WAVES; k += 64) {
-    const int64_t i = w0 + k + lane;
-    const bool on = i < a.n;
-    uint32_t key = 0;
-    int32_t pos = 0;
-    if (on) { key = sort_key<FIRST>(a, i); pos = FIRST ? (int32_t)i : a.pos_in[i]; }
+  const auto place = [&](bool on, uint32_t key, int32_t pos) {
     const int d = (int)(key >> a.shift) & (NB - 1);
     uint64_t same = __ballot(on);
-    if (same == 0) break;
 #pragma unroll
     for (int b = 0; b < BITS; ++b) {
       const uint64_t set = __ballot((d >> b) & 1);
@@ -187,6 +194,16 @@ __global__ __launch_bounds__(SORT_NT) void k_sort_scatter(SortPass a) {
       a.key_out[at + rank] = key;
       a.pos_out[at + rank] = pos;
     }
+  };
+#pragma unroll
+  for (int k = 0; k < PRE; ++k) place(w0 + k * 64 + lane < a.n, pre_key[k], pre_pos[k]);
+  for (int k = PRE * 64; k < a.per_block / SORT_WAVES && w0 + k < a.n; k += 64) {
+    const int64_t i = w0 + k + lane;
+    const bool on = i < a.n;
+    uint32_t key = 0;
+    int32_t pos = 0;
+    if (on) { key = sort_key<FIRST>(a, i); pos = FIRST ? (int32_t)i : a.pos_in[i]; }
+    place(on, key, pos);
   }
 }
 
@@ -414,9 +431,9 @@ static int sort_per_block(int64_t n, int bits) {
   const int64_t per = (n + most - 1) / most;
   return (int)((per < 1024 ? 1024 : per + SORT_NT - 1) / SORT_NT * SORT_NT);
 }
-// Positions of a wave: about 8192 waves over the chip, at least 16 positions.
+// Positions of a wave: about 8192 waves over the chip, at least 8 positions.
 static int chunk_rows(int64_t n, int tiles) {
-  int r = 16;
+  int r = 8;
   while (r < 512 && n * tiles > (int64_t)r * 8192) r *= 2;
   return r;
 }

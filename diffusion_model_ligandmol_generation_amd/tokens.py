@@ -29,20 +29,23 @@ PolicyLoss = namedtuple("PolicyLoss", "loss surrogate kl clip_fraction logp")
 PolicyGrad = namedtuple("PolicyGrad", "loss surrogate kl clip_fraction logp d_logits")
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 class _on:
     """Makes a tensor's device the current one (free when it already is) and gives its current stream."""
-    __slots__ = ("device", "back")
+    __slots__ = ("index", "back")
 
     def __init__(self, device):
-        self.device = device
+        self.index = device.index
 
     def __enter__(self):
         now = torch.cuda.current_device()
         self.back = None
-        if self.device.index is not None and self.device.index != now:
-            torch.cuda.set_device(self.device)
+        if self.index != now:
+            torch.cuda.set_device(self.index)
             self.back = now
-        return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
         if self.back is not None:
@@ -66,13 +69,12 @@ def _check_ids(tokens, device, name="tokens"):
 def _rows(t, width):
     """[..., width] as rows with unit stride: (tensor to keep alive, number of rows, elements between rows)."""
     n = t.numel() // width
+    if t.is_contiguous():
+        return t, n, width
     if t.dim() != 2:
         t = t.reshape(n, width)
-    if n <= 1 or width == 1:
-        t = t.contiguous()
-        return t, n, width
-    if t.stride(1) != 1 or t.stride(0) < width:   # transposed, or rows that overlap (an expanded tensor)
-        t = t.contiguous()
+    if n <= 1 or width == 1 or t.stride(1) != 1 or t.stride(0) < width:   # transposed, or rows that overlap (expanded)
+        return t.contiguous(), n, width
     return t, n, t.stride(0)
 
 
@@ -86,7 +88,7 @@ def _vector(t, n, device, name):
         if t.dtype not in _DTYPES and t.dtype != torch.float64:
             raise ValueError(f"{name} must be a floating-point tensor, got {t.dtype}")
         t = t.float()
-    return t.detach().contiguous()
+    return t.contiguous()
 
 
 def _ptr_vector(seq_ptr, device, name="seq_ptr"):
@@ -94,7 +96,9 @@ def _ptr_vector(seq_ptr, device, name="seq_ptr"):
         raise ValueError(f"{name} must be a 1-D int32 tensor of first positions, one more than there are sequences")
     if seq_ptr.device != device:
         raise ValueError(f"{name} lives on {seq_ptr.device}, the logits on {device}")
-    return seq_ptr.to(torch.int32).contiguous()
+    if seq_ptr.dtype != torch.int32:
+        seq_ptr = seq_ptr.to(torch.int32)
+    return seq_ptr.contiguous()
 
 
 def _finite_scale(value, name):
@@ -123,9 +127,9 @@ def _embed(tokens, table, scale):
     _check_ids(tokens, dev)
     scale = _finite_scale(scale, "scale")
     V, D = table.shape
-    table, _, stride = _rows(table.detach(), D)
+    table, _, stride = _rows(table, D)
     ids = tokens.contiguous()
-    out = torch.empty(*tokens.shape, D, dtype=table.dtype, device=dev)
+    out = torch.empty((*tokens.shape, D), dtype=table.dtype, device=dev)
     with _on(dev) as stream:
         check(_lib.load().ligdiff_embed(table.data_ptr(), _DTYPES[table.dtype], V, D, stride, ids.data_ptr(),
                                         _TOKEN_BYTES[ids.dtype], ids.numel(), scale, out.data_ptr(), D, stream), "ligdiff_embed")
@@ -162,12 +166,12 @@ def embed_tokens_grad(d_out, tokens, n_rows, scale=1.0, out=None, accumulate=Fal
     D = d_out.shape[-1] if d_out.dim() else 0
     if n_rows < 1 or D < 1 or tuple(d_out.shape[:-1]) != tuple(tokens.shape):
         raise ValueError("d_out must be [*tokens.shape, width] with width and n_rows at least 1")
-    rows, n, stride = _rows(d_out.detach(), D)
+    rows, n, stride = _rows(d_out, D)
     ids = tokens.contiguous()
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs the tensor to add to (out)")
-        out = torch.empty(n_rows, D, dtype=d_out.dtype, device=dev)
+        out = torch.empty((n_rows, D), dtype=d_out.dtype, device=dev)
     elif out.shape != (n_rows, D) or out.device != dev or out.dtype not in (d_out.dtype, torch.float32):
         raise ValueError(f"out must be [{n_rows}, {D}] on {dev}, of d_out's type or fp32")
     elif (D > 1 and out.stride(1) != 1) or (n_rows > 1 and out.stride(0) < D):
@@ -196,7 +200,7 @@ def _token_args(logits, tokens, temperature):
     if not 0.0 < temperature <= 3e38:
         raise ValueError("temperature must be positive")
     V = logits.shape[-1]
-    rows, n, stride = _rows(logits.detach(), V)
+    rows, n, stride = _rows(logits, V)
     ids = tokens.contiguous()
     return TokenArgs(rows.data_ptr(), ids.data_ptr(), stride, n, V, _DTYPES[rows.dtype], _TOKEN_BYTES[ids.dtype],
                      temperature), rows, ids, n, V
