@@ -165,10 +165,6 @@ __device__ __forceinline__ void row_skip(const RowOut& o, int64_t t, int V, int 
   }
 }
 
-// The weight that a row has in the mean.
-__device__ __forceinline__ double row_weight(const PolicyIn& p, int seq, double inv_total) {
-  return p.per_seq_mean ? inv_total / (double)p.seq_len[seq] : inv_total;
-}
 template <int NT> __device__ __forceinline__ double inverse_total(const PolicyIn& p, double* red) {
   double total = p.denom;
   if (!(total > 0.0)) {
@@ -259,6 +255,8 @@ __device__ __forceinline__ void exponentials(u32x4 (&x)[NV], float m, float mc, 
     }
   }
 }
+// Short rows are loaded one row ahead of their arithmetic: a wave has two rows' bytes under way.
+#define ROW_AHEAD(TPR, REGS, MODE) ((TPR) <= 64 && (REGS) <= 8)
 // Waves a SIMD holds at once: what the registers of a row allow.
 #define ROW_WAVES(TPR, REGS, MODE) ((MODE) == TK_LOGP ? ((REGS) <= 16 ? 8 : 6) : (TPR) == 1024 ? ((REGS) <= 16 ? 8 : 4) : (REGS) <= 8 ? 6 : (REGS) <= 16 ? 5 : 4)
 
@@ -269,6 +267,7 @@ template <typename T, int TPR, int NV, int MODE>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)) void k_token_rows(TokenRows a, PolicyIn p, RowOut o) {
   constexpr int N = Pack<T>::N, NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR, NW = TPR / 64, GRP = TPR < 64 ? TPR : 64;
   constexpr bool KEEP = MODE == TK_POLICY && sizeof(T) == 4;   // the exponentials take the logits' registers
+  constexpr bool AHEAD = ROW_AHEAD(TPR, NV * 4, MODE);
   __shared__ float2 sh[2][NW > 1 ? NW : 1];
   __shared__ double red[NT / 64];
   __shared__ double acc[MODE == TK_POLICY ? RPB : 1][3];
@@ -283,34 +282,60 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
   }
   int parity = 0;
   const int64_t step = (int64_t)gridDim.x * RPB;
-  RowScalars next = row_scalars<MODE>(a, p, o, (int64_t)blockIdx.x * RPB + mine);
-  for (int64_t base = (int64_t)blockIdx.x * RPB; base < a.n; base += step) {
-    const int64_t t = base + mine;
-    RowScalars c = next;
-    if constexpr (TPR >= 64) c = RowScalars{uniform(c.id), uniform(c.seq), uniform(c.old), uniform(c.ref)};
-    next = row_scalars<MODE>(a, p, o, t + step);
-    if (TPR <= 64 && t >= a.n) continue;
-    const int id = c.id;
-    if (id < 0 || c.seq < 0) {
-      row_skip<T>(o, t, V, r, TPR, r == 0);
-      continue;
-    }
+  const auto scalars = [&](int64_t t) {
+    RowScalars c = row_scalars<MODE>(a, p, o, t);
+    if (MODE == TK_POLICY && c.seq < 0) c.id = -1;
+    return c;
+  };
+  const auto load = [&](const RowScalars& c, int64_t t, u32x4 (&x)[NV], float& et, float& xt, float& A, int& len) {
     const T* row = reinterpret_cast<const T*>(a.x) + t * a.stride;
-    u32x4 x[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       x[k] = raw_minus_inf<T>();
       if (r + k * TPR < nb) x[k] = load_raw(row + (int64_t)(r + k * TPR) * N);
     }
-    float et = -__builtin_inff();
+    et = -__builtin_inff();
     if (r < tail) et = (float)row[nb * N + r];
-    float xt = (float)row[id];
-    double w = 0.0;
-    float A = 0.f;
+    xt = (float)row[c.id];
     if constexpr (MODE == TK_POLICY) {
       A = p.adv[p.adv_per_token ? t : (int64_t)c.seq];
-      w = row_weight(p, c.seq, inv_total);
+      len = p.per_seq_mean ? p.seq_len[c.seq] : 1;
     }
+  };
+  RowScalars next = scalars((int64_t)blockIdx.x * RPB + mine), after{};
+  u32x4 x1[AHEAD ? NV : 1];
+  float et1 = 0.f, xt1 = 0.f, A1 = 0.f;
+  int len1 = 1;
+  if constexpr (AHEAD) {
+    if (next.id >= 0) load(next, (int64_t)blockIdx.x * RPB + mine, x1, et1, xt1, A1, len1);
+    after = scalars((int64_t)blockIdx.x * RPB + mine + step);
+  }
+  for (int64_t base = (int64_t)blockIdx.x * RPB; base < a.n; base += step) {
+    const int64_t t = base + mine;
+    RowScalars c = next;
+    u32x4 x[NV];
+    float et, xt, A = 0.f;
+    int len = 1;
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) x[k] = x1[k];
+      et = et1; xt = xt1; A = A1; len = len1;
+      next = after;
+      if (next.id >= 0) load(next, t + step, x1, et1, xt1, A1, len1);
+      after = scalars(t + 2 * step);
+    } else {
+      if constexpr (TPR >= 64) c = RowScalars{uniform(c.id), uniform(c.seq), uniform(c.old), uniform(c.ref)};
+      next = scalars(t + step);
+    }
+    if (TPR <= 64 && t >= a.n) continue;
+    const int id = c.id;
+    if (id < 0) {
+      row_skip<T>(o, t, V, r, TPR, r == 0);
+      continue;
+    }
+    if constexpr (!AHEAD) load(c, t, x, et, xt, A, len);
+    double w = 0.0;
+    if constexpr (MODE == TK_POLICY) w = p.per_seq_mean ? inv_total / (double)len : inv_total;
     float m = et;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -445,7 +470,7 @@ __global__ __launch_bounds__(1024) void k_token_rows_long(TokenRows a, PolicyIn 
     float A = 0.f;
     if constexpr (MODE == TK_POLICY) {
       A = p.adv[p.adv_per_token ? t : (int64_t)c.seq];
-      w = row_weight(p, c.seq, inv_total);
+      w = p.per_seq_mean ? inv_total / (double)p.seq_len[c.seq] : inv_total;
     }
     float m = -__builtin_inff(), s = 0.f;   // of this lane: s relative to m
     for (int i = r; i < nb + (r < tail ? NT : 0); i += NT) {
