@@ -63,7 +63,8 @@ __device__ __forceinline__ void kl_terms(float q, float& em1, float& kl) {
   }
 }
 
-enum { TK_LOGP = 0, TK_POLICY = 1 };
+enum { TK_LOGP = 0, TK_POLICY = 1, TK_SMALL = 2 };   // TK_SMALL: the policy loss of at most SMALL_ROWS rows, by one block
+#define SMALL_ROWS 64
 
 struct PolicyIn {
   const int32_t* seq_of;     // [n] sequence of a row, -1 for rows that take no part
@@ -78,6 +79,8 @@ struct PolicyIn {
   const float* ref_logp;     // may be null: no KL term
   float clip_lo, clip_hi, kl_coef, grad_scale;
   double* partial;           // [gridDim.x][3]: surrogate, kl, share of clipped rows
+  const int32_t* seq_ptr;    // small batches: their one block finds the sequences itself
+  float* result;             // and writes the result
 };
 struct RowOut {
   float* logp;               // [n] or null
@@ -104,8 +107,8 @@ template <int MODE> __device__ __forceinline__ RowScalars row_scalars(const Toke
   RowScalars r{-1, 0, 0.f, 0.f};
   if (t >= a.n) return r;
   r.id = a.tok.at(t);
-  if constexpr (MODE == TK_POLICY) {
-    r.seq = p.seq_of[t];
+  if constexpr (MODE != TK_LOGP) {
+    if (MODE == TK_POLICY) r.seq = p.seq_of[t];
     if (p.old_logp) r.old = p.old_logp[t];
     if (p.ref_logp) r.ref = p.ref_logp[t];
   } else if (o.minus) r.ref = o.minus[t];
@@ -119,7 +122,7 @@ __device__ __forceinline__ float row_epilogue(const TokenRows& a, const PolicyIn
   const double z = far_out(M) ? ((double)xt - (double)M) * a.c : fma((double)xt, (double)a.c, -(double)(M * a.c));
   const double lp = S == 0.f ? -__builtin_inf() : fma(z, 0.69314718055994530942, -log_of_sum(S));
   float g = 0.f, coef = 0.f;
-  if constexpr (MODE == TK_POLICY) {
+  if constexpr (MODE != TK_LOGP) {
     const float rho = p.old_logp ? expf((float)(lp - (double)c.old)) : lp == lp ? 1.0f : (float)lp;
     const float hi = 1.0f + p.clip_hi, lo = 1.0f - p.clip_lo;
     const bool clipped = (A > 0.f && rho > hi) || (A < 0.f && rho < lo);
@@ -185,6 +188,47 @@ template <int RPB> __device__ __forceinline__ void policy_partial(const PolicyIn
     double v = acc[0][threadIdx.x];
     for (int g = 1; g < RPB; ++g) v += acc[g][threadIdx.x];
     p.partial[(int64_t)blockIdx.x * 3 + threadIdx.x] = v;
+  }
+}
+// The only block of a small batch: the sequence of each row and the number of its sequence's rows, and 1 / the total.
+__device__ __forceinline__ double small_rows(const TokenRows& a, const PolicyIn& p, int* seq, int* len) {
+  const int t = threadIdx.x;
+  __shared__ int count;
+  if (t < 64) {
+    int s = -1;
+    if (t < (int)a.n && a.tok.at(t) >= 0) {
+      s = 0;
+      if (p.seq_ptr) {
+        uint32_t lo = 0, hi = (uint32_t)p.n_seq + 1u;   // the number of offsets <= t
+        while (lo < hi) {
+          const uint32_t mid = lo + ((hi - lo) >> 1);
+          if (p.seq_ptr[mid] <= t) lo = mid + 1; else hi = mid;
+        }
+        s = lo > (uint32_t)p.n_seq ? -1 : (int)lo - 1;
+      }
+    }
+    seq[t] = s;
+    int same = 0;
+    for (int k = 0; k < 64; ++k) same += __shfl(s, k) == s;
+    len[t] = same;
+    const int all = __popcll(__ballot(s >= 0));
+    if (t == 0) count = all;
+  }
+  __syncthreads();
+  const double total = p.denom > 0.0 ? p.denom : p.per_seq_mean ? (double)p.n_seq : (double)count;
+  return total > 0.0 ? 1.0 / total : 0.0;
+}
+template <int RPB> __device__ __forceinline__ void policy_result(const PolicyIn& p, const double (&acc)[RPB][3]) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double v[3] = {0.0, 0.0, 0.0};
+    for (int g = 0; g < RPB; ++g)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) v[k] += acc[g][k];
+    p.result[0] = (float)(v[0] + (double)p.kl_coef * v[1]);
+    p.result[1] = (float)v[0];
+    p.result[2] = (float)v[1];
+    p.result[3] = (float)v[2];
   }
 }
 __global__ __launch_bounds__(256) void k_policy_final(const double* __restrict__ partial, int blocks, double kl_coef, float* __restrict__ result) {
@@ -266,25 +310,28 @@ __device__ __forceinline__ void exponentials(u32x4 (&x)[NV], float m, float mc, 
 template <typename T, int TPR, int NV, int MODE>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)) void k_token_rows(TokenRows a, PolicyIn p, RowOut o) {
   constexpr int N = Pack<T>::N, NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR, NW = TPR / 64, GRP = TPR < 64 ? TPR : 64;
-  constexpr bool KEEP = MODE == TK_POLICY && sizeof(T) == 4;   // the exponentials take the logits' registers
+  constexpr bool KEEP = MODE != TK_LOGP && sizeof(T) == 4;   // the exponentials take the logits' registers
   constexpr bool AHEAD = ROW_AHEAD(TPR, NV * 4, MODE);
   __shared__ float2 sh[2][NW > 1 ? NW : 1];
   __shared__ double red[NT / 64];
-  __shared__ double acc[MODE == TK_POLICY ? RPB : 1][3];
+  __shared__ double acc[MODE != TK_LOGP ? RPB : 1][3];
+  __shared__ int small_seq[MODE == TK_SMALL ? SMALL_ROWS : 1], small_len[MODE == TK_SMALL ? SMALL_ROWS : 1];
   const int r = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x;
   const int mine = TPR < 64 ? threadIdx.x / TPR : TPR == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0;
   const int V = a.V, nb = V / N, tail = V - nb * N;
   double inv_total = 0.0;
-  if constexpr (MODE == TK_POLICY) {
+  if constexpr (MODE != TK_LOGP) {
     if (threadIdx.x < RPB * 3) acc[threadIdx.x / 3][threadIdx.x % 3] = 0.0;
-    inv_total = uniform(inverse_total<NT>(p, red));
+    if constexpr (MODE == TK_SMALL) inv_total = small_rows(a, p, small_seq, small_len);
+    else inv_total = uniform(inverse_total<NT>(p, red));
     __syncthreads();
   }
   int parity = 0;
   const int64_t step = (int64_t)gridDim.x * RPB;
   const auto scalars = [&](int64_t t) {
     RowScalars c = row_scalars<MODE>(a, p, o, t);
-    if (MODE == TK_POLICY && c.seq < 0) c.id = -1;
+    if (MODE == TK_SMALL && t < a.n) c.seq = small_seq[t];
+    if (MODE != TK_LOGP && c.seq < 0) c.id = -1;
     return c;
   };
   const auto load = [&](const RowScalars& c, int64_t t, u32x4 (&x)[NV], float& et, float& xt, float& A, int& len) {
@@ -297,9 +344,9 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
     et = -__builtin_inff();
     if (r < tail) et = (float)row[nb * N + r];
     xt = (float)row[c.id];
-    if constexpr (MODE == TK_POLICY) {
+    if constexpr (MODE != TK_LOGP) {
       A = p.adv[p.adv_per_token ? t : (int64_t)c.seq];
-      len = p.per_seq_mean ? p.seq_len[c.seq] : 1;
+      len = !p.per_seq_mean ? 1 : MODE == TK_SMALL ? small_len[t] : p.seq_len[c.seq];
     }
   };
   RowScalars next = scalars((int64_t)blockIdx.x * RPB + mine), after{};
@@ -335,7 +382,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
     }
     if constexpr (!AHEAD) load(c, t, x, et, xt, A, len);
     double w = 0.0;
-    if constexpr (MODE == TK_POLICY) w = p.per_seq_mean ? inv_total / (double)len : inv_total;
+    if constexpr (MODE != TK_LOGP) w = p.per_seq_mean ? inv_total / (double)len : inv_total;
     float m = et;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -367,11 +414,11 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
     if constexpr (TPR >= 64) {
       inv_s = uniform(inv_s);
       xt = uniform(xt); M = uniform(M); S = uniform(S);
-      if constexpr (MODE == TK_POLICY) { A = uniform(A); w = uniform(w); }
+      if constexpr (MODE != TK_LOGP) { A = uniform(A); w = uniform(w); }
     }
-    float g = row_epilogue<MODE>(a, p, o, t, c, xt, M, S, inv_s, r == 0, A, w, acc[MODE == TK_POLICY ? mine : 0]);
+    float g = row_epilogue<MODE>(a, p, o, t, c, xt, M, S, inv_s, r == 0, A, w, acc[MODE != TK_LOGP ? mine : 0]);
     if constexpr (TPR >= 64) g = uniform(g);
-    if constexpr (MODE == TK_POLICY) {
+    if constexpr (MODE != TK_LOGP) {
       if (o.d == nullptr) continue;
       T* d = reinterpret_cast<T*>(o.d) + t * o.d_stride;
       if (g == 0.f) {   // sends no gradient, also where the row holds a NaN
@@ -405,6 +452,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
     }
   }
   if constexpr (MODE == TK_POLICY) policy_partial<RPB>(p, acc);
+  if constexpr (MODE == TK_SMALL) policy_result<RPB>(p, acc);
 }
 
 // One row's gradient from its logits, maximum and 1 / sum, by TPR lanes: g ([v = id] - p[v]).  A factor of 0 sends no
@@ -511,13 +559,20 @@ __global__ __launch_bounds__(1024) void k_token_rows_long(TokenRows a, PolicyIn 
 
 // d_logits[t, v] = coef mult upstream / temperature ([v = id_t] - p[t, v]) from the saved maximum and 1 / sum: no reduction,
 // the rows are streamed.  coef is that of the row, or of its sequence when an index is given.
+// The loss of a preference step, added up by the last block of its gradient launch.
+struct LossTail { const double* partial; int blocks; double denom; float* loss; };
+__device__ __forceinline__ void preference_final(const LossTail& f);
 template <typename T, int TPR>
-__global__ __launch_bounds__(256) void k_token_grad(TokenRows a, const float* __restrict__ stats, const float* __restrict__ coef,
+__global__ __launch_bounds__(256) void k_token_grad(TokenRows a, LossTail f, const float* __restrict__ stats, const float* __restrict__ coef,
                                                     const int32_t* __restrict__ index, int64_t n_coef, float mult, const float* __restrict__ upstream, T* __restrict__ d, int64_t d_stride) {
   constexpr int RPB = 256 / TPR;
   const int r = threadIdx.x % TPR;
   const double k = (double)mult * a.inv_t * (upstream ? (double)*upstream : 1.0);
-  for (int64_t t = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; t < a.n; t += (int64_t)gridDim.x * RPB) {
+  const int blocks = gridDim.x - (f.loss != nullptr);
+  if ((int)blockIdx.x == blocks) { preference_final(f); return; }
+  // (the last rows first: they are the last that the forward launch read)
+  for (int64_t i = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; i < a.n; i += (int64_t)blocks * RPB) {
+    const int64_t t = a.n - 1 - i;
     const int id = a.tok.at(t);
     const int64_t ci = index ? (int64_t)index[t] : t;
     const float g = id < 0 || ci < 0 || ci >= n_coef ? 0.f : (float)((double)coef[ci] * k);
@@ -546,18 +601,29 @@ __device__ __forceinline__ uint32_t wave_count_upto(const int32_t* __restrict__ 
   }
   return lo;
 }
-template <bool SUM>
-__global__ __launch_bounds__(256) void k_row_segments(TokenView tok, int64_t n, const int32_t* __restrict__ seq_ptr, int32_t S,
-                                                      const float* __restrict__ diff, int32_t* __restrict__ seq_of,
-                                                      double* __restrict__ part_sum, int32_t* __restrict__ part_len,
-                                                      int32_t* __restrict__ chunk_len) {
-  __shared__ double pre[SUM ? SEG_ROWS + 1 : 1];
-  __shared__ int cnt[SEG_ROWS + 1];
-  __shared__ double wsum[4];
-  __shared__ int wcnt[4], wmax[4], ends[2];
+struct SegRows {
+  TokenView tok; int64_t n;
+  const int32_t* seq_ptr; int32_t S;
+  const float* diff;          // [n]
+  int32_t* seq_of;            // [n]
+  double* part_sum;           // [chunks + S]
+  int32_t* part_len;          // [chunks + S] or null
+  int32_t* chunk_len;         // [chunks] or null
+};
+template <bool SUM> struct SegShared {
+  double pre[SUM ? SEG_ROWS + 1 : 1], wsum[4];
+  int cnt[SEG_ROWS + 1], wcnt[4], wmax[4], ends[2];
+};
+template <bool SUM> __device__ __forceinline__ void row_segments(const SegRows& g, int64_t c, SegShared<SUM>& sh) {
+  const TokenView& tok = g.tok;
+  const int64_t n = g.n;
+  const int32_t* __restrict__ seq_ptr = g.seq_ptr;
+  const int32_t S = g.S;
+  double* const pre = sh.pre;
+  int* const cnt = sh.cnt;
   int* const mark = cnt;   // (the counts replace the marks once every thread has read its own)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t c = blockIdx.x, c0 = c * SEG_ROWS;
+  const int64_t c0 = c * SEG_ROWS;
   const int rows = (int)(n - c0 < SEG_ROWS ? n - c0 : SEG_ROWS);
   bool on[4];
   float d[4];
@@ -566,18 +632,18 @@ __global__ __launch_bounds__(256) void k_row_segments(TokenView tok, int64_t n, 
     const int i = tid * 4 + j;
     const int64_t at = c0 + (i < rows ? i : rows - 1);
     on[j] = (tok.at(at) >= 0) & (i < rows);
-    d[j] = SUM ? diff[at] : 0.f;
+    d[j] = SUM ? g.diff[at] : 0.f;
   }
   // sequences of the chunk's first and last row (-1: before the first, S: behind the last)
   if (seq_ptr && wave < 2) {
     const int k = (int)wave_count_upto(seq_ptr, (uint32_t)S + 1u, (int32_t)(wave ? c0 + rows - 1 : c0)) - 1;
-    if (lane == 0) ends[wave] = k;
+    if (lane == 0) sh.ends[wave] = k;
   }
-  if (!seq_ptr && tid < 2) ends[tid] = 0;
+  if (!seq_ptr && tid < 2) sh.ends[tid] = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) mark[tid * 4 + j] = -1;
   __syncthreads();
-  const int s0 = ends[0], s1 = ends[1], sa = s0 < 0 ? 0 : s0;
+  const int s0 = sh.ends[0], s1 = sh.ends[1], sa = s0 < 0 ? 0 : s0;
   // a row's sequence is the last that starts at or before it: starts are marked, then a running maximum
   if (seq_ptr)
     for (int64_t s = (int64_t)sa + tid; s <= s1; s += 256) {
@@ -591,11 +657,11 @@ __global__ __launch_bounds__(256) void k_row_segments(TokenView tok, int64_t n, 
   int run = top;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(run, o); if (lane >= o && u > run) run = u; }
-  if (lane == 63) wmax[wave] = run;
+  if (lane == 63) sh.wmax[wave] = run;
   int before = __shfl_up(run, 1);
   if (lane == 0) before = s0;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) before = wmax[w] > before ? wmax[w] : before;
+  for (int w = 0; w < wave; ++w) before = sh.wmax[w] > before ? sh.wmax[w] : before;
   int k[4];
   double v[4];
 #pragma unroll
@@ -605,7 +671,7 @@ __global__ __launch_bounds__(256) void k_row_segments(TokenView tok, int64_t n, 
     k[j] = m[j] >= 0;
     v[j] = SUM && k[j] ? (double)d[j] : 0.0;
     const int i = tid * 4 + j;
-    if (i < rows) seq_of[c0 + i] = m[j];
+    if (i < rows) g.seq_of[c0 + i] = m[j];
   }
   int ci = (k[0] + k[1]) + (k[2] + k[3]);
   double vi = (v[0] + v[1]) + (v[2] + v[3]);
@@ -617,11 +683,11 @@ __global__ __launch_bounds__(256) void k_row_segments(TokenView tok, int64_t n, 
     const double vu = SUM ? __shfl_up(vi, o) : 0.0;
     if (lane >= o) { ci += cu; vi += vu; }
   }
-  if (lane == 63) { wcnt[wave] = ci; wsum[wave] = vi; }
+  if (lane == 63) { sh.wcnt[wave] = ci; sh.wsum[wave] = vi; }
   __syncthreads();
   int cb = ci - own_c;
   double vb = vi - own_v;
-  for (int w = 0; w < wave; ++w) { cb += wcnt[w]; vb += wsum[w]; }
+  for (int w = 0; w < wave; ++w) { cb += sh.wcnt[w]; vb += sh.wsum[w]; }
   if (tid == 0) { cnt[0] = 0; if (SUM) pre[0] = 0.0; }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -630,17 +696,21 @@ __global__ __launch_bounds__(256) void k_row_segments(TokenView tok, int64_t n, 
     if (SUM) pre[tid * 4 + j + 1] = vb;
   }
   __syncthreads();
-  if (tid == 0 && chunk_len) chunk_len[c] = cnt[rows];
-  if (!part_len) return;
+  if (tid == 0 && g.chunk_len) g.chunk_len[c] = cnt[rows];
+  if (!g.part_len) return;
   for (int64_t s = (int64_t)sa + tid; s <= s1 && s < S; s += 256) {
     const int64_t t0 = seq_ptr ? seq_ptr[s] : 0, t1 = seq_ptr ? seq_ptr[s + 1] : n;
     const int a = t0 <= c0 ? 0 : t0 - c0 < rows ? (int)(t0 - c0) : rows;
     const int b = t1 <= c0 ? 0 : t1 - c0 < rows ? (int)(t1 - c0) : rows;
     if (b > a) {
-      part_len[c + s] = cnt[b] - cnt[a];
-      if (SUM) part_sum[c + s] = pre[b] - pre[a];
+      g.part_len[c + s] = cnt[b] - cnt[a];
+      if (SUM) g.part_sum[c + s] = pre[b] - pre[a];
     }
   }
+}
+template <bool SUM> __global__ __launch_bounds__(256) void k_row_segments(SegRows g) {
+  __shared__ SegShared<SUM> sh;
+  row_segments<SUM>(g, blockIdx.x, sh);
 }
 // The parts of sequence s, added up by the 64 lanes of a wave.
 template <bool SUM>
@@ -677,58 +747,78 @@ struct PrefIn {
   float beta, smooth;
   int32_t kind, average;
   double denom, grad_scale;
+  float* loss;
   float* log_ratio; float* margin; float* slope;
   double* partial;          // [gridDim.x]
 };
-// Pairs: sequence p is preferred over sequence P + p.  A wave joins both sequences' differences (a margin is what two long
-// sums leave: 64 bits), forms the loss and d loss / d logp of either sequence's rows.
+// The loss of pair pr from both sequences' sums and numbers of rows, and d loss / d logp of either sequence's rows.
+__device__ __forceinline__ double pair_loss(const PrefIn& a, int64_t pr, double sum0, int len0, double sum1, int len1) {
+  const double share0 = a.average && len0 > 0 ? 1.0 / (double)len0 : 1.0, share1 = a.average && len1 > 0 ? 1.0 / (double)len1 : 1.0;
+  const double ratio0 = sum0 * share0, ratio1 = sum1 * share1, gap = ratio0 - ratio1;
+  double loss, slope;
+  if (a.kind == LIGDIFF_PREFERENCE_SIGMOID) {
+    // -(1 - e) log sigmoid(z) - e log sigmoid(-z) = log(1 + exp(-z)) + e z
+    const double z = (double)a.beta * gap, x = exp(-fabs(z));
+    loss = log1p(x) + (z < 0.0 ? -z : 0.0) + (double)a.smooth * z;
+    const double sig = z >= 0.0 ? 1.0 / (1.0 + x) : x / (1.0 + x);
+    slope = (double)a.beta * (sig - 1.0 + (double)a.smooth);
+  } else {
+    const double z = gap - 0.5 / (double)a.beta;
+    loss = z * z;
+    slope = 2.0 * z;
+  }
+  slope *= a.grad_scale / a.denom;
+  a.log_ratio[pr] = (float)ratio0;
+  a.log_ratio[pr + a.P] = (float)ratio1;
+  a.margin[pr] = (float)gap;
+  a.slope[pr] = (float)(slope * share0);
+  a.slope[pr + a.P] = (float)(-slope * share1);
+  return loss;
+}
+// Pairs: sequence p is preferred over sequence P + p.  A wave joins the parts of both (a margin is what two long sums leave:
+// 64 bits); 64 pairs a wave at a time when the batch is one chunk and every sequence has one part.
 __global__ __launch_bounds__(256) void k_preference(PrefIn a) {
   __shared__ double red[4];
-  const int lane = threadIdx.x & 63;
   double total = 0.0;
   for (int64_t pr = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); pr < a.P; pr += (int64_t)gridDim.x * 4) {
-    double ratio[2], share[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      double sum;
-      int len;
-      join_parts<true>(a.seq_ptr, a.n, pr + (int64_t)h * a.P, a.part_sum, a.part_len, sum, len);
-      share[h] = a.average && len > 0 ? 1.0 / (double)len : 1.0;
-      ratio[h] = sum * share[h];
-    }
-    if (lane != 0) continue;
-    const double gap = ratio[0] - ratio[1];
-    double loss, slope;
-    if (a.kind == LIGDIFF_PREFERENCE_SIGMOID) {
-      // -(1 - e) log sigmoid(z) - e log sigmoid(-z) = log(1 + exp(-z)) + e z
-      const double z = (double)a.beta * gap, x = exp(-fabs(z));
-      loss = log1p(x) + (z < 0.0 ? -z : 0.0) + (double)a.smooth * z;
-      const double sig = z >= 0.0 ? 1.0 / (1.0 + x) : x / (1.0 + x);
-      slope = (double)a.beta * (sig - 1.0 + (double)a.smooth);
-    } else {
-      const double z = gap - 0.5 / (double)a.beta;
-      loss = z * z;
-      slope = 2.0 * z;
-    }
-    total += loss;
-    slope *= a.grad_scale / a.denom;
-    a.log_ratio[pr] = (float)ratio[0];
-    a.log_ratio[pr + a.P] = (float)ratio[1];
-    a.margin[pr] = (float)gap;
-    a.slope[pr] = (float)(slope * share[0]);
-    a.slope[pr + a.P] = (float)(-slope * share[1]);
+    double s0, s1;
+    int l0, l1;
+    join_parts<true>(a.seq_ptr, a.n, pr, a.part_sum, a.part_len, s0, l0);
+    join_parts<true>(a.seq_ptr, a.n, pr + a.P, a.part_sum, a.part_len, s1, l1);
+    if ((threadIdx.x & 63) == 0) total += pair_loss(a, pr, s0, l0, s1, l1);
   }
   total = block_sum<256>(total, red);
   if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
 }
-__global__ __launch_bounds__(256) void k_preference_final(const double* __restrict__ partial, int blocks, double denom, float* __restrict__ loss) {
+// A batch of one chunk: rows -> sequences, pairs and the loss in one launch of one block.
+__global__ __launch_bounds__(256) void k_preference_small(SegRows g, PrefIn a) {
+  __shared__ SegShared<true> sh;
+  __shared__ double red[4];
+  row_segments<true>(g, 0, sh);
+  __syncthreads();
+  double total = 0.0;
+  for (int64_t pr = threadIdx.x; pr < a.P; pr += 256) {
+    double sum[2] = {0.0, 0.0};
+    int len[2] = {0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t q = pr + (int64_t)h * a.P, t0 = a.seq_ptr[q] < 0 ? 0 : a.seq_ptr[q], t1 = a.seq_ptr[q + 1] > a.n ? a.n : a.seq_ptr[q + 1];
+      if (t1 > t0) { sum[h] = g.part_sum[q]; len[h] = g.part_len[q]; }
+    }
+    total += pair_loss(a, pr, sum[0], len[0], sum[1], len[1]);
+  }
+  total = block_sum<256>(total, red);
+  if (threadIdx.x == 0) *a.loss = (float)(total / a.denom);
+}
+__device__ __forceinline__ void preference_final(const LossTail& f) {
   __shared__ double red[4];
   double v = 0.0;
 #pragma unroll 4
-  for (int b = threadIdx.x; b < blocks; b += 256) v += partial[b];
+  for (int b = threadIdx.x; b < f.blocks; b += 256) v += f.partial[b];
   v = block_sum<256>(v, red);
-  if (threadIdx.x == 0) *loss = (float)(v / denom);
+  if (threadIdx.x == 0) *f.loss = (float)(v / f.denom);
 }
+__global__ __launch_bounds__(256) void k_preference_final(LossTail f) { preference_final(f); }
 
 // An empty batch: no row kernel runs.
 __global__ void k_empty_policy(float* result) { if (threadIdx.x < 4) result[threadIdx.x] = 0.f; }
@@ -746,11 +836,19 @@ static int launch_rows_as(const TokenRows& a, const PolicyIn& p, const RowOut& o
   hipLaunchKernelGGL((k_token_rows<T, TPR, NV, MODE>), dim3(grid), dim3(NT), 0, s, a, p, o);
   return grid;
 }
+// A batch of at most SMALL_ROWS short rows is one launch of one block: three launches take longer than its four rounds.
+static bool rows_of_16_lanes(int dtype, int32_t V) { return V / (dtype == LIGDIFF_F32 ? 4 : 8) <= 64; }
 // The least lanes whose registers hold a row: 16 lanes up to 64 packs, a wave up to 512, 256 lanes up to 2048, 1024 up to
 // 8192 (32768 fp32 or 65536 half-precision logits); beyond that the row is read twice.  Returns the number of blocks.
 template <typename T, int MODE>
 static int launch_rows(const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
   const int packs = a.V / Pack<T>::N;
+  if (MODE == TK_POLICY && a.n <= SMALL_ROWS && packs <= 64) {
+    if (packs <= 16) hipLaunchKernelGGL((k_token_rows<T, 16, 1, TK_SMALL>), dim3(1), dim3(256), 0, s, a, p, o);
+    else if (packs <= 32) hipLaunchKernelGGL((k_token_rows<T, 16, 2, TK_SMALL>), dim3(1), dim3(256), 0, s, a, p, o);
+    else hipLaunchKernelGGL((k_token_rows<T, 16, 4, TK_SMALL>), dim3(1), dim3(256), 0, s, a, p, o);
+    return 1;
+  }
   if (packs <= 16) return launch_rows_as<T, 16, 1, MODE>(a, p, o, s);
   if (packs <= 32) return launch_rows_as<T, 16, 2, MODE>(a, p, o, s);
   if (packs <= 64) return launch_rows_as<T, 16, 4, MODE>(a, p, o, s);
@@ -771,24 +869,23 @@ template <int MODE> static int launch_rows_dtype(int dtype, const TokenRows& a, 
   if (dtype == LIGDIFF_BF16) return launch_rows<bf16_t, MODE>(a, p, o, s);
   return launch_rows<f16_t, MODE>(a, p, o, s);
 }
-template <typename T>
-static void launch_grad(const TokenRows& a, const float* stats, const float* coef, const int32_t* index, int64_t n_coef, float mult, const float* up, void* d,
-                        int64_t d_stride, hipStream_t s) {
-  const int packs = a.V / Pack<T>::N;
-  const int cap = 8192;
-  if (packs <= 64)
-    hipLaunchKernelGGL((k_token_grad<T, 16>), dim3(row_grid((a.n + 15) / 16, cap)), dim3(256), 0, s, a, stats, coef, index, n_coef, mult, up, (T*)d, d_stride);
-  else if (packs <= 512)
-    hipLaunchKernelGGL((k_token_grad<T, 64>), dim3(row_grid((a.n + 3) / 4, cap)), dim3(256), 0, s, a, stats, coef, index, n_coef, mult, up, (T*)d, d_stride);
-  else
-    hipLaunchKernelGGL((k_token_grad<T, 256>), dim3(row_grid(a.n, cap)), dim3(256), 0, s, a, stats, coef, index, n_coef, mult, up, (T*)d, d_stride);
+struct GradIn { const float* stats; const float* coef; const int32_t* index; int64_t n_coef; float mult; const float* up; void* d; int64_t d_stride; };
+template <typename T, int TPR> static void launch_grad_as(const TokenRows& a, const GradIn& g, const LossTail& f, hipStream_t s) {
+  constexpr int RPB = 256 / TPR;
+  const int grid = row_grid((a.n + RPB - 1) / RPB, 8192) + (f.loss != nullptr);
+  hipLaunchKernelGGL((k_token_grad<T, TPR>), dim3(grid), dim3(256), 0, s, a, f, g.stats, g.coef, g.index, g.n_coef, g.mult, g.up, (T*)g.d, g.d_stride);
 }
-static void launch_grad_dtype(int dtype, const TokenRows& a, const float* stats, const float* coef, const int32_t* index,
-                              int64_t n_coef, float mult, const float* up, void* d, int64_t d_stride, hipStream_t s) {
-  if (a.n == 0) return;
-  if (dtype == LIGDIFF_F32) launch_grad<float>(a, stats, coef, index, n_coef, mult, up, d, d_stride, s);
-  else if (dtype == LIGDIFF_BF16) launch_grad<bf16_t>(a, stats, coef, index, n_coef, mult, up, d, d_stride, s);
-  else launch_grad<f16_t>(a, stats, coef, index, n_coef, mult, up, d, d_stride, s);
+template <typename T> static void launch_grad(const TokenRows& a, const GradIn& g, const LossTail& f, hipStream_t s) {
+  const int packs = a.V / Pack<T>::N;
+  if (packs <= 64) launch_grad_as<T, 16>(a, g, f, s);
+  else if (packs <= 512) launch_grad_as<T, 64>(a, g, f, s);
+  else launch_grad_as<T, 256>(a, g, f, s);
+}
+// (the caller has seen to it that there are rows)
+static void launch_grad_dtype(int dtype, const TokenRows& a, const GradIn& g, const LossTail& f, hipStream_t s) {
+  if (dtype == LIGDIFF_F32) launch_grad<float>(a, g, f, s);
+  else if (dtype == LIGDIFF_BF16) launch_grad<bf16_t>(a, g, f, s);
+  else launch_grad<f16_t>(a, g, f, s);
 }
 
 static int fill_rows(TokenRows* r, const ligdiff_token_args* a) {
@@ -821,7 +918,9 @@ extern "C" int ligdiff_token_logprob_grad(const ligdiff_token_args* args, const 
   const int rc = fill_rows(&a, args);
   if (rc) return rc;
   if (a.n > 0 && (!stats || !coef || !d_logits || d_stride < a.V || n_coef < (coef_index ? 1 : a.n))) return LIGDIFF_ERR_ARG;
-  launch_grad_dtype(args->dtype, a, stats, coef, coef_index, n_coef, mult, upstream, d_logits, d_stride, (hipStream_t)stream);
+  if (a.n > 0)
+    launch_grad_dtype(args->dtype, a, GradIn{stats, coef, coef_index, n_coef, mult, upstream, d_logits, d_stride}, LossTail{},
+                      (hipStream_t)stream);
   LD_CHECK_LAUNCH();
   return LIGDIFF_OK;
 }
@@ -869,23 +968,28 @@ extern "C" int ligdiff_preference_loss(const ligdiff_token_args* args, const lig
   const PrefWs w = pref_ws(q->workspace, a.n, q->n_pairs);
   if (q->workspace_bytes < w.bytes) return LIGDIFF_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
-  if (a.n > 0) {
-    launch_rows_dtype<TK_LOGP>(args->dtype, a, PolicyIn{}, RowOut{w.diff, q->ref_logp, q->stats, nullptr, nullptr, 0}, s);
-    hipLaunchKernelGGL((k_row_segments<true>), dim3((unsigned)seg_chunks(a.n)), dim3(256), 0, s, a.tok, a.n, q->seq_ptr,
-                       2 * q->n_pairs, w.diff, q->row_seq, w.part_sum, w.part_len, (int32_t*)nullptr);
-  }
   PrefIn p;
   p.n = a.n; p.seq_ptr = q->seq_ptr; p.P = q->n_pairs; p.part_sum = w.part_sum; p.part_len = w.part_len;
   p.beta = q->beta; p.smooth = q->label_smoothing; p.kind = q->kind; p.average = q->average != 0;
   p.denom = q->denominator > 0.f ? (double)q->denominator : (double)q->n_pairs;
   p.grad_scale = (double)q->grad_scale;
-  p.log_ratio = q->log_ratio; p.margin = q->margin; p.slope = q->slope;
+  p.loss = q->loss; p.log_ratio = q->log_ratio; p.margin = q->margin; p.slope = q->slope;
   p.partial = w.partial;
-  const int blocks = row_grid(((int64_t)q->n_pairs + 3) / 4, PREF_BLOCKS);
-  hipLaunchKernelGGL(k_preference, dim3(blocks), dim3(256), 0, s, p);
-  hipLaunchKernelGGL(k_preference_final, dim3(1), dim3(256), 0, s, w.partial, blocks, p.denom, q->loss);
-  if (q->d_logits)
-    launch_grad_dtype(args->dtype, a, q->stats, q->slope, q->row_seq, 2 * (int64_t)q->n_pairs, 1.0f, nullptr, q->d_logits, q->d_stride, s);
+  LossTail f{};
+  const SegRows g{a.tok, a.n, q->seq_ptr, 2 * q->n_pairs, w.diff, q->row_seq, w.part_sum, w.part_len, nullptr};
+  if (a.n > 0) launch_rows_dtype<TK_LOGP>(args->dtype, a, PolicyIn{}, RowOut{w.diff, q->ref_logp, q->stats, nullptr, nullptr, 0}, s);
+  // one block while it has a chunk at most and the pairs do not keep it longer than two launches would take
+  if (a.n > 0 && a.n <= SEG_ROWS && q->n_pairs <= 1024) {
+    hipLaunchKernelGGL(k_preference_small, dim3(1), dim3(256), 0, s, g, p);
+  } else {
+    if (a.n > 0) hipLaunchKernelGGL((k_row_segments<true>), dim3((unsigned)seg_chunks(a.n)), dim3(256), 0, s, g);
+    const int blocks = row_grid(((int64_t)q->n_pairs + 3) / 4, PREF_BLOCKS);
+    hipLaunchKernelGGL(k_preference, dim3(blocks), dim3(256), 0, s, p);
+    f = LossTail{w.partial, blocks, p.denom, q->loss};
+  }
+  if (a.n > 0 && q->d_logits)
+    launch_grad_dtype(args->dtype, a, GradIn{q->stats, q->slope, q->row_seq, 2 * (int64_t)q->n_pairs, 1.0f, nullptr, q->d_logits, q->d_stride}, f, s);
+  else if (f.loss) hipLaunchKernelGGL(k_preference_final, dim3(1), dim3(256), 0, s, f);
   LD_CHECK_LAUNCH();
   return LIGDIFF_OK;
 }
@@ -927,19 +1031,22 @@ extern "C" int ligdiff_policy_loss(const ligdiff_token_args* args, const ligdiff
     return LIGDIFF_OK;
   }
   const int chunks = (int)seg_chunks(a.n);
-  hipLaunchKernelGGL((k_row_segments<false>), dim3(chunks), dim3(256), 0, s, a.tok, a.n, q->seq_ptr, q->n_seq, (const float*)nullptr,
-                     w.seq_of, (double*)nullptr, per_seq ? w.part_len : nullptr, w.chunk_len);
-  if (per_seq)
+  const bool small = a.n <= SMALL_ROWS && rows_of_16_lanes(args->dtype, a.V);
+  if (!small)
+    hipLaunchKernelGGL((k_row_segments<false>), dim3(chunks), dim3(256), 0, s,
+                       SegRows{a.tok, a.n, q->seq_ptr, q->n_seq, nullptr, w.seq_of, nullptr, per_seq ? w.part_len : nullptr, w.chunk_len});
+  // (in a batch of one chunk a sequence is its one part)
+  if (per_seq && !small && chunks > 1)
     hipLaunchKernelGGL(k_sequence_lengths, dim3(ceil_div(q->n_seq, 4)), dim3(256), 0, s, q->seq_ptr, a.n, q->n_seq, w.part_len, w.seq_len);
   PolicyIn p;
-  p.seq_of = w.seq_of; p.seq_len = w.seq_len; p.chunk_len = w.chunk_len; p.n_chunks = chunks;
+  p.seq_of = w.seq_of; p.seq_len = chunks > 1 ? w.seq_len : w.part_len; p.chunk_len = w.chunk_len; p.n_chunks = chunks;
   p.denom = (double)q->denominator; p.n_seq = q->n_seq; p.per_seq_mean = per_seq;
   p.adv = q->advantage; p.adv_per_token = q->advantage_per_token != 0;
   p.old_logp = q->old_logp; p.ref_logp = q->ref_logp;
   p.clip_lo = q->clip_low; p.clip_hi = q->clip_high; p.kl_coef = q->kl_coef; p.grad_scale = q->grad_scale;
-  p.partial = w.partial;
+  p.partial = w.partial; p.result = q->result; p.seq_ptr = q->seq_ptr;
   const int blocks = launch_rows_dtype<TK_POLICY>(args->dtype, a, p, RowOut{q->logp, nullptr, q->stats, q->coef, q->d_logits, q->d_stride}, s);
-  hipLaunchKernelGGL(k_policy_final, dim3(1), dim3(256), 0, s, w.partial, blocks, (double)q->kl_coef, q->result);
+  if (!small) hipLaunchKernelGGL(k_policy_final, dim3(1), dim3(256), 0, s, w.partial, blocks, (double)q->kl_coef, q->result);
   LD_CHECK_LAUNCH();
   return LIGDIFF_OK;
 }

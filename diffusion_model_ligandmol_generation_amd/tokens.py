@@ -272,13 +272,20 @@ def _preference(logits, tokens, seq_ptr, ref_logp, beta, label_smoothing, kind, 
     nbytes = lib.ligdiff_preference_workspace_bytes(n, P)
     f32 = dict(dtype=torch.float32, device=dev)
     with _on(dev) as stream:
-        loss, log_ratio, margin, slope = (torch.empty(s, **f32) for s in ((), 2 * P, P, 2 * P))
-        stats, row_seq = torch.empty(n, 2, **f32), torch.empty(n, dtype=torch.int32, device=dev)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        d = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
+        loss, log_ratio, margin = torch.empty((), **f32), torch.empty(2 * P, **f32), torch.empty(P, **f32)
+        slope = stats = row_seq = d = None
+        if want_grad:   # what only a later gradient needs lies behind the workspace
+            d = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+            ws = torch.empty(nbytes + 8 * P + 12 * n, dtype=torch.uint8, device=dev)
+            at = ws.data_ptr() + nbytes
+            saved = (at, at + 8 * P, at + 8 * P + 8 * n)
+        else:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            slope, stats, row_seq = torch.empty(2 * P, **f32), torch.empty(n, 2, **f32), torch.empty(n, dtype=torch.int32, device=dev)
+            saved = (slope.data_ptr(), stats.data_ptr(), row_seq.data_ptr())
         q = PreferenceArgs(ptr.data_ptr(), None if ref is None else ref.data_ptr(), P, _lib.PREFERENCE_KINDS[kind],
                            1 if average else 0, beta, label_smoothing, denominator, grad_scale, loss.data_ptr(),
-                           log_ratio.data_ptr(), margin.data_ptr(), slope.data_ptr(), stats.data_ptr(), row_seq.data_ptr(),
+                           log_ratio.data_ptr(), margin.data_ptr(), *saved,
                            None if d is None else d.data_ptr(), V, ws.data_ptr(), nbytes)
         check(lib.ligdiff_preference_loss(C.byref(a), C.byref(q), stream), "ligdiff_preference_loss")
     return loss, log_ratio, margin, slope, stats, row_seq, d
