@@ -207,6 +207,82 @@ __global__ __launch_bounds__(SORT_NT) void k_sort_scatter(SortPass a) {
   }
 }
 
+// Up to SORT_SMALL positions: all passes of 8 bits by one block in LDS, one launch instead of two a pass.
+#define SORT_SMALL 4096
+#define SORT_SMALL_NT 1024
+template <int PASSES>
+__global__ __launch_bounds__(SORT_SMALL_NT) void k_sort_small(SortPass a) {
+  constexpr int WAVES = SORT_SMALL_NT / 64, EACH = SORT_SMALL / SORT_SMALL_NT;   // positions of a lane: 64 apart in its wave's part
+  __shared__ uint32_t key[SORT_SMALL];
+  __shared__ uint16_t pos[SORT_SMALL];
+  __shared__ int cnt[WAVES][256];
+  __shared__ int wtot[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = (int)a.n, w0 = wave * 64 * EACH;
+  uint32_t k[EACH];
+  uint16_t p[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int i = w0 + e * 64 + lane;
+    k[e] = i < n ? sort_key<true>(a, i) : 0;
+    p[e] = (uint16_t)i;
+  }
+#pragma unroll
+  for (int pass = 0; pass < PASSES; ++pass) {
+    for (int i = tid; i < WAVES * 256; i += SORT_SMALL_NT) (&cnt[0][0])[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < EACH; ++e)
+      if (w0 + e * 64 + lane < n) atomicAdd(&cnt[wave][(k[e] >> (8 * pass)) & 255], 1);
+    __syncthreads();
+    int total = 0, scan = 0;
+    if (tid < 256) {
+      for (int w = 0; w < WAVES; ++w) total += cnt[w][tid];
+      scan = total;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(scan, o); if (lane >= o) scan += u; }
+      if (lane == 63) wtot[wave] = scan;
+    }
+    __syncthreads();
+    if (tid < 256) {
+      int run = scan - total;
+      for (int w = 0; w < wave; ++w) run += wtot[w];
+      if (PASSES == 1 && a.row_ptr && tid <= a.rows) a.row_ptr[tid] = run;
+      for (int w = 0; w < WAVES; ++w) { const int c = cnt[w][tid]; cnt[w][tid] = run; run += c; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const bool on = w0 + e * 64 + lane < n;
+      const int d = (int)(k[e] >> (8 * pass)) & 255;
+      uint64_t same = __ballot(on);
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        const uint64_t set = __ballot((d >> b) & 1);
+        same &= (d >> b) & 1 ? set : ~set;
+      }
+      const int rank = __popcll(same & ((1ull << lane) - 1));
+      int at = 0;
+      if (on) at = cnt[wave][d];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (on && rank == 0) cnt[wave][d] = at + __popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (on) {
+        if (pass == PASSES - 1) { a.key_out[at + rank] = k[e]; a.pos_out[at + rank] = p[e]; }
+        else { key[at + rank] = k[e]; pos[at + rank] = p[e]; }
+      }
+    }
+    if (pass < PASSES - 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int i = w0 + e * 64 + lane;
+        if (i < n) { k[e] = key[i]; p[e] = pos[i]; }
+      }
+      __syncthreads();
+    }
+  }
+}
+
 // ------------------------------------------------------------------ sums of rows of equal tokens
 struct SegIn {
   const void* d_out; int64_t d_stride;
@@ -456,6 +532,19 @@ static EmbedWs embed_ws(void* base, int64_t n, int32_t rows, int32_t width) {
 }
 size_t embed_grad_workspace(int64_t n, int32_t rows, int32_t width) { return embed_ws(nullptr, n, rows, width).bytes; }
 
+// Sorts into key[0] / pos[0]; returns whether it wrote row_ptr.
+static bool sort_small(const EmbedGrad& g, const EmbedWs& w, hipStream_t s) {
+  SortPass a{};
+  a.tok = g.tok; a.n = g.n; a.key_out = w.key[0]; a.pos_out = w.pos[0]; a.rows = g.rows;
+  const int passes = sort_passes(g.tok.n_rows, 8);
+  const bool ptr = passes == 1 && g.rows < 256;
+  a.row_ptr = ptr ? w.row_ptr : nullptr;
+  if (passes == 1) hipLaunchKernelGGL(k_sort_small<1>, dim3(1), dim3(SORT_SMALL_NT), 0, s, a);
+  else if (passes == 2) hipLaunchKernelGGL(k_sort_small<2>, dim3(1), dim3(SORT_SMALL_NT), 0, s, a);
+  else if (passes == 3) hipLaunchKernelGGL(k_sort_small<3>, dim3(1), dim3(SORT_SMALL_NT), 0, s, a);
+  else hipLaunchKernelGGL(k_sort_small<4>, dim3(1), dim3(SORT_SMALL_NT), 0, s, a);
+  return ptr;
+}
 template <int BITS> static int sort_tokens(const EmbedGrad& g, const EmbedWs& w, hipStream_t s) {
   SortPass a;
   a.tok = g.tok; a.n = g.n; a.per_block = sort_per_block(g.n, BITS); a.hist = w.hist; a.rows = g.rows;
@@ -497,7 +586,9 @@ void embed_grad(const EmbedGrad& g, void* workspace, hipStream_t s) {
   SegIn a;
   a.have_ptr = false;
   int passes = 1;
-  if (g.n > 0) {
+  if (g.n > 0 && g.n <= SORT_SMALL) {
+    a.have_ptr = sort_small(g, w, s);
+  } else if (g.n > 0) {
     const int bits = sort_bits(g.rows);
     passes = bits == 8 ? sort_tokens<8>(g, w, s) : sort_tokens<11>(g, w, s);
     a.have_ptr = passes == 1 && g.rows < (1 << bits);

@@ -14,6 +14,7 @@ owns its backward pass hands it on with ``logits.backward(d_logits)`` and saves 
 The reference has no counterpart (one-hot types, no loss on the distribution of ``atom_pred``)."""
 import ctypes as C
 from collections import namedtuple
+from functools import lru_cache
 
 import torch
 
@@ -50,6 +51,11 @@ class _on:
     def __exit__(self, *exc):
         if self.back is not None:
             torch.cuda.set_device(self.back)
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(entry, *sizes):
+    return getattr(_lib.load(), entry)(*sizes)
 
 
 def _check_float(t, name):
@@ -164,7 +170,7 @@ def embed_tokens_grad(d_out, tokens, n_rows, scale=1.0, out=None, accumulate=Fal
     _check_ids(tokens, dev)
     scale, n_rows = _finite_scale(scale, "scale"), int(n_rows)
     D = d_out.shape[-1] if d_out.dim() else 0
-    if n_rows < 1 or D < 1 or tuple(d_out.shape[:-1]) != tuple(tokens.shape):
+    if n_rows < 1 or D < 1 or d_out.shape[:-1] != tokens.shape:
         raise ValueError("d_out must be [*tokens.shape, width] with width and n_rows at least 1")
     rows, n, stride = _rows(d_out, D)
     ids = tokens.contiguous()
@@ -177,7 +183,7 @@ def embed_tokens_grad(d_out, tokens, n_rows, scale=1.0, out=None, accumulate=Fal
     elif (D > 1 and out.stride(1) != 1) or (n_rows > 1 and out.stride(0) < D):
         raise ValueError("out must have rows of unit stride that do not overlap")
     lib = _lib.load()
-    nbytes = lib.ligdiff_embed_grad_workspace_bytes(n, n_rows, D)
+    nbytes = _workspace_bytes("ligdiff_embed_grad_workspace_bytes", n, n_rows, D)
     with _on(dev) as stream:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         check(lib.ligdiff_embed_grad(rows.data_ptr(), _DTYPES[rows.dtype], stride, ids.data_ptr(), _TOKEN_BYTES[ids.dtype], n,
@@ -194,7 +200,7 @@ def _token_args(logits, tokens, temperature):
         raise ValueError("logits must be [..., vocabulary]")
     dev = logits.device
     _check_ids(tokens, dev)
-    if tuple(tokens.shape) != tuple(logits.shape[:-1]):
+    if tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
     temperature = float(temperature)
     if not 0.0 < temperature <= 3e38:
@@ -269,7 +275,7 @@ def _preference(logits, tokens, seq_ptr, ref_logp, beta, label_smoothing, kind, 
     ref = None if ref_logp is None else _vector(ref_logp, n, dev, "ref_logp")
     denominator, grad_scale = _denominator(denominator), _finite_scale(grad_scale, "grad_scale")
     lib = _lib.load()
-    nbytes = lib.ligdiff_preference_workspace_bytes(n, P)
+    nbytes = _workspace_bytes("ligdiff_preference_workspace_bytes", n, P)
     f32 = dict(dtype=torch.float32, device=dev)
     with _on(dev) as stream:
         loss, log_ratio, margin = torch.empty((), **f32), torch.empty(2 * P, **f32), torch.empty(P, **f32)
@@ -352,7 +358,7 @@ def _policy(logits, tokens, seq_ptr, advantage, old_logp, ref_logp, advantage_pe
     denominator, grad_scale = _denominator(denominator), _finite_scale(grad_scale, "grad_scale")
     mean = _lib.POLICY_MEANS[aggregate]
     lib = _lib.load()
-    nbytes = lib.ligdiff_policy_workspace_bytes(n, S, mean)
+    nbytes = _workspace_bytes("ligdiff_policy_workspace_bytes", n, S, mean)
     f32 = dict(dtype=torch.float32, device=dev)
     with _on(dev) as stream:
         result, logp = torch.empty(4, **f32), torch.empty(tokens.shape, **f32)
