@@ -224,6 +224,7 @@ SIGNATURES = {
 }
 
 FWD_PROPERTIES, FWD_NULL_COND, FWD_SKIP_PROP_HEAD, FWD_SAVE_FOR_BACKWARD, FWD_T_BROADCAST = 1, 2, 4, 8, 16
+FWD_ATOM_TYPES = 32
 
 _lib = None
 

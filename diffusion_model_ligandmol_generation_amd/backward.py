@@ -6,7 +6,7 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .engine import _ptr, _stream
+from .engine import _ptr, _stream, node_features
 
 
 def _has_grad_slot(name):
@@ -119,14 +119,13 @@ class ScoreNetworkFunction(torch.autograd.Function):
         over which backward sums the parameter gradients.  ``model.library_options`` (an engine Options struct, else
         absent): per-call options of the forward / backward pair, e.g. the split-operand GEMM mode."""
         N, B = graph.n_atoms, graph.n_mols
-        x = x.detach().contiguous().float()
+        x, flags = node_features(x.detach(), N)
         pos = pos.detach().contiguous().float()
         t = t.detach().reshape(-1).contiguous().float()
         if t.numel() == 1 and B > 1:
             t = t.repeat(B)
         if t.numel() != B:
             raise ValueError("t needs one value per molecule")
-        flags = 0
         props = None
         if properties is not None:
             flags |= _lib.FWD_PROPERTIES

@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include "forward.h"
+#include "embed.h"
 #include "gemm_bwd.h"
 #include "gemm_dw.h"
 #include "launch.h"
@@ -19,6 +20,8 @@ struct BwdLayout {
   size_t dmod[LD_MAXL], b256a, b256b, b256c, b256d, b512, b2048, b8, bhid;
   size_t wt;   // transposed weight block of the dX GEMM in flight (<= 1536 x 256 elements, fp32 or split bf16: 6 bytes each)
   size_t wt_all, wt_all_floats;   // every weight block the input-gradient GEMMs need transposed, filled by ONE launch
+  size_t types;              // LIGDIFF_FWD_ATOM_TYPES: gradients of the per-type atom branch, [2][LD_A + 1, 256]
+  size_t sort, sort_bytes;   // and the workspace of the sums over equal types
   size_t pool, pool_bytes;   // single-use buffers: everything a weight-gradient launch on the side stream reads
   size_t total;
 };
@@ -54,6 +57,9 @@ static void bwd_layout(BwdLayout* L, int64_t N, int64_t E, int32_t B) {
   L->wt = take(1536 * 256 * 3 / 2);
   L->wt_all_floats = WT_ALL_FLOATS(nl);
   L->wt_all = take(L->wt_all_floats);
+  L->types = take(2 * (LD_A + 1) * 256);
+  L->sort_bytes = embed_grad_workspace(N, LD_A + 1, 256);
+  L->sort = take(L->sort_bytes / 4);
   L->pool = off;
   L->pool_bytes = bwd_pool_bytes(N, E, nl);
   off += L->pool_bytes;
@@ -595,10 +601,22 @@ extern "C" int ligdiff_backward_train(const float* const* w, float* const* gr, c
 
   // ------------------------------------------------------------------ embeddings (model1.py:709-718)
   {
-    float* du = fresh((int64_t)N * 256);
-    ln_bwd<0, 1>(A(F.ua), 256, w[W_ATOM_G], w[W_ATOM_BE], 1e-5f, dxa, 256, nullptr, 0, nullptr, du, 256, gr[W_ATOM_G],
-                 gr[W_ATOM_BE], N, s);
-    gemm_dw_direct(du, 256, 256, x, LD_A, LD_A, N, gr[W_ATOM_W], LD_A, side.fork(), gr[W_ATOM_B]);
+    if (flags & LIGDIFF_FWD_ATOM_TYPES) {
+      // all atoms of a type share the branch's input: sum their gradients by sorted types, then LayerNorm and weights on
+      // LD_A + 1 rows
+      float* dt = T(L.types);
+      float* du = dt + (LD_A + 1) * 256;
+      const EmbedGrad eg{dxa, LIGDIFF_F32, 256, TokenView{x, 4, LD_A}, N, LD_A + 1, 256, 1.0f, dt, LIGDIFF_F32, 256, false};
+      embed_grad(eg, T(L.sort), s);
+      ln_bwd<0, 1>(A(F.type_pre), 256, w[W_ATOM_G], w[W_ATOM_BE], 1e-5f, dt, 256, nullptr, 0, nullptr, du, 256, gr[W_ATOM_G],
+                   gr[W_ATOM_BE], LD_A + 1, s);
+      hipLaunchKernelGGL(k_type_embed_dw, dim3(LD_A + 1), dim3(256), 0, s, du, gr[W_ATOM_W], gr[W_ATOM_B]);
+    } else {
+      float* du = fresh((int64_t)N * 256);
+      ln_bwd<0, 1>(A(F.ua), 256, w[W_ATOM_G], w[W_ATOM_BE], 1e-5f, dxa, 256, nullptr, 0, nullptr, du, 256, gr[W_ATOM_G],
+                   gr[W_ATOM_BE], N, s);
+      gemm_dw_direct(du, 256, 256, x, LD_A, LD_A, N, gr[W_ATOM_W], LD_A, side.fork(), gr[W_ATOM_B]);
+    }
     float* up = T(L.n256c);
     float* dup = fresh((int64_t)N * 256);
     hipLaunchKernelGGL(k_pos_embed_pre, dim3(nb4N), dim3(256), 0, s, pos, w[W_POS_W], w[W_POS_B], up, N);

@@ -29,6 +29,7 @@ struct FwdLayout {
   size_t t1_pre, ua, pen_pre, pg_pre, pz, pw;
   size_t pre_e[LD_MAXL], u_m[LD_MAXL], hc_pre[LD_MAXL], cw[LD_MAXL], dist[LD_MAXL], r1pre[LD_MAXL], hid_pre[LD_MAXL], u_h[LD_MAXL];
   size_t oproj[LD_MAXL], fproj[LD_MAXL], ffh_pre[LD_MAXL], lse[LD_MAXL], u_head, u_ph;
+  size_t type_pre, type_emb;        // LIGDIFF_FWD_ATOM_TYPES: [LD_A + 1, 256] atom branch per type, before LayerNorm and after GELU
   size_t wsplit, wsplit_bytes;      // split-bf16 copies of the GEMM weights (split-operand mode only, else 0 bytes)
   size_t total;
 };
@@ -69,7 +70,7 @@ struct FwdProbe { const char* label; hipEvent_t e0, e1; int hits; };
 
 // Bits a caller of the C ABI may set in `flags` (the LIGDIFF_FWD_* values); anything else is refused.
 #define FWD_PUBLIC_FLAGS (LIGDIFF_FWD_PROPERTIES | LIGDIFF_FWD_NULL_COND | LIGDIFF_FWD_SKIP_PROP_HEAD | \
-                          LIGDIFF_FWD_SAVE_FOR_BACKWARD | LIGDIFF_FWD_T_BROADCAST)
+                          LIGDIFF_FWD_SAVE_FOR_BACKWARD | LIGDIFF_FWD_T_BROADCAST | LIGDIFF_FWD_ATOM_TYPES)
 // Shape / pointer validation of a caller's ligdiff_graph, shared by every entry point that takes one
 // (sizes positive and below 2^30, arrays present, largest molecule within LIGDIFF_MAX_ATOMS).
 int check_graph(const ligdiff_graph* g);

@@ -345,6 +345,7 @@ void fwd_layout(FwdLayout* L, int64_t N, int64_t E, int32_t B, int flags) {
     }
     L->u_head = take(N * 512); L->u_ph = take((size_t)B * 256);
   }
+  if (flags & LIGDIFF_FWD_ATOM_TYPES) { L->type_pre = take((LD_A + 1) * 256); L->type_emb = take((LD_A + 1) * 256); }
   L->wsplit = off;
   L->wsplit_bytes = split_gemm_enabled() ? split_region_bytes(nl) : 0;
   off += L->wsplit_bytes;
@@ -488,7 +489,13 @@ int run_forward(const float* const* w, const ligdiff_graph* g, const float* x, c
     e.temb = F(L.temb); e.temb_stride = tstride; e.pemb = pemb; e.pemb_stride = pstride;
     e.atom_mol = g->atom_mol; e.H = F(L.h0); e.ua_out = S(L.ua);
     PB("embed");
-    if (use_cs()) {
+    if (flags & LIGDIFF_FWD_ATOM_TYPES) {
+      hipLaunchKernelGGL(k_type_embed, dim3(ceil_div(LD_A + 1, 4)), dim3(256), 0, s, w[W_ATOM_W], w[W_ATOM_B], w[W_ATOM_G],
+                         w[W_ATOM_BE], F(L.type_pre), F(L.type_emb));
+      hipLaunchKernelGGL(k_pos_embed, dim3(ceil_div(N, 4)), dim3(256), 0, s, pos, w[W_POS_W], w[W_POS_B], w[W_POS_G],
+                         w[W_POS_BE], F(L.temb), tstride, pemb, pstride, g->atom_mol, F(L.h0), N, pemb_mols, nullptr, nullptr,
+                         nullptr, nullptr, reinterpret_cast<const int32_t*>(x), F(L.type_emb));
+    } else if (use_cs()) {
       // h = GELU(LN(x Wa^T + ba)) + R,  R = GELU(LN(pos Wp^T + bp)) + t_emb (+ prop_emb); the same launch
       // zero-extends x and Wa to 128 columns for the GEMM (64 extra workgroups for the weight rows)
       float* R = F(L.xn1[0]);   // free until the attention layers

@@ -5,7 +5,7 @@ import torch
 
 
 class MoleculeBatch:
-    """Attribute bag with the fields model.forward / the trainer read: x [N,119], pos [N,3],
+    """Attribute bag with the fields model.forward / the trainer read: x [N,119] (or integer atom types [N]), pos [N,3],
     edge_index [2,E] int64 (atom indices offset by the molecule's first atom), batch [N] int64,
     properties [B,15] or None."""
 
@@ -24,13 +24,16 @@ class MoleculeBatch:
 def collate_molecules(mols):
     """PyG-style collation (main.py:205-212): node arrays concatenated along dim 0, edge_index columns
     offset by the number of preceding atoms, batch[i] = molecule of atom i.  ``mols``: dicts (or
-    objects) with x [n,119], pos [n,3], edge_index [2,e] and optionally properties [15]."""
+    objects) with x [n,119] or integer atom types [n] (the same in all of them), pos [n,3], edge_index [2,e] and
+    optionally properties [15]."""
     get = (lambda m, k: m[k]) if isinstance(mols[0], dict) else getattr
     has = (lambda m, k: k in m) if isinstance(mols[0], dict) else hasattr
     xs, ps, es, bs, prs = [], [], [], [], []
     off = 0
     for i, m in enumerate(mols):
-        x = torch.as_tensor(get(m, "x"), dtype=torch.float32)
+        x = torch.as_tensor(get(m, "x"))
+        if x.dim() != 1 or x.is_floating_point() or x.dtype == torch.bool:   # (1-D integers: atom types)
+            x = x.float()
         n = x.shape[0]
         xs.append(x)
         ps.append(torch.as_tensor(get(m, "pos"), dtype=torch.float32))

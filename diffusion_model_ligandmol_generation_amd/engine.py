@@ -33,6 +33,21 @@ def _require_cuda(t, name):
         raise RuntimeError(f"{name} must live on a HIP device: the hot path has no CPU implementation")
 
 
+def node_features(x, n_atoms):
+    """(tensor, flags) of a model's node input as the library takes it: [N,119] fp32 features, or integer atom types [N]
+    (int32, FWD_ATOM_TYPES), which stand for their one-hot rows."""
+    if x.dim() == 1 and not x.is_floating_point() and x.dtype != torch.bool:
+        if x.shape[0] != n_atoms:
+            raise ValueError("atom types must be [N]")
+        if x.dtype != torch.int32:   # (a wider type's value keeps its meaning: what does not fit is no type)
+            x = torch.where((x >= 0) & (x < 119), x, torch.full_like(x, 119)).to(torch.int32)
+        return x.contiguous(), _lib.FWD_ATOM_TYPES
+    x = x.contiguous().float()
+    if x.shape != (n_atoms, 119):
+        raise ValueError("x must be [N,119] and pos [N,3]")
+    return x, 0
+
+
 class PackedGraph:
     """Device-resident CSR form of a ragged batch (struct ligdiff_graph).
 
@@ -221,12 +236,11 @@ class ScoreNetworkEngine:
         self._check_sizes(graph)
         for name, v in (("x", x), ("pos", pos), ("t", t)):
             _require_cuda(v, name)
-        x = x.contiguous().float()
+        x, flags = node_features(x, N)
         pos = pos.contiguous().float()
         t = t.reshape(-1).contiguous().float()
-        if x.shape != (N, 119) or pos.shape != (N, 3):
+        if pos.shape != (N, 3):
             raise ValueError("x must be [N,119] and pos [N,3]")
-        flags = 0
         if t_index is not None:
             if t_index.dtype != torch.int32 or not t_index.is_cuda:
                 raise ValueError("t_index must be a device int32 tensor")

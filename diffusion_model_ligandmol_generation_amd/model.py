@@ -120,8 +120,8 @@ class ResearchAccurateDiffusionModel(nn.Module):
         return d
 
     def forward(self, data, t, properties=None, classifier_free_guidance=False):
-        """model1.py:699-755.  ``data`` is any object with .x [N,119], .pos [N,3],
-        .edge_index [2,E] int64 and .batch [N] int64 (sorted).  Returns
+        """model1.py:699-755.  ``data`` is any object with .x [N,119] (or integer atom types [N], which stand for their
+        one-hot rows: the embedding is then a lookup), .pos [N,3], .edge_index [2,E] int64 and .batch [N] int64 (sorted).  Returns
         (atom_pred [N,119], pos_pred [N,3], prop_pred [B,15], consistency_outputs).
 
         Train mode applies the attention layers' dropout (see ``dropout_spec``); ``data.dropout_seed``

@@ -100,7 +100,7 @@ class ResearchAccurateTrainer:
         model = self.model
         eng = model.engine()
         lib = eng.lib
-        x = batch.x.to(dev).float().contiguous()
+        x = batch.x.to(dev)                    # [N,119], or integer atom types [N] (the model takes either)
         pos = batch.pos.to(dev).float().contiguous()
         N = x.shape[0]
         if getattr(batch, "batch", None) is None:                                   # train.py:281-284
@@ -202,6 +202,123 @@ class ResearchAccurateTrainer:
         losses["dit_total"] = vals[3] + vals[4]
         losses["e3_total"] = vals[5] + vals[6] + vals[7]
         return losses
+
+    # ------------------------------------------------------------------ fine-tuning on atom types
+    def _fine_tune_draws(self, batch, draws):
+        """The random numbers of one noised forward pass: given ones, or new ones on the trainer's device.  Reference,
+        sampling and trained policy are compared at the same noise, so one set goes to all of them."""
+        draws = dict(draws or {})
+        n_mols = int(batch.batch.max()) + 1 if getattr(batch, "batch", None) is not None else 1
+        if "u" not in draws:
+            draws["u"] = torch.rand(n_mols, device=self.device)
+        if "noise" not in draws:
+            draws["noise"] = torch.randn(batch.pos.shape, device=self.device)
+        return draws
+
+    def _atom_type_logits(self, model, batch, draws):
+        """``atom_pred`` [N,119] of ``model`` on the batch with its coordinates noised as in the training step
+        (train.py:286-312), and the packed graph."""
+        dev = self.device
+        eng = model.engine()
+        pos = batch.pos.to(dev).float().contiguous()
+        if getattr(batch, "batch", None) is None:
+            batch.batch = torch.zeros(pos.shape[0], dtype=torch.long, device=dev)
+        batch.batch = batch.batch.to(dev)
+        batch.edge_index = batch.edge_index.to(dev)
+        graph = packed_graph_of(batch)
+        N, B = graph.n_atoms, graph.n_mols
+        u, noise = draws["u"].to(dev).float().contiguous(), draws["noise"].to(dev).float().contiguous()
+        if u.shape != (B,) or noise.shape != (N, 3):
+            raise ValueError("draws must hold u [B] and noise [N,3]")
+        edm = model.edm_preconditioning
+        coef, c_noise = torch.empty(B, 4, device=dev), torch.empty(B, device=dev)
+        noisy, pre_pos = torch.empty_like(pos), torch.empty_like(pos)
+        with torch.cuda.device(dev):
+            check(eng.lib.ligdiff_edm_prepare(_ptr(u), _ptr(pos), _ptr(noise), _ptr(graph.atom_mol), N, B,
+                                              float(edm.sigma_min), float(edm.sigma_max), float(edm.sigma_data), _ptr(coef),
+                                              _ptr(c_noise), _ptr(noisy), _ptr(pre_pos), _stream()), "ligdiff_edm_prepare")
+
+        class _Data:
+            pass
+
+        d = _Data()
+        d.x, d.pos, d.edge_index, d.batch, d._ligdiff_graph = batch.x.to(dev), pre_pos, batch.edge_index, batch.batch, graph
+        d.skip_consistency = True
+        if "dropout_seed" in draws:
+            d.dropout_seed = int(draws["dropout_seed"])
+        props = getattr(batch, "properties", None)
+        return model(d, c_noise, None if props is None else props.to(dev).float())[0], graph
+
+    @staticmethod
+    def _atom_types(batch, device):
+        types = getattr(batch, "atom_types", None)
+        if types is None:
+            raise ValueError("the batch needs atom_types [N], the types that were chosen")
+        return types.to(device)
+
+    def atom_type_logprobs(self, batch, draws=None, model=None, temperature=1.0):
+        """(logp [N], draws): log-probabilities that ``model`` (the trainer's own by default; a frozen copy as the
+        reference) gives to ``batch.atom_types`` at the noise of ``draws``, without gradient.  Hand the same draws and the
+        returned values to ``preference_step`` / ``policy_step``.  Dropout follows the model's mode: ``model.eval()`` (gradients
+        flow all the same), or a ``dropout_seed`` in the draws, keeps its noise out of the ratios."""
+        from .tokens import token_logprobs
+        model = self.model if model is None else model
+        draws = self._fine_tune_draws(batch, draws)
+        with torch.no_grad():
+            logits, _ = self._atom_type_logits(model, batch, draws)
+            return token_logprobs(logits, self._atom_types(batch, self.device), temperature), draws
+
+    def _fine_tune_update(self, logits, result):
+        """Backward pass from the gradient of the logits, gradient sum over the ranks, clipping and optimiser step."""
+        self.optimizer.zero_grad()
+        logits.backward(result.d_logits)
+        self._allreduce_gradients()
+        self.optimizer.clip_and_step(self.model, max_norm=1.0)
+        self.step_count += 1
+
+    def _sum_over_ranks(self, *values):
+        """Each of the numbers summed over the process group (host-side)."""
+        if self.group is None:
+            return values
+        import torch.distributed as dist
+        t = torch.tensor(values, dtype=torch.float64)
+        dist.all_reduce(t, group=self.count_group)
+        return tuple(t.tolist())
+
+    def preference_step(self, batch, draws, ref_logp=None, beta=0.1, label_smoothing=0.0, kind="sigmoid", average=False,
+                        temperature=1.0):
+        """One optimiser step on pairs of ligands: of the 2 P molecules of the batch, number p is preferred over number
+        P + p (``tokens.preference_loss`` on ``atom_pred`` and ``batch.atom_types``).  ``draws`` and ``ref_logp`` come from
+        ``atom_type_logprobs(batch, model=reference)``.  Under data parallelism each rank brings its own pairs and the
+        loss is the mean over all of them.  Returns tokens.PreferenceGrad (this rank's share of the loss)."""
+        from .tokens import preference_loss_and_grad
+        types = self._atom_types(batch, self.device)
+        draws = self._fine_tune_draws(batch, draws)
+        logits, graph = self._atom_type_logits(self.model, batch, draws)
+        pairs, = self._sum_over_ranks(graph.n_mols // 2)
+        r = preference_loss_and_grad(logits, types, graph.mol_ptr, ref_logp, beta, label_smoothing, kind, average, temperature,
+                                     denominator=pairs if self.group is not None else None)
+        self._fine_tune_update(logits, r)
+        return r
+
+    def policy_step(self, batch, draws, advantage, old_logp=None, ref_logp=None, advantage_per="sequence", clip_low=0.2,
+                    clip_high=0.2, kl_coef=0.0, aggregate="token", temperature=1.0):
+        """One optimiser step on rewards (``tokens.policy_loss`` on ``atom_pred`` and ``batch.atom_types``): ``advantage`` has
+        one value for each molecule (or atom), ``old_logp`` are the log-probabilities under the policy that chose the
+        types, ``ref_logp`` those under the reference, both from ``atom_type_logprobs`` with the same ``draws``.  Under data
+        parallelism the mean goes over all ranks' atoms / molecules.  Returns tokens.PolicyGrad (this rank's share)."""
+        from .tokens import policy_loss_and_grad
+        types = self._atom_types(batch, self.device)
+        draws = self._fine_tune_draws(batch, draws)
+        logits, graph = self._atom_type_logits(self.model, batch, draws)
+        denominator = None
+        if self.group is not None:
+            own = graph.n_mols if aggregate == "sequence" else int(((types >= 0) & (types < logits.shape[1])).sum())
+            denominator, = self._sum_over_ranks(own)
+        r = policy_loss_and_grad(logits, types, graph.mol_ptr, advantage, old_logp, ref_logp, advantage_per, clip_low, clip_high,
+                                 kl_coef, aggregate, temperature, denominator=denominator)
+        self._fine_tune_update(logits, r)
+        return r
 
     # ------------------------------------------------------------------ optimisation step
     def _allreduce_gradients(self):

@@ -190,7 +190,9 @@ enum ligdiff_forward_flags {
   LIGDIFF_FWD_NULL_COND = 2,    /* classifier_free_guidance=True: learned null vector     */
   LIGDIFF_FWD_SKIP_PROP_HEAD = 4, /* do not compute prop_pred (samplers ignore it)        */
   LIGDIFF_FWD_SAVE_FOR_BACKWARD = 8, /* keep activations in the workspace for backward    */
-  LIGDIFF_FWD_T_BROADCAST = 16  /* t has ONE element used for every molecule              */
+  LIGDIFF_FWD_T_BROADCAST = 16, /* t has ONE element used for every molecule              */
+  LIGDIFF_FWD_ATOM_TYPES = 32   /* `x` points to int32 atom types [N] instead of one-hot   */
+                                /* rows [N,119]; a type outside [0,119) is a row of zeros  */
 };
 
 size_t ligdiff_forward_workspace_bytes(int64_t n_atoms, int64_t n_edges, int32_t n_mols, int flags);
@@ -203,6 +205,9 @@ size_t ligdiff_forward_workspace_bytes(int64_t n_atoms, int64_t n_edges, int32_t
  * (may be NULL with LIGDIFF_FWD_SKIP_PROP_HEAD).
  * t_index_dev: if non-NULL, a device int32; the time value used is (float)*t_index_dev
  * for every molecule and `t` is ignored (lets a captured graph step through time).
+ * With LIGDIFF_FWD_ATOM_TYPES the atom branch GELU(LN(x Wa^T + ba)) of the embedding (model1.py:599-609) is looked up in a
+ * table of its 120 possible rows instead of computed per atom (the results agree to rounding); the backward call takes
+ * the same x and flags.  The sampling loops, whose x is continuous, do not take it.
  */
 int ligdiff_forward(const float* const* weights, const ligdiff_graph* graph, const float* x,
                     const float* pos, const float* t, const int32_t* t_index_dev,
