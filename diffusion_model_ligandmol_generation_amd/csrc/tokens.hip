@@ -275,8 +275,8 @@ __device__ __forceinline__ void set_pack(u32x4& x, const float (&v)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) x[j] = __float_as_uint(v[j]);
 }
-template <typename T, int NV, typename F>
-__device__ __forceinline__ void exponentials(u32x4 (&x)[NV], float m, float mc, float c, bool far, F&& take) {
+template <typename T, int NV, int TPR, typename F>
+__device__ __forceinline__ void exponentials(u32x4 (&x)[NV], int nb, float m, float mc, float c, bool far, F&& take) {
   constexpr int N = Pack<T>::N;
   if (__builtin_expect(far, 0)) {
 #pragma unroll
@@ -290,6 +290,7 @@ __device__ __forceinline__ void exponentials(u32x4 (&x)[NV], float m, float mc, 
   } else {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
+      if (k > 0 && k * TPR >= nb) break;   // no lane has a pack here
       if (sizeof(T) == 2) asm volatile("" : "+v"(x[k]));
       float e[N];
 #pragma unroll
@@ -302,7 +303,7 @@ __device__ __forceinline__ void exponentials(u32x4 (&x)[NV], float m, float mc, 
 // Short rows are loaded one row ahead of their arithmetic: a wave has two rows' bytes under way.
 #define ROW_AHEAD(TPR, REGS, MODE) ((TPR) <= 64 && (REGS) <= 8)
 // Waves a SIMD holds at once: what the registers of a row allow.
-#define ROW_WAVES(TPR, REGS, MODE) ((MODE) == TK_LOGP ? ((REGS) <= 16 ? 8 : 6) : (TPR) == 1024 ? ((REGS) <= 16 ? 8 : 4) : (REGS) <= 8 ? 6 : (REGS) <= 16 ? 5 : 4)
+#define ROW_WAVES(TPR, REGS, MODE) ((MODE) == TK_LOGP ? ((REGS) <= 16 ? 8 : (REGS) <= 32 ? 6 : 4) : (TPR) == 1024 ? ((REGS) <= 16 ? 8 : 4) : (REGS) <= 8 ? 6 : (REGS) <= 16 ? 5 : 4)
 
 // Rows that fit the registers of TPR lanes, NV packs a lane: the logits are read once, exponentiated once, and the policy
 // loss writes its gradient from the same registers.  TPR = 16 / 64: several rows a block and no barrier; 256 / 1024: one
@@ -385,9 +386,11 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
     if constexpr (MODE != TK_LOGP) w = p.per_seq_mean ? inv_total / (double)len : inv_total;
     float m = et;
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+      if (k > 0 && k * TPR >= nb) break;
 #pragma unroll
       for (int j = 0; j < N; ++j) m = fmaxf(m, raw_get<T>(x[k], j));
+    }
     m = group_max<GRP>(m);
     // this wave's own part: e = exp2(c x - mc)
     const bool none = m == -__builtin_inff(), far = !none && far_out(m);
@@ -395,7 +398,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
     float s;
     if (__builtin_expect(far, 0)) s = et = __builtin_amdgcn_exp2f(shifted(et, m) * a.c);
     else s = et = __builtin_amdgcn_exp2f(fmaf(et, a.c, -mc));
-    exponentials<T, NV>(x, m, mc, a.c, far, [&](int k, float (&e)[N]) {
+    exponentials<T, NV, TPR>(x, nb, m, mc, a.c, far, [&](int k, float (&e)[N]) {
 #pragma unroll
       for (int j = 0; j < N; ++j) s += e[j];
       if constexpr (KEEP) set_pack(x[k], e);
@@ -446,7 +449,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
           out(k, e);
         }
       } else {
-        exponentials<T, NV>(x, m, mc, a.c, far, out);
+        exponentials<T, NV, TPR>(x, nb, m, mc, a.c, far, out);
       }
       if (r < tail) d[nb * N + r] = (T)(q * et + (nb * N + r == id ? g : 0.f));
     }
@@ -838,8 +841,13 @@ static int launch_rows_as(const TokenRows& a, const PolicyIn& p, const RowOut& o
 }
 // A batch of at most SMALL_ROWS short rows is one launch of one block: three launches take longer than its four rounds.
 static bool rows_of_16_lanes(int dtype, int32_t V) { return V / (dtype == LIGDIFF_F32 ? 4 : 8) <= 64; }
-// The least lanes whose registers hold a row: 16 lanes up to 64 packs, a wave up to 512, 256 lanes up to 2048, 1024 up to
-// 8192 (32768 fp32 or 65536 half-precision logits); beyond that the row is read twice.  Returns the number of blocks.
+// The fewest lanes whose registers hold a row, and the fewest packs a lane: 16 lanes up to 128 packs, a wave up to 512, 256 lanes
+// up to 2048, 1024 up to 8192 (32768 fp32 or 65536 half-precision logits).  More lanes than that wait for each other more
+// often and hold fewer rows under way.  Measured on 268 MB of fp32 logits, log-probabilities / policy loss with gradient, us:
+// 128 packs 16 lanes 41/110, 64 lanes 49/125, 256 lanes 168/345; 512 packs 64 lanes 41/112, 256 lanes 52/127; 2048 packs
+// 256 lanes 42/111, 1024 lanes 53/113; 8192 packs 1024 lanes 44/114, reading twice 45/167.  So beyond 8192 packs the
+// log-probabilities stream the row (one read in either form: 12000 packs 45 against 47) and the policy loss keeps it up to
+// 16384 packs (134 against 171).  Returns the number of blocks.
 template <typename T, int MODE>
 static int launch_rows(const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
   const int packs = a.V / Pack<T>::N;
@@ -852,13 +860,16 @@ static int launch_rows(const TokenRows& a, const PolicyIn& p, const RowOut& o, h
   if (packs <= 16) return launch_rows_as<T, 16, 1, MODE>(a, p, o, s);
   if (packs <= 32) return launch_rows_as<T, 16, 2, MODE>(a, p, o, s);
   if (packs <= 64) return launch_rows_as<T, 16, 4, MODE>(a, p, o, s);
-  if (packs <= 128) return launch_rows_as<T, 64, 2, MODE>(a, p, o, s);
+  if (packs <= 128) return launch_rows_as<T, 16, 8, MODE>(a, p, o, s);
   if (packs <= 256) return launch_rows_as<T, 64, 4, MODE>(a, p, o, s);
   if (packs <= 512) return launch_rows_as<T, 64, 8, MODE>(a, p, o, s);
   if (packs <= 1024) return launch_rows_as<T, 256, 4, MODE>(a, p, o, s);
   if (packs <= 2048) return launch_rows_as<T, 256, 8, MODE>(a, p, o, s);
   if (packs <= 4096) return launch_rows_as<T, 1024, 4, MODE>(a, p, o, s);
   if (packs <= 8192) return launch_rows_as<T, 1024, 8, MODE>(a, p, o, s);
+  if constexpr (MODE == TK_POLICY) {
+    if (packs <= 16384) return launch_rows_as<T, 1024, 16, MODE>(a, p, o, s);
+  }
   const int grid = row_grid(a.n, TK_GRID_CAP);
   hipLaunchKernelGGL((k_token_rows_long<T, MODE>), dim3(grid), dim3(1024), 0, s, a, p, o);
   return grid;
