@@ -67,12 +67,12 @@ struct TokenView {
   }
 };
 
-// Sum / maximum over the TPR consecutive lanes of a row group (16 or 64), every lane receives it.
+// Sum / maximum over the TPR consecutive lanes of a row group (8, 16 or 64), every lane receives it.
 template <int TPR> __device__ __forceinline__ float group_sum(float v) {
   v += dpp_move<0xB1>(v);
   v += dpp_move<0x4E>(v);
   v += dpp_move<0x141>(v);
-  v += dpp_move<0x140>(v);
+  if (TPR >= 16) v += dpp_move<0x140>(v);
   if (TPR >= 64) { v = add_xor16(v); v += __shfl_xor(v, 32); }
   return v;
 }
@@ -80,7 +80,7 @@ template <int TPR> __device__ __forceinline__ float group_max(float v) {
   v = fmaxf(v, dpp_move<0xB1>(v));
   v = fmaxf(v, dpp_move<0x4E>(v));
   v = fmaxf(v, dpp_move<0x141>(v));
-  v = fmaxf(v, dpp_move<0x140>(v));
+  if (TPR >= 16) v = fmaxf(v, dpp_move<0x140>(v));
   if (TPR >= 64) { v = fmaxf(v, __shfl_xor(v, 16)); v = fmaxf(v, __shfl_xor(v, 32)); }
   return v;
 }

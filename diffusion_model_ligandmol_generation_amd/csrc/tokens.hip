@@ -150,6 +150,26 @@ __device__ __forceinline__ float row_epilogue(const TokenRows& a, const PolicyIn
   return g;
 }
 
+template <typename T> __device__ __forceinline__ void row_zero(T* d, int V, int r, int tpr) {
+  constexpr int N = Pack<T>::N;
+  const float z[N] = {};
+  const int nb = V / N;
+  for (int i = r; i < nb; i += tpr) store_pack(d + (int64_t)i * N, z);
+  if (r < V - nb * N) d[nb * N + r] = (T)0.f;
+}
+// Writes the rows that a wave has left in LDS as one run of memory.  Rows of a few hundred bytes that end inside cache lines,
+// written by 8 lanes each, would touch every line in two or three pieces.  A wave's LDS operations are in order: no barrier.
+template <typename T> __device__ __forceinline__ void write_flat(const T* stage, T* d, int count) {
+  constexpr int N = Pack<T>::N;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const int lane = threadIdx.x & 63, packs = count / N;
+#pragma unroll 4
+  for (int i = lane; i < packs; i += 64)
+    *reinterpret_cast<typename Pack<T>::Mem*>(d + (int64_t)i * N) = *reinterpret_cast<const u32x4*>(stage + i * N);
+  if (lane < count - packs * N) d[packs * N + lane] = stage[packs * N + lane];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
 // A row that takes no part: nothing of it is read, its log-probability and its gradient are 0.
 template <typename T>
 __device__ __forceinline__ void row_skip(const RowOut& o, int64_t t, int V, int r, int tpr, bool writer) {
@@ -158,14 +178,7 @@ __device__ __forceinline__ void row_skip(const RowOut& o, int64_t t, int V, int 
     if (o.stats) { o.stats[2 * t] = 0.f; o.stats[2 * t + 1] = 0.f; }
     if (o.coef) o.coef[t] = 0.f;
   }
-  if (o.d) {
-    T* d = reinterpret_cast<T*>(o.d) + t * o.d_stride;
-    constexpr int N = Pack<T>::N;
-    const float z[N] = {};
-    const int nb = V / N;
-    for (int i = r; i < nb; i += tpr) store_pack(d + (int64_t)i * N, z);
-    if (r < V - nb * N) d[nb * N + r] = (T)0.f;
-  }
+  if (o.d) row_zero(reinterpret_cast<T*>(o.d) + t * o.d_stride, V, r, tpr);
 }
 
 template <int NT> __device__ __forceinline__ double inverse_total(const PolicyIn& p, double* red) {
@@ -301,18 +314,20 @@ __device__ __forceinline__ void exponentials(u32x4 (&x)[NV], int nb, float m, fl
   }
 }
 // Short rows are loaded one row ahead of their arithmetic: a wave has two rows' bytes under way.
-#define ROW_AHEAD(TPR, REGS, MODE) ((TPR) <= 64 && (REGS) <= 8)
+#define ROW_AHEAD(TPR, REGS, MODE) ((REGS) <= 8)
 // Waves a SIMD holds at once: what the registers of a row allow.
 #define ROW_WAVES(TPR, REGS, MODE) ((MODE) == TK_LOGP ? ((REGS) <= 16 ? 8 : (REGS) <= 32 ? 6 : 4) : (TPR) == 1024 ? ((REGS) <= 16 ? 8 : 4) : (REGS) <= 8 ? 6 : (REGS) <= 16 ? 5 : 4)
 
 // Rows that fit the registers of TPR lanes, NV packs a lane: the logits are read once, exponentiated once, and the policy
-// loss writes its gradient from the same registers.  TPR = 16 / 64: several rows a block and no barrier; 256 / 1024: one
+// loss writes its gradient from the same registers.  TPR = 8 / 16 / 64: several rows a block and no barrier; 256 / 1024: one
 // row a block, whose waves take the maximum and sum of their own part and exchange the pair once.
-template <typename T, int TPR, int NV, int MODE>
+template <typename T, int TPR, int NV, int MODE, bool STAGE = false>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)) void k_token_rows(TokenRows a, PolicyIn p, RowOut o) {
   constexpr int N = Pack<T>::N, NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR, NW = TPR / 64, GRP = TPR < 64 ? TPR : 64;
   constexpr bool KEEP = MODE != TK_LOGP && sizeof(T) == 4;   // the exponentials take the logits' registers
   constexpr bool AHEAD = ROW_AHEAD(TPR, NV * 4, MODE);
+  constexpr int STAGE_ROWS = 64 / (TPR < 64 ? TPR : 64), STAGE_V = TPR * NV * N + N;   // (a multiple of a pack)
+  __shared__ __attribute__((aligned(16))) T stage[STAGE ? NT / 64 * STAGE_ROWS * STAGE_V : 1];
   __shared__ float2 sh[2][NW > 1 ? NW : 1];
   __shared__ double red[NT / 64];
   __shared__ double acc[MODE != TK_LOGP ? RPB : 1][3];
@@ -375,11 +390,14 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
       if constexpr (TPR >= 64) c = RowScalars{uniform(c.id), uniform(c.seq), uniform(c.old), uniform(c.ref)};
       next = scalars(t + step);
     }
-    if (TPR <= 64 && t >= a.n) continue;
+    const auto work = [&]() {
+    if (TPR <= 64 && t >= a.n) return;
     const int id = c.id;
+    T* const staged = stage + (STAGE ? (threadIdx.x >> 6) * STAGE_ROWS * STAGE_V + (threadIdx.x & 63) / TPR * V : 0);
     if (id < 0) {
-      row_skip<T>(o, t, V, r, TPR, r == 0);
-      continue;
+      row_skip<T>(STAGE ? RowOut{o.logp, nullptr, o.stats, o.coef, nullptr, 0} : o, t, V, r, TPR, r == 0);
+      if constexpr (STAGE) row_zero(staged, V, r, TPR);
+      return;
     }
     if constexpr (!AHEAD) load(c, t, x, et, xt, A, len);
     double w = 0.0;
@@ -422,36 +440,47 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
     float g = row_epilogue<MODE>(a, p, o, t, c, xt, M, S, inv_s, r == 0, A, w, acc[MODE != TK_LOGP ? mine : 0]);
     if constexpr (TPR >= 64) g = uniform(g);
     if constexpr (MODE != TK_LOGP) {
-      if (o.d == nullptr) continue;
-      T* d = reinterpret_cast<T*>(o.d) + t * o.d_stride;
-      if (g == 0.f) {   // sends no gradient, also where the row holds a NaN
-        row_skip<T>(RowOut{nullptr, nullptr, nullptr, nullptr, o.d, o.d_stride}, t, V, r, TPR, false);
-        continue;
-      }
-      const float q = -g * f * inv_s;
-      const int it = id / N;
-      const auto out = [&](int k, float (&e)[N]) {
-        const int i = r + k * TPR;
-#pragma unroll
-        for (int j = 0; j < N; ++j) e[j] *= q;
-        if (i == it) {
-#pragma unroll
-          for (int j = 0; j < N; ++j) e[j] += j == id - it * N ? g : 0.f;
+      if (!STAGE && o.d == nullptr) return;
+      const auto write = [&](T* d) {
+        if (g == 0.f) {   // sends no gradient, also where the row holds a NaN
+          row_zero(d, V, r, TPR);
+          return;
         }
-        if (i < nb) store_pack(d + (int64_t)i * N, e);
+        const float q = -g * f * inv_s;
+        const int it = id / N;
+        const auto out = [&](int k, float (&e)[N]) {
+          const int i = r + k * TPR;
+#pragma unroll
+          for (int j = 0; j < N; ++j) e[j] *= q;
+          if (i == it) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) e[j] += j == id - it * N ? g : 0.f;
+          }
+          if (i < nb) store_pack(d + (int64_t)i * N, e);
+        };
+        if constexpr (KEEP) {
+#pragma unroll
+          for (int k = 0; k < NV; ++k) {
+            float e[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) e[j] = raw_get<T>(x[k], j);
+            out(k, e);
+          }
+        } else {
+          exponentials<T, NV, TPR>(x, nb, m, mc, a.c, far, out);
+        }
+        if (r < tail) d[nb * N + r] = (T)(q * et + (nb * N + r == id ? g : 0.f));
       };
-      if constexpr (KEEP) {
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          float e[N];
-#pragma unroll
-          for (int j = 0; j < N; ++j) e[j] = raw_get<T>(x[k], j);
-          out(k, e);
-        }
-      } else {
-        exponentials<T, NV, TPR>(x, nb, m, mc, a.c, far, out);
-      }
-      if (r < tail) d[nb * N + r] = (T)(q * et + (nb * N + r == id ? g : 0.f));
+      if constexpr (STAGE) write(staged);
+      else write(reinterpret_cast<T*>(o.d) + t * o.d_stride);
+    }
+    };
+    work();
+    if constexpr (STAGE) {
+      const int64_t t0 = base + (int64_t)(threadIdx.x >> 6) * STAGE_ROWS;
+      if (t0 < a.n)
+        write_flat(stage + (threadIdx.x >> 6) * STAGE_ROWS * STAGE_V, reinterpret_cast<T*>(o.d) + t0 * V,
+                   (int)(a.n - t0 < STAGE_ROWS ? a.n - t0 : STAGE_ROWS) * V);
     }
   }
   if constexpr (MODE == TK_POLICY) policy_partial<RPB>(p, acc);
@@ -565,7 +594,8 @@ __global__ __launch_bounds__(1024) void k_token_rows_long(TokenRows a, PolicyIn 
 // The loss of a preference step, added up by the last block of its gradient launch.
 struct LossTail { const double* partial; int blocks; double denom; float* loss; };
 __device__ __forceinline__ void preference_final(const LossTail& f);
-template <typename T, int TPR>
+// FLAT: 0, or the packs of the longest row that is written through LDS (and a part of one more).
+template <typename T, int TPR, int FLAT>
 __global__ __launch_bounds__(256) void k_token_grad(TokenRows a, LossTail f, const float* __restrict__ stats, const float* __restrict__ coef,
                                                     const int32_t* __restrict__ index, int64_t n_coef, float mult, const float* __restrict__ upstream, T* __restrict__ d, int64_t d_stride) {
   constexpr int RPB = 256 / TPR;
@@ -573,14 +603,24 @@ __global__ __launch_bounds__(256) void k_token_grad(TokenRows a, LossTail f, con
   const double k = (double)mult * a.inv_t * (upstream ? (double)*upstream : 1.0);
   const int blocks = gridDim.x - (f.loss != nullptr);
   if ((int)blockIdx.x == blocks) { preference_final(f); return; }
-  // (the last rows first: they are the last that the forward launch read)
-  for (int64_t i = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; i < a.n; i += (int64_t)blocks * RPB) {
-    const int64_t t = a.n - 1 - i;
-    const int id = a.tok.at(t);
-    const int64_t ci = index ? (int64_t)index[t] : t;
-    const float g = id < 0 || ci < 0 || ci >= n_coef ? 0.f : (float)((double)coef[ci] * k);
-    row_gradient<T, TPR>(a, reinterpret_cast<const T*>(a.x) + t * a.stride, d + t * d_stride, id, r, stats[2 * t],
-                         g == 0.f ? 0.f : stats[2 * t + 1], g);
+  constexpr int ROWS = TPR < 64 ? 64 / TPR : 1;
+  constexpr int FLAT_V = (FLAT + 1) * Pack<T>::N;
+  __shared__ __attribute__((aligned(16))) T stage[FLAT ? 4 * ROWS * FLAT_V : 1];
+  T* const mine = stage + (FLAT ? (threadIdx.x >> 6) * ROWS * FLAT_V : 0);
+  for (int64_t base = (int64_t)blockIdx.x * RPB; base < a.n; base += (int64_t)blocks * RPB) {
+    const int64_t t = base + threadIdx.x / TPR;
+    if (t < a.n) {
+      const int id = a.tok.at(t);
+      const int64_t ci = index ? (int64_t)index[t] : t;
+      const float g = id < 0 || ci < 0 || ci >= n_coef ? 0.f : (float)((double)coef[ci] * k);
+      const T* row = reinterpret_cast<const T*>(a.x) + t * a.stride;
+      if constexpr (FLAT) row_gradient<T, TPR>(a, row, mine + (threadIdx.x & 63) / TPR * a.V, id, r, stats[2 * t], stats[2 * t + 1], g);
+      else row_gradient<T, TPR>(a, row, d + t * d_stride, id, r, stats[2 * t], stats[2 * t + 1], g);
+    }
+    if constexpr (FLAT) {
+      const int64_t t0 = base + (int64_t)(threadIdx.x >> 6) * ROWS;
+      if (t0 < a.n) write_flat(mine, d + t0 * a.V, (int)(a.n - t0 < ROWS ? a.n - t0 : ROWS) * a.V);
+    }
   }
 }
 
@@ -832,19 +872,22 @@ __global__ void k_empty_policy(float* result) { if (threadIdx.x < 4) result[thre
 static int row_grid(int64_t groups, int most) { return (int)(groups < most ? groups : most); }
 
 #define TK_GRID_CAP 2048
-template <typename T, int TPR, int NV, int MODE>
+// Rows next to each other that end inside cache lines.
+static bool ragged_lines(int32_t V, int64_t d_stride, size_t size) { return d_stride == V && (V * size) % 128 != 0; }
+template <typename T, int TPR, int NV, int MODE, bool STAGE = false>
 static int launch_rows_as(const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
   constexpr int NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR;
   const int grid = row_grid((a.n + RPB - 1) / RPB, TK_GRID_CAP * 256 / NT);
-  hipLaunchKernelGGL((k_token_rows<T, TPR, NV, MODE>), dim3(grid), dim3(NT), 0, s, a, p, o);
+  hipLaunchKernelGGL((k_token_rows<T, TPR, NV, MODE, STAGE>), dim3(grid), dim3(NT), 0, s, a, p, o);
   return grid;
 }
-// A batch of at most SMALL_ROWS short rows is one launch of one block: three launches take longer than its four rounds.
-static bool rows_of_16_lanes(int dtype, int32_t V) { return V / (dtype == LIGDIFF_F32 ? 4 : 8) <= 64; }
-// The fewest lanes whose registers hold a row, and the fewest packs a lane: 16 lanes up to 128 packs, a wave up to 512, 256 lanes
-// up to 2048, 1024 up to 8192 (32768 fp32 or 65536 half-precision logits).  More lanes than that wait for each other more
-// often and hold fewer rows under way.  Measured on 268 MB of fp32 logits, log-probabilities / policy loss with gradient, us:
-// 128 packs 16 lanes 41/110, 64 lanes 49/125, 256 lanes 168/345; 512 packs 64 lanes 41/112, 256 lanes 52/127; 2048 packs
+// A batch of at most SMALL_ROWS short rows is one launch of one block: three launches take longer than its two rounds.
+static bool rows_of_8_lanes(int dtype, int32_t V) { return V / (dtype == LIGDIFF_F32 ? 4 : 8) <= 64; }
+// The fewest lanes whose registers hold a row, and the fewest packs a lane: 8 lanes up to 64 packs, 16 up to 128, a wave up to 512,
+// 256 lanes up to 2048, 1024 up to 8192 (32768 fp32 or 65536 half-precision logits).  More lanes than that wait for each
+// other more often, hold fewer rows under way and do the work per row (64-bit log, ratio, KL term) for fewer rows at a time.
+// Measured on 268 MB of fp32 logits, log-probabilities / policy loss with gradient, us: 32 packs 8 lanes 43/113, 16 lanes 48/124,
+// 64 lanes 154/292; 64 packs 8 lanes 40/111, 16 lanes 42/112; 128 packs 16 lanes 41/110, 64 lanes 49/125, 256 lanes 168/345; 512 packs 64 lanes 41/112, 256 lanes 52/127; 2048 packs
 // 256 lanes 42/111, 1024 lanes 53/113; 8192 packs 1024 lanes 44/114, reading twice 45/167.  So beyond 8192 packs the
 // log-probabilities stream the row (one read in either form: 12000 packs 45 against 47) and the policy loss keeps it up to
 // 16384 packs (134 against 171).  Returns the number of blocks.
@@ -852,14 +895,22 @@ template <typename T, int MODE>
 static int launch_rows(const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
   const int packs = a.V / Pack<T>::N;
   if (MODE == TK_POLICY && a.n <= SMALL_ROWS && packs <= 64) {
-    if (packs <= 16) hipLaunchKernelGGL((k_token_rows<T, 16, 1, TK_SMALL>), dim3(1), dim3(256), 0, s, a, p, o);
-    else if (packs <= 32) hipLaunchKernelGGL((k_token_rows<T, 16, 2, TK_SMALL>), dim3(1), dim3(256), 0, s, a, p, o);
-    else hipLaunchKernelGGL((k_token_rows<T, 16, 4, TK_SMALL>), dim3(1), dim3(256), 0, s, a, p, o);
+    if (packs <= 16) hipLaunchKernelGGL((k_token_rows<T, 8, 2, TK_SMALL>), dim3(1), dim3(256), 0, s, a, p, o);
+    else if (packs <= 32) hipLaunchKernelGGL((k_token_rows<T, 8, 4, TK_SMALL>), dim3(1), dim3(256), 0, s, a, p, o);
+    else hipLaunchKernelGGL((k_token_rows<T, 8, 8, TK_SMALL>), dim3(1), dim3(256), 0, s, a, p, o);
     return 1;
   }
-  if (packs <= 16) return launch_rows_as<T, 16, 1, MODE>(a, p, o, s);
-  if (packs <= 32) return launch_rows_as<T, 16, 2, MODE>(a, p, o, s);
-  if (packs <= 64) return launch_rows_as<T, 16, 4, MODE>(a, p, o, s);
+  if constexpr (MODE == TK_POLICY) {
+    // (through LDS: 119 fp32 a row 69 us against 86 for 147 MB, 200 fp32 61 against 72, 500 bf16 70 against 76; but 30 fp32 57
+    // against 52 and 90 bf16 78 against 74: rows of two lines at most are as well written directly)
+    if (packs <= 64 && (size_t)a.V * sizeof(T) > 256 && o.d && ragged_lines(a.V, o.d_stride, sizeof(T))) {
+      if (packs <= 32) return launch_rows_as<T, 8, 4, MODE, true>(a, p, o, s);
+      return launch_rows_as<T, 8, 8, MODE, true>(a, p, o, s);
+    }
+  }
+  if (packs <= 16) return launch_rows_as<T, 8, 2, MODE>(a, p, o, s);
+  if (packs <= 32) return launch_rows_as<T, 8, 4, MODE>(a, p, o, s);
+  if (packs <= 64) return launch_rows_as<T, 8, 8, MODE>(a, p, o, s);
   if (packs <= 128) return launch_rows_as<T, 16, 8, MODE>(a, p, o, s);
   if (packs <= 256) return launch_rows_as<T, 64, 4, MODE>(a, p, o, s);
   if (packs <= 512) return launch_rows_as<T, 64, 8, MODE>(a, p, o, s);
@@ -881,16 +932,23 @@ template <int MODE> static int launch_rows_dtype(int dtype, const TokenRows& a, 
   return launch_rows<f16_t, MODE>(a, p, o, s);
 }
 struct GradIn { const float* stats; const float* coef; const int32_t* index; int64_t n_coef; float mult; const float* up; void* d; int64_t d_stride; };
-template <typename T, int TPR> static void launch_grad_as(const TokenRows& a, const GradIn& g, const LossTail& f, hipStream_t s) {
+template <typename T, int TPR, int FLAT> static void launch_grad_as(const TokenRows& a, const GradIn& g, const LossTail& f, hipStream_t s) {
   constexpr int RPB = 256 / TPR;
   const int grid = row_grid((a.n + RPB - 1) / RPB, 8192) + (f.loss != nullptr);
-  hipLaunchKernelGGL((k_token_grad<T, TPR>), dim3(grid), dim3(256), 0, s, a, f, g.stats, g.coef, g.index, g.n_coef, g.mult, g.up, (T*)g.d, g.d_stride);
+  hipLaunchKernelGGL((k_token_grad<T, TPR, FLAT>), dim3(grid), dim3(256), 0, s, a, f, g.stats, g.coef, g.index, g.n_coef, g.mult, g.up, (T*)g.d, g.d_stride);
 }
 template <typename T> static void launch_grad(const TokenRows& a, const GradIn& g, const LossTail& f, hipStream_t s) {
   const int packs = a.V / Pack<T>::N;
-  if (packs <= 64) launch_grad_as<T, 16>(a, g, f, s);
-  else if (packs <= 512) launch_grad_as<T, 64>(a, g, f, s);
-  else launch_grad_as<T, 256>(a, g, f, s);
+  // Rows that fill cache lines: 8 lanes a row (512 bytes 50 us against 61 with 16 lanes, 147 MB), 16 from 32 packs on (1024 bytes
+  // 52 against 50).  Ragged rows: 8 lanes up to 192 bytes (45 fp32 39 us, 42 through LDS, 50 with 16 lanes), longer ones
+  // through LDS (119 fp32 72 us, 97 with 8 and 76 with 16 lanes; 250 fp32 70, 96, 79; 119 bf16 72, 81, 86).
+  const bool ragged = ragged_lines(a.V, g.d_stride, sizeof(T)), flat = ragged && (size_t)a.V * sizeof(T) > 192;
+  if (flat && packs <= 32) launch_grad_as<T, 8, 32>(a, g, f, s);
+  else if (flat && packs <= 64) launch_grad_as<T, 8, 64>(a, g, f, s);
+  else if (packs <= 32) launch_grad_as<T, 8, 0>(a, g, f, s);
+  else if (packs <= 64) launch_grad_as<T, 16, 0>(a, g, f, s);
+  else if (packs <= 512) launch_grad_as<T, 64, 0>(a, g, f, s);
+  else launch_grad_as<T, 256, 0>(a, g, f, s);
 }
 // (the caller has seen to it that there are rows)
 static void launch_grad_dtype(int dtype, const TokenRows& a, const GradIn& g, const LossTail& f, hipStream_t s) {
@@ -1042,7 +1100,7 @@ extern "C" int ligdiff_policy_loss(const ligdiff_token_args* args, const ligdiff
     return LIGDIFF_OK;
   }
   const int chunks = (int)seg_chunks(a.n);
-  const bool small = a.n <= SMALL_ROWS && rows_of_16_lanes(args->dtype, a.V);
+  const bool small = a.n <= SMALL_ROWS && rows_of_8_lanes(args->dtype, a.V);
   if (!small)
     hipLaunchKernelGGL((k_row_segments<false>), dim3(chunks), dim3(256), 0, s,
                        SegRows{a.tok, a.n, q->seq_ptr, q->n_seq, nullptr, w.seq_of, nullptr, per_seq ? w.part_len : nullptr, w.chunk_len});
