@@ -610,7 +610,7 @@ extern "C" int ligdiff_backward_train(const float* const* w, float* const* gr, c
       embed_grad(eg, T(L.sort), s);
       ln_bwd<0, 1>(A(F.type_pre), 256, w[W_ATOM_G], w[W_ATOM_BE], 1e-5f, dt, 256, nullptr, 0, nullptr, du, 256, gr[W_ATOM_G],
                    gr[W_ATOM_BE], LD_A + 1, s);
-      hipLaunchKernelGGL(k_type_embed_dw, dim3(LD_A + 1), dim3(256), 0, s, du, gr[W_ATOM_W], gr[W_ATOM_B]);
+      type_embed_dw(du, gr[W_ATOM_W], gr[W_ATOM_B], s);
     } else {
       float* du = fresh((int64_t)N * 256);
       ln_bwd<0, 1>(A(F.ua), 256, w[W_ATOM_G], w[W_ATOM_BE], 1e-5f, dxa, 256, nullptr, 0, nullptr, du, 256, gr[W_ATOM_G],

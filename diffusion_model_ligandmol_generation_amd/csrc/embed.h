@@ -13,3 +13,8 @@ struct EmbedGrad {
 };
 size_t embed_grad_workspace(int64_t n, int32_t rows, int32_t width);
 void embed_grad(const EmbedGrad& g, void* workspace, hipStream_t s);   // sizes checked by the caller
+
+// The atom branch of the score network's input embedding for integer atom types: a table of LD_A + 1 rows, before LayerNorm and
+// after GELU, and the weight gradients from those of the rows before LayerNorm.
+void type_embed(const float* Wa, const float* ba, const float* ga, const float* bea, float* pre, float* emb, hipStream_t s);
+void type_embed_dw(const float* du, float* dWa, float* dba, hipStream_t s);

@@ -622,3 +622,51 @@ extern "C" int ligdiff_embed_grad(const void* d_out, int32_t dtype, int64_t d_st
   LD_CHECK_LAUNCH();
   return LIGDIFF_OK;
 }
+
+// ------------------------------------------------------------------ atom types of the score network
+// Atom branch of the input embedding per TYPE (model1.py:599-609 on one-hot rows): u = Wa[:, v] + ba, GELU(LN(u)); row LD_A
+// is that of a zero feature row.  One wave a type; the atoms then look their row up (k_pos_embed), 120 rows of
+// arithmetic instead of one per atom and no [N,119] features to read.
+__global__ __launch_bounds__(256) void k_type_embed(const float* __restrict__ Wa, const float* __restrict__ ba,
+                                                    const float* __restrict__ ga, const float* __restrict__ bea,
+                                                    float* __restrict__ pre, float* __restrict__ emb) {
+  const int lane = threadIdx.x & 63;
+  const int v = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (v > LD_A) return;
+  f32x4 u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int col = lane * 4 + i;
+    u[i] = ba[col] + (v < LD_A ? Wa[(size_t)col * LD_A + v] : 0.f);
+  }
+  const float mean = wave_sum((u[0] + u[1]) + (u[2] + u[3])) * (1.0f / 256.0f);
+  const f32x4 d = u - mean;
+  const float var = wave_sum((d[0] * d[0] + d[1] * d[1]) + (d[2] * d[2] + d[3] * d[3])) * (1.0f / 256.0f);
+  const float rstd = 1.0f / sqrtf(var + 1e-5f);
+  f32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = gelu_exact(d[i] * rstd * ga[lane * 4 + i] + bea[lane * 4 + i]);
+  *reinterpret_cast<f32x4*>(pre + (size_t)v * 256 + lane * 4) = u;
+  *reinterpret_cast<f32x4*>(emb + (size_t)v * 256 + lane * 4) = o;
+}
+
+// Gradient of the per-type atom branch: du [LD_A + 1, 256] before LayerNorm -> Wa[:, v] += du[v], ba += sum_v du[v].  Block v
+// writes column v of Wa; block LD_A the bias (a column a thread, in the order of the types).
+__global__ __launch_bounds__(256) void k_type_embed_dw(const float* __restrict__ du, float* __restrict__ dWa, float* __restrict__ dba) {
+  const int c = threadIdx.x, v = blockIdx.x;
+  if (v < LD_A) {
+    dWa[(size_t)c * LD_A + v] += du[(size_t)v * 256 + c];
+    return;
+  }
+  float sum = 0.f;
+#pragma unroll 8
+  for (int k = 0; k <= LD_A; ++k) sum += du[(size_t)k * 256 + c];
+  dba[c] += sum;
+}
+
+void type_embed(const float* Wa, const float* ba, const float* ga, const float* bea, float* pre, float* emb, hipStream_t s) {
+  hipLaunchKernelGGL(k_type_embed, dim3(ceil_div(LD_A + 1, 4)), dim3(256), 0, s, Wa, ba, ga, bea, pre, emb);
+}
+void type_embed_dw(const float* du, float* dWa, float* dba, hipStream_t s) {
+  hipLaunchKernelGGL(k_type_embed_dw, dim3(LD_A + 1), dim3(256), 0, s, du, dWa, dba);
+}

@@ -7,6 +7,7 @@
 #include "epilogues.h"
 #include "gemm3.h"
 #include "chain_args.h"
+#include "embed.h"
 #include "forward.h"
 #include "kernels.h"
 #include "weights.h"
@@ -490,8 +491,7 @@ int run_forward(const float* const* w, const ligdiff_graph* g, const float* x, c
     e.atom_mol = g->atom_mol; e.H = F(L.h0); e.ua_out = S(L.ua);
     PB("embed");
     if (flags & LIGDIFF_FWD_ATOM_TYPES) {
-      hipLaunchKernelGGL(k_type_embed, dim3(ceil_div(LD_A + 1, 4)), dim3(256), 0, s, w[W_ATOM_W], w[W_ATOM_B], w[W_ATOM_G],
-                         w[W_ATOM_BE], F(L.type_pre), F(L.type_emb));
+      type_embed(w[W_ATOM_W], w[W_ATOM_B], w[W_ATOM_G], w[W_ATOM_BE], F(L.type_pre), F(L.type_emb), s);
       hipLaunchKernelGGL(k_pos_embed, dim3(ceil_div(N, 4)), dim3(256), 0, s, pos, w[W_POS_W], w[W_POS_B], w[W_POS_G],
                          w[W_POS_BE], F(L.temb), tstride, pemb, pstride, g->atom_mol, F(L.h0), N, pemb_mols, nullptr, nullptr,
                          nullptr, nullptr, reinterpret_cast<const int32_t*>(x), F(L.type_emb));

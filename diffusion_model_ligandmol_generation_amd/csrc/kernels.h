@@ -157,32 +157,6 @@ __global__ __launch_bounds__(256) void k_pos_embed(const float* __restrict__ pos
   *reinterpret_cast<f32x4*>(R + (size_t)row * 256 + lane * 4) = o;
 }
 
-// Atom branch of the input embedding per TYPE (model1.py:599-609 on one-hot rows): u = Wa[:, v] + ba, GELU(LN(u)); row LD_A
-// is that of a zero feature row.  One wave a type; the atoms then look their row up (k_pos_embed), 120 rows of
-// arithmetic instead of one per atom and no [N,119] features to read.
-__global__ __launch_bounds__(256) void k_type_embed(const float* __restrict__ Wa, const float* __restrict__ ba,
-                                                    const float* __restrict__ ga, const float* __restrict__ bea,
-                                                    float* __restrict__ pre, float* __restrict__ emb) {
-  const int lane = threadIdx.x & 63;
-  const int v = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (v > LD_A) return;
-  f32x4 u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int col = lane * 4 + i;
-    u[i] = ba[col] + (v < LD_A ? Wa[(size_t)col * LD_A + v] : 0.f);
-  }
-  const float mean = wave_sum((u[0] + u[1]) + (u[2] + u[3])) * (1.0f / 256.0f);
-  const f32x4 d = u - mean;
-  const float var = wave_sum((d[0] * d[0] + d[1] * d[1]) + (d[2] * d[2] + d[3] * d[3])) * (1.0f / 256.0f);
-  const float rstd = 1.0f / sqrtf(var + 1e-5f);
-  f32x4 o;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = gelu_exact(d[i] * rstd * ga[lane * 4 + i] + bea[lane * 4 + i]);
-  *reinterpret_cast<f32x4*>(pre + (size_t)v * 256 + lane * 4) = u;
-  *reinterpret_cast<f32x4*>(emb + (size_t)v * 256 + lane * 4) = o;
-}
-
 // Message aggregation + coordinate scatter, model1.py:100 / :110-112 / :724-725.
 // One wave per destination atom.  The atom's incoming messages are CONTIGUOUS rows of
 // msg (CSR order), so the sum streams 1-KiB rows, 16 B per lane, in the fixed edge order

@@ -679,20 +679,6 @@ __global__ __launch_bounds__(256) void k_pool_bwd(const float* __restrict__ dpoo
   *p += *reinterpret_cast<const f32x4*>(dpooled + (size_t)m * 256 + lane * 4) * inv;
 }
 
-// Gradient of the per-type atom branch: du [LD_A + 1, 256] before LayerNorm -> Wa[:, v] += du[v], ba += sum_v du[v].  Block v
-// writes column v of Wa; block LD_A the bias (a column a thread, in the order of the types).
-__global__ __launch_bounds__(256) void k_type_embed_dw(const float* __restrict__ du, float* __restrict__ dWa, float* __restrict__ dba) {
-  const int c = threadIdx.x, v = blockIdx.x;
-  if (v < LD_A) {
-    dWa[(size_t)c * LD_A + v] += du[(size_t)v * 256 + c];
-    return;
-  }
-  float sum = 0.f;
-#pragma unroll 8
-  for (int k = 0; k <= LD_A; ++k) sum += du[(size_t)k * 256 + c];
-  dba[c] += sum;
-}
-
 // u_p[n, c] = pos[n] . Wp[c] + bp[c]   (recomputed pre-LayerNorm value of the position embedding)
 __global__ __launch_bounds__(256) void k_pos_embed_pre(const float* __restrict__ pos, const float* __restrict__ Wp,
                                                        const float* __restrict__ bp, float* __restrict__ up, int N) {
