@@ -19,9 +19,10 @@ struct TokenRows {
 
 // exp((x - m) / temperature) of a row with maximum m is exp2(c x - mc), mc = c m: one fused multiply-add, rounded once, also
 // for logits far from 0.  mc is a rounded number, but the same one in every element and in logp, where it cancels exactly;
-// so does c, whose rounding only means a temperature that is off by 2^-25.  A maximum near the end of the fp32 range (rows
-// masked with the type's lowest value) would overflow mc: such a row is shifted by m first, and its mc is 0.
-__device__ __forceinline__ bool far_out(float m) { return !(fabsf(m) < 1e38f); }
+// so does c, whose rounding only means a temperature that is off by 2^-25.  The largest exponent is mc's rounding error, at
+// most |mc| 2^-24: below 1 as long as |mc| < 2^24.  Rows further out (masked with -1e10 or the type's lowest value, very low
+// temperatures), where that error could overflow the exponential or lose it, are shifted by m first, and their mc is 0.
+__device__ __forceinline__ bool far_out(float m, float c) { return !(fabsf(m) * c < 16777216.f); }
 __device__ __forceinline__ float shifted(float x, float m) { return x == m ? 0.f : x - m; }   // (+inf - +inf is not asked for)
 
 
@@ -119,7 +120,7 @@ template <int MODE>
 __device__ __forceinline__ float row_epilogue(const TokenRows& a, const PolicyIn& p, const RowOut& o, int64_t t, const RowScalars& c,
                                               float xt, float M, float S, float inv_s, bool writer, float A, double w, double* acc) {
   // a row of -inf only has no distribution: S = 0, logp = -inf, no gradient
-  const double z = far_out(M) ? ((double)xt - (double)M) * a.c : fma((double)xt, (double)a.c, -(double)(M * a.c));
+  const double z = far_out(M, a.c) ? ((double)xt - (double)M) * a.c : fma((double)xt, (double)a.c, -(double)(M * a.c));
   const double lp = S == 0.f ? -__builtin_inf() : fma(z, 0.69314718055994530942, -log_of_sum(S));
   float g = 0.f, coef = 0.f;
   if constexpr (MODE != TK_LOGP) {
@@ -266,7 +267,11 @@ __device__ __forceinline__ float part_factor(float m, float M, float c) {
 #pragma clang fp contract(off)   // both products are the rounded numbers that the exponentials used
   if (m == -__builtin_inff()) return 0.f;
   const float mc = m * c, Mc = M * c;
-  return __builtin_amdgcn_exp2f(far_out(m) || far_out(M) ? shifted(m, M) * c : mc - Mc);
+  if (__builtin_expect(far_out(m, c) || far_out(M, c), 0)) {   // one of them may be shifted: exact products (48 bits) for it
+    const double dm = far_out(m, c) ? (double)m * c : (double)mc, dM = far_out(M, c) ? (double)M * c : (double)Mc;
+    return m == M ? 1.f : __builtin_amdgcn_exp2f((float)(dm - dM));
+  }
+  return __builtin_amdgcn_exp2f(mc - Mc);
 }
 // The maximum and sum of a row from those of its 4 or 16 waves (0 and 0 for a row of -inf only).
 template <int NW> __device__ __forceinline__ void join_waves(const float2* sh, float c, float& M, float& S) {
@@ -411,7 +416,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
     }
     m = group_max<GRP>(m);
     // this wave's own part: e = exp2(c x - mc)
-    const bool none = m == -__builtin_inff(), far = !none && far_out(m);
+    const bool none = m == -__builtin_inff(), far = !none && far_out(m, a.c);
     const float mc = none || far ? 0.f : m * a.c;
     float s;
     if (__builtin_expect(far, 0)) s = et = __builtin_amdgcn_exp2f(shifted(et, m) * a.c);
@@ -493,7 +498,7 @@ template <typename T, int TPR>
 __device__ __forceinline__ void row_gradient(const TokenRows& a, const T* row, T* d, int id, int r, float M, float inv_s, float g) {
   constexpr int N = Pack<T>::N;
   const int V = a.V, nb = V / N, tail = V - nb * N;
-  const bool off = g == 0.f || inv_s == 0.f, far = far_out(M);
+  const bool off = g == 0.f || inv_s == 0.f, far = far_out(M, a.c);
   const float mc = far ? 0.f : M * a.c, q = -g * inv_s;
   const int it = id / N;
   if (off) {
@@ -568,7 +573,7 @@ __global__ __launch_bounds__(1024) void k_token_rows_long(TokenRows a, PolicyIn 
         s *= part_factor(m, mx, a.c);
         m = mx;
       }
-      const bool none = m == -__builtin_inff(), far = !none && far_out(m);
+      const bool none = m == -__builtin_inff(), far = !none && far_out(m, a.c);
       const float mc = none || far ? 0.f : m * a.c;
 #pragma unroll
       for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f(fmaf(far ? shifted(v[j], m) : v[j], a.c, -mc));
@@ -625,10 +630,11 @@ __global__ __launch_bounds__(256) void k_token_grad(TokenRows a, LossTail f, con
 }
 
 // Rows in chunks of SEG_ROWS, one block a chunk: the sequence of each row (-1 for ignored rows and rows outside every
-// sequence), the chunk's number of taking rows, and for every
-// sequence that meets the chunk the sum and the number of its rows in it, from prefix sums in 64 bits.  What sequence s has
-// in chunk c goes to place c + s: both grow along the rows, so no two parts share a place.  A sequence of any length is
-// then the sum of its parts, and no block waits for one long sequence.
+// sequence), the chunk's number of taking rows, and for every sequence that meets the chunk the sum and the number of its
+// rows in it.  The sums are running ones in 64 bits that start anew with every sequence: differences of one running sum over
+// the whole chunk would carry an infinity or NaN of one sequence into those behind it.  What sequence s has in chunk c goes to
+// place c + s: both grow along the rows, so no two parts share a place.  A sequence of any length is then the sum of its
+// parts, and no block waits for one long sequence.
 #define SEG_ROWS 1024
 // The number of seq_ptr[0 .. n) that are <= t, by a whole wave: 64 probes a step.  (In 32 bits: n <= 2^31, a probe lies
 // below 2^31 + 2^25.  The compiler's scalar code for the 64-bit form selects by a stale condition bit.)
@@ -654,15 +660,14 @@ struct SegRows {
   int32_t* chunk_len;         // [chunks] or null
 };
 template <bool SUM> struct SegShared {
-  double pre[SUM ? SEG_ROWS + 1 : 1], wsum[4];
-  int cnt[SEG_ROWS + 1], wcnt[4], wmax[4], ends[2];
+  double run[SUM ? SEG_ROWS : 1], wsum[4];    // a row's sequence up to it, within the chunk
+  int cnt[SEG_ROWS + 1], wcnt[4], wmax[4], wkey[4], ends[2];
 };
 template <bool SUM> __device__ __forceinline__ void row_segments(const SegRows& g, int64_t c, SegShared<SUM>& sh) {
   const TokenView& tok = g.tok;
   const int64_t n = g.n;
   const int32_t* __restrict__ seq_ptr = g.seq_ptr;
   const int32_t S = g.S;
-  double* const pre = sh.pre;
   int* const cnt = sh.cnt;
   int* const mark = cnt;   // (the counts replace the marks once every thread has read its own)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -710,33 +715,49 @@ template <bool SUM> __device__ __forceinline__ void row_segments(const SegRows& 
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     m[j] = before > m[j] ? before : m[j];
-    if (!on[j] || m[j] >= S) m[j] = -1;
-    k[j] = m[j] >= 0;
+    k[j] = on[j] && m[j] >= 0 && m[j] < S;
     v[j] = SUM && k[j] ? (double)d[j] : 0.0;
     const int i = tid * 4 + j;
-    if (i < rows) g.seq_of[c0 + i] = m[j];
+    if (i < rows) g.seq_of[c0 + i] = k[j] ? m[j] : -1;
+  }
+  // running sums that start anew with a sequence: the sequences never fall along the rows, so two places are of one run
+  // exactly if they are of one sequence
+  if (SUM) {
+#pragma unroll
+    for (int j = 1; j < 4; ++j)
+      if (m[j] == m[j - 1]) v[j] += v[j - 1];
   }
   int ci = (k[0] + k[1]) + (k[2] + k[3]);
-  double vi = (v[0] + v[1]) + (v[2] + v[3]);
-  const int own_c = ci;
-  const double own_v = vi;
+  const int own_c = ci, key = m[3];
+  double vi = v[3];
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int cu = __shfl_up(ci, o);
+    const int cu = __shfl_up(ci, o), ku = SUM ? __shfl_up(key, o) : 0;
     const double vu = SUM ? __shfl_up(vi, o) : 0.0;
-    if (lane >= o) { ci += cu; vi += vu; }
+    if (lane >= o) {
+      ci += cu;
+      if (SUM && ku == key) vi += vu;
+    }
   }
-  if (lane == 63) { sh.wcnt[wave] = ci; sh.wsum[wave] = vi; }
+  const int key_below = SUM ? __shfl_up(key, 1) : 0, first = SUM ? __shfl(m[0], 0) : 0;
+  double add = SUM ? __shfl_up(vi, 1) : 0.0;    // what came before the lane's first row, in this wave
+  if (lane == 0 || key_below != m[0]) add = 0.0;
+  if (lane == 63) {
+    sh.wcnt[wave] = ci;
+    if (SUM) { sh.wsum[wave] = vi; sh.wkey[wave] = key; }
+  }
   __syncthreads();
   int cb = ci - own_c;
-  double vb = vi - own_v;
-  for (int w = 0; w < wave; ++w) { cb += sh.wcnt[w]; vb += sh.wsum[w]; }
-  if (tid == 0) { cnt[0] = 0; if (SUM) pre[0] = 0.0; }
+  for (int w = 0; w < wave; ++w) {
+    cb += sh.wcnt[w];
+    if (SUM && m[0] == first && sh.wkey[w] == first) add += sh.wsum[w];
+  }
+  if (tid == 0) cnt[0] = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    cb += k[j]; vb += v[j];
+    cb += k[j];
     cnt[tid * 4 + j + 1] = cb;
-    if (SUM) pre[tid * 4 + j + 1] = vb;
+    if (SUM) sh.run[tid * 4 + j] = m[j] == m[0] ? v[j] + add : v[j];
   }
   __syncthreads();
   if (tid == 0 && g.chunk_len) g.chunk_len[c] = cnt[rows];
@@ -747,7 +768,7 @@ template <bool SUM> __device__ __forceinline__ void row_segments(const SegRows& 
     const int b = t1 <= c0 ? 0 : t1 - c0 < rows ? (int)(t1 - c0) : rows;
     if (b > a) {
       g.part_len[c + s] = cnt[b] - cnt[a];
-      if (SUM) g.part_sum[c + s] = pre[b] - pre[a];
+      if (SUM) g.part_sum[c + s] = sh.run[b - 1];
     }
   }
 }
@@ -960,7 +981,7 @@ static void launch_grad_dtype(int dtype, const TokenRows& a, const GradIn& g, co
 static int fill_rows(TokenRows* r, const ligdiff_token_args* a) {
   if (!a || a->n_tokens < 0 || a->n_tokens > 0x7fffffffLL || a->vocab < 1 || a->row_stride < a->vocab ||
       a->dtype < LIGDIFF_F32 || a->dtype > LIGDIFF_F16 || (a->token_bytes != 4 && a->token_bytes != 8) ||
-      !(a->temperature > 0.f) || !(a->temperature <= 3.0e38f))
+      !(a->temperature >= 1e-20f) || !(a->temperature <= 1e20f))
     return LIGDIFF_ERR_ARG;
   if (a->n_tokens > 0 && (!a->logits || !a->tokens)) return LIGDIFF_ERR_ARG;
   r->x = a->logits; r->stride = a->row_stride; r->n = a->n_tokens; r->V = a->vocab;

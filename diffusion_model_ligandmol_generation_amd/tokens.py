@@ -203,8 +203,8 @@ def _token_args(logits, tokens, temperature):
     if tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
     temperature = float(temperature)
-    if not 0.0 < temperature <= 3e38:
-        raise ValueError("temperature must be positive")
+    if not 1e-20 <= temperature <= 1e20:
+        raise ValueError("temperature must be between 1e-20 and 1e20")
     V = logits.shape[-1]
     rows, n, stride = _rows(logits, V)
     ids = tokens.contiguous()

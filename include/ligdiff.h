@@ -621,7 +621,7 @@ typedef struct ligdiff_token_args {
   int32_t vocab;
   int32_t dtype;
   int32_t token_bytes;
-  float temperature;        /* > 0: the distribution is softmax(logits / temperature)       */
+  float temperature;        /* 1e-20 .. 1e20: softmax(logits / temperature)                 */
 } ligdiff_token_args;
 
 /* logp [n_tokens] = log softmax(logits / temperature)[t, tokens[t]].  stats (may be NULL) [n_tokens, 2]: what the gradient

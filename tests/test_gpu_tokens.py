@@ -479,6 +479,111 @@ def test_gradients_against_differences(tk):
     assert abs((got.double() * v).sum() - want) <= 4 * LOGP / 0.8 * size
 
 
+# the borders of the forms that keep a row in registers, stage it or stream it: 1024 x 16 packs and longer (8192 packs of 4
+# are 32768, 16384 are 65536), short ragged and aligned rows, and up to 64 rows in one launch
+BORDERS = [(64, 119), (65, 119), (1, 65536), (3, 65537), (2, 131072), (2, 131075), (900, 3), (900, 20), (900, 48), (900, 100), (900, 128),
+           (900, 200), (500, 251), (500, 256), (500, 500), (200, 1027), (70, 2047), (70, 4096)]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("T,V", BORDERS)
+def test_policy_borders(tk, dtype, T, V):
+    case = (T, V, min(T, 5), False, True, True, 0.2, 0.25, 0.1, "sequence", 1.0, None, True)
+    x, ids, ptr, adv, old, ref = policy_inputs(case, dtype)
+    scale = 1024.0 if dtype == "fp16" else 1.0
+    want = policy_oracle(x, ids, ptr, adv, False, old, ref, 0.2, 0.25, 0.1, "sequence", 1.0, None)
+    off = LOGP + max(0, V / 1024 - 64) * U       # (a lane of the longest rows adds up more than 64 terms)
+    e = off + 16 * U
+    slack = policy_slack(want, scale, 1.0) * (off / LOGP)
+    for y in (x, strided(x, 8, 0)[0], strided(x, 5, 1)[0]):
+        got = tk.policy_loss_and_grad(y, ids, ptr, adv, old, ref, "sequence", 0.2, 0.25, 0.1, "sequence", 1.0, None, scale)
+        within(got.logp[want["on"]], want["logp"][want["on"]], off, "logp")
+        within(got.loss, want["loss"], (e * (want["ds"] + 0.1 * want["dk"]) + 8 * U * want["w"]).sum(), "loss")
+        within(got.d_logits, want["d"] * scale, slack, "d_logits")
+
+
+@pytest.mark.parametrize("T,P", [(1023, 1024), (1024, 1024), (1024, 1025), (1025, 1), (1025, 1025), (3000, 1500), (64, 32), (65, 32)])
+def test_preference_borders(tk, T, P):
+    """One chunk of rows and up to 1024 pairs go in fewer launches: the same formula on both sides."""
+    g = gen(T + P)
+    x = torch.randn(T, 37, device="cuda", generator=g)
+    ids, ptr = ids_of(T, 37, g, 0.1), cuts(T, 2 * P, g)
+    got = tk.preference_loss_and_grad(x, ids, ptr, beta=0.4)
+    want = preference_oracle(x, ids, ptr, None, 0.4, 0.0, "sigmoid", False, 1.0, None)
+    slack = (want["n"] + 1) * (LOGP + U)
+    gap = slack[:P] + slack[P:]
+    within(got.log_ratio, want["log_ratio"], slack, "log_ratio")
+    within(got.margin, want["margin"], gap, "margin")
+    within(got.loss, want["loss"], 0.4 * gap.mean() + 1e-12, "loss")
+    g_off = torch.where(want["g"] != 0, (0.04 / P * gap)[owner_of(ptr, T).clamp(min=0) % P], 0.0) + 4 * U * want["g"].abs()
+    within(got.d_logits, want["d"], g_off[:, None] + 3 * LOGP * want["g"].abs()[:, None] * (want["p"] + 1e-3), "d_logits")
+
+
+@pytest.mark.parametrize("kind", ["alternate", "long"])
+def test_infinite_sequences_reach_no_other(tk, kind):
+    """A sequence whose log ratio is infinite or NaN changes no bit of any other's, on either side of it, in chunks of 1024
+    rows that it shares with others or crosses."""
+    g = gen(21)
+    T, P = 5000, 40
+    x, ids = torch.randn(T, 119, device="cuda", generator=g), ids_of(T, 119, g, 0.1)
+    ptr = cuts(T, 2 * P, g) if kind == "alternate" else torch.cat([torch.arange(0, 79, device="cuda") * 10, torch.tensor([1700, T], device="cuda")])
+    clean = tk.preference_loss_and_grad(x, ids, ptr)
+    owner = owner_of(ptr, T)
+    hit = [3, 20, 41, 78] if kind == "alternate" else [2, 30, 78]
+    ids_on = (ids >= 0) & (ids < 119)
+    bad = []
+    for k, s in enumerate(hit):
+        rows = ((owner == s) & ids_on).nonzero()[:, 0]
+        if len(rows) == 0:
+            continue
+        x[rows[len(rows) // 2]] = float("nan") if k % 2 else float("-inf")
+        bad.append(s)
+    assert bad
+    got = tk.preference_loss_and_grad(x, ids, ptr)
+    keep = torch.ones(2 * P, dtype=torch.bool, device="cuda")
+    keep[bad] = False
+    assert torch.equal(got.log_ratio[keep], clean.log_ratio[keep]) and not got.log_ratio[~keep].isfinite().any()
+    pairs = keep[:P] & keep[P:]
+    assert torch.equal(got.margin[pairs], clean.margin[pairs]) and not got.margin[~pairs].isfinite().any()
+    rows = pairs[owner.clamp(min=0) % P]
+    assert torch.equal(got.d_logits[rows], clean.d_logits[rows])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("V", [5, 119, 1000, 5000, 20000, 70001])
+def test_rows_far_from_zero(tk, dtype, V):
+    """Rows masked with -1e9 ... -1e38, offset by large numbers, and very low temperatures.  The values are small integers
+    times a power of two beside the offset, so that the type holds every difference exactly.  The roundings of the temperature
+    and of c and, in a shifted row, of x - m and of its product are off by 4 u of a difference in all, on top of LOGP."""
+    g = gen(V)
+    t = DTYPES[dtype]
+    ids = ids_of(24, V, g)
+    x = torch.randn(24, V, device="cuda", generator=g).to(t)
+    for k, e in enumerate((9, 10, 12, 15, 20, 30, 37, 38)):
+        x[k] = -10.0 ** e                                  # nothing but masked: uniform
+        x[8 + k, ::2] = -10.0 ** e                         # half of them masked
+    steps = torch.randint(0, 4, (8, V), device="cuda", generator=g).to(t)
+    for k, e in enumerate((6, 7, 20, 24, 31, 40, 100, 120)):
+        unit = 2.0 ** e * (2.0 ** -6 if t == torch.bfloat16 else 2.0 ** -20)    # steps of the offset 2^e that the type has
+        x[16 + k] = 2.0 ** e + steps[k] * unit
+    for tau in (1.0, 1e-3, 1e-20, 1e20):
+        z = x.double() / tau
+        got = tk.token_logprobs(x, ids, tau)
+        lp, p, on = logp_oracle(x, ids, tau)
+        zc = (z - z.amax(1, keepdim=True)).abs()
+        reach, soft = zc.gather(1, ids[:, None])[:, 0], (p * zc).sum(1)      # of the chosen id, and in the logarithm's sum
+        slack = LOGP + 4 * U * (reach + soft)
+        lp = torch.where(lp < -3.4e38, torch.full_like(lp, float("-inf")), lp)    # beyond what fp32 holds
+        within(got, lp, slack, ("logp", tau))
+        r = tk.policy_loss_and_grad(x, ids, None, torch.ones(1, device="cuda"), kl_coef=0.0, temperature=tau)
+        want = d_logits_oracle(p, ids, on, torch.full((24,), -1 / 24 / tau, dtype=torch.float64, device="cuda"))
+        slack = ((3 * LOGP + 4 * U * (zc + soft[:, None])) * p + 3 * LOGP * 1e-3) / 24 / tau + 4 * U * want.abs()
+        within(r.d_logits, want, slack, ("d_logits", tau))
+    for bad in (1e-21, 1e21, 0.0, float("inf")):
+        with pytest.raises(ValueError, match="temperature"):
+            tk.token_logprobs(x, ids, bad)
+
+
 # ------------------------------------------------------------------------------------------------ how they are called
 def test_two_backwards_of_one_graph(tk):
     g = gen(10)

@@ -22,7 +22,8 @@ def rows(**kw):
 @pytest.mark.parametrize("kw", [dict(vocab=0), dict(vocab=-3), dict(row_stride=118), dict(row_stride=0), dict(n_tokens=-1),
                                 dict(n_tokens=1 << 31), dict(dtype=3), dict(dtype=-1), dict(token_bytes=2),
                                 dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("nan")),
-                                dict(temperature=float("inf")), dict(logits=None), dict(tokens=None)])
+                                dict(temperature=float("inf")), dict(temperature=1e-21), dict(temperature=1e21), dict(logits=None),
+                                dict(tokens=None)])
 def test_token_rows_are_checked(lib, kw):
     a = rows(**kw)
     assert lib.ligdiff_token_logprob(C.byref(a), P, P, None) == ARG
