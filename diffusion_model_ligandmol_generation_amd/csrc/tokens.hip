@@ -267,10 +267,9 @@ __device__ __forceinline__ float part_factor(float m, float M, float c) {
 #pragma clang fp contract(off)   // both products are the rounded numbers that the exponentials used
   if (m == -__builtin_inff()) return 0.f;
   const float mc = m * c, Mc = M * c;
-  if (__builtin_expect(far_out(m, c) || far_out(M, c), 0)) {   // one of them may be shifted: exact products (48 bits) for it
-    const double dm = far_out(m, c) ? (double)m * c : (double)mc, dM = far_out(M, c) ? (double)M * c : (double)Mc;
-    return m == M ? 1.f : __builtin_amdgcn_exp2f((float)(dm - dM));
-  }
+  const bool far_m = far_out(m, c), far_M = far_out(M, c);
+  if (__builtin_expect(far_m || far_M, 0))   // (a shifted one has no rounded product)
+    return __builtin_amdgcn_exp2f(shifted(m, M) * c + (far_M ? 0.f : __builtin_fmaf(M, c, -Mc)) - (far_m ? 0.f : __builtin_fmaf(m, c, -mc)));
   return __builtin_amdgcn_exp2f(mc - Mc);
 }
 // The maximum and sum of a row from those of its 4 or 16 waves (0 and 0 for a row of -inf only).

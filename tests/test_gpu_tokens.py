@@ -584,6 +584,23 @@ def test_rows_far_from_zero(tk, dtype, V):
             tk.token_logprobs(x, ids, bad)
 
 
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("V", [1000, 5000, 20000, 70001])
+def test_parts_on_both_sides_of_far(tk, V, sign):
+    """Rows whose parts have maxima on both sides of the border 2^24 / log2(e) = 11629080 at which a row is shifted."""
+    g = gen(V)
+    x = sign * (11629080.0 + torch.randint(-8, 9, (16, V), device="cuda", generator=g).float())
+    x[:8] -= torch.arange(V, device="cuda").float() * (16 / V)       # (and a slope, rounded to whole numbers)
+    x = x.round()
+    ids = ids_of(16, V, g)
+    got = tk.token_logprobs(x, ids)
+    lp, p, on = logp_oracle(x, ids)
+    within(got, lp, LOGP + 4 * U * 64, "logp")                       # (no difference is above 32, as in the test above)
+    r = tk.policy_loss_and_grad(x, ids, None, torch.ones(1, device="cuda"), kl_coef=0.0)
+    want = d_logits_oracle(p, ids, on, torch.full((16,), -1 / 16, dtype=torch.float64, device="cuda"))
+    within(r.d_logits, want, (3 * LOGP + 4 * U * 64) / 16 * (p + 1e-3) + 4 * U * want.abs(), "d_logits")
+
+
 # ------------------------------------------------------------------------------------------------ how they are called
 def test_two_backwards_of_one_graph(tk):
     g = gen(10)
