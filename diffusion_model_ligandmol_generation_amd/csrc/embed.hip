@@ -1,10 +1,11 @@
 // Embedding lookup with scaling, and its gradient by sorted tokens.
 //   out[i, :] = scale W[tok_i, :]                       d_W[v, :] = scale sum_{i: tok_i = v} d_out[i, :]
-// Both are bound by HBM.  The gradient sorts the token positions (a stable radix sort of 8-byte records, small against the
-// rows) and then sums rows of equal tokens: every row of d_out is read once, in 32 bits and in a fixed order, no float
-// atomics, so the result does not change from run to run.  The tokens of a batch are very uneven (half of a ligand's atoms are
-// carbon), so the sorted positions are cut into chunks of equal length whatever the tokens are; a token whose positions
-// lie in several chunks leaves one partial row in each, and a second launch joins them.
+// Both are bound by HBM, small calls by their launches.  The gradient reads every row of d_out once and adds in 32 bits and in a
+// fixed order, no float atomics, so the result does not change from run to run.  The tokens of a batch are very uneven (half
+// of a ligand's atoms are carbon), so the work is cut into equal numbers of rows whatever their tokens are.  Tables of up to
+// 128 rows are added up in LDS (two launches).  For larger ones the token positions are sorted (a stable radix sort of 8-byte
+// records, small against the rows) and cut into chunks; a token whose positions lie in several chunks leaves one partial row
+// in each, and a last launch joins them.
 #include "embed.h"
 
 // ------------------------------------------------------------------ lookup
@@ -490,6 +491,140 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void k_segment_join(SegIn a) {
   }
 }
 
+// ------------------------------------------------------------------ tables that fit into LDS
+// Up to TABLE_ROWS rows need no sort: a wave adds its rows of d_out to a table of its own in LDS, 64 columns wide, lane by lane and
+// in order; a row more takes the tokens without one.  The block joins its waves' tables and writes one part; k_table_join
+// adds the parts in order.  Four rows make one trip to LDS; read, add and write take a tenth of the time of LDS's float
+// atomics (29696 x 256 rows and 119 tokens: 52 us with atomics, 16 so, 20 sorted).  What bounds it at 119 rows, where one
+// block of four waves fits into a compute unit, is the instructions of its waves; many rows come at 4.2 TB/s.
+#define TABLE_ROWS 128
+#define TABLE_WAVES 4
+#define TABLE_U 16   // rows in flight, twice
+struct TableIn {
+  const void* d_out; int64_t d_stride;
+  TokenView tok; int64_t n;
+  int32_t rows, D, n_tiles, n_chunks;
+  int64_t per_wave;
+  float scale;
+  float* part;                               // [n_chunks][rows][D]
+  void* d_table; int64_t t_stride;
+  bool accumulate;
+};
+template <typename T> struct RawBits { typedef uint16_t type; };
+template <> struct RawBits<float> { typedef float type; };
+template <typename T, int ROWS>
+__global__ __launch_bounds__(TABLE_WAVES * 64) void k_table_sums(TableIn a) {
+  __shared__ __attribute__((aligned(16))) float tab[TABLE_WAVES][ROWS + 1][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int chunk = blockIdx.x / a.n_tiles, tile = blockIdx.x % a.n_tiles;
+  const int col = tile * 64 + lane;
+  const uint32_t at = (uint32_t)(col < a.D ? col : a.D - 1) * (uint32_t)sizeof(T);
+  const int64_t w0 = ((int64_t)chunk * TABLE_WAVES + wave) * a.per_wave, left = a.n - w0;
+  const int rows = left <= 0 ? 0 : (int)(left < a.per_wave ? left : a.per_wave);
+  f32x4* const clear = reinterpret_cast<f32x4*>(&tab[wave][0][0]);
+#pragma unroll 4
+  for (int k = lane; k < (a.rows + 1) * 16; k += 64) clear[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // a lane only ever touches its own column of its own wave's table
+  typename RawBits<T>::type v[2][TABLE_U];    // as loaded (a conversion right behind the load would wait for it)
+  int id[2];                                  // of 64 rows, a lane each
+  const auto tokens = [&](int b) {
+    int k = a.rows;
+    if (b + lane < rows) {
+      k = a.tok.at(w0 + b + lane);
+      if (k < 0) k = a.tok.n_rows;            // (row n_rows of the table, or the one behind it)
+    }
+    return k;
+  };
+  // the rows of a batch lie at fixed 32-bit offsets from its first (the host sees to it), behind the last row at the last one's
+  const int64_t step = a.d_stride * (int64_t)sizeof(T);
+  const char* row = reinterpret_cast<const char*>(a.d_out) + w0 * step;
+  uint32_t off[TABLE_U];
+#pragma unroll
+  for (int u = 0; u < TABLE_U; ++u) off[u] = at + (uint32_t)u * (uint32_t)step;
+  const auto fetch = [&](int b, typename RawBits<T>::type (&x)[TABLE_U]) {
+    if (b >= rows) return;
+    if (rows - b < TABLE_U) {
+#pragma unroll
+      for (int u = 0; u < TABLE_U; ++u)
+        off[u] = at + (uint32_t)(u < rows - b ? u : rows - b - 1) * (uint32_t)step;
+    }
+#pragma unroll
+    for (int u = 0; u < TABLE_U; ++u) {
+      asm("" : "+v"(off[u]));     // a 32-bit offset to the row's scalar address
+      x[u] = *reinterpret_cast<const typename RawBits<T>::type*>(row + off[u]);
+    }
+    row += TABLE_U * step;
+  };
+  float* const own = &tab[wave][0][lane];
+  if (rows > 0) {
+    id[0] = tokens(0);
+    fetch(0, v[0]);
+    for (int b = 0; b < rows; b += 64) {
+      id[1] = tokens(b + 64);
+#pragma unroll
+      for (int q = 0; q < 64 / TABLE_U; ++q) {
+        if (b + q * TABLE_U >= rows) break;
+        fetch(b + (q + 1) * TABLE_U, v[(q + 1) & 1]);
+#pragma unroll
+        for (int u = 0; u < TABLE_U; u += 4) {   // four at a time: one trip to LDS; a later row of the same token adds to the earlier
+          float x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            asm("" : "+v"(v[q & 1][u + j]));
+            x[j] = (float)__builtin_bit_cast(T, v[q & 1][u + j]);
+          }
+          const int k0 = __builtin_amdgcn_readlane(id[0], q * TABLE_U + u), k1 = __builtin_amdgcn_readlane(id[0], q * TABLE_U + u + 1);
+          const int k2 = __builtin_amdgcn_readlane(id[0], q * TABLE_U + u + 2), k3 = __builtin_amdgcn_readlane(id[0], q * TABLE_U + u + 3);
+          const float t0 = own[k0 * 64], t1 = own[k1 * 64], t2 = own[k2 * 64], t3 = own[k3 * 64];
+          const float s0 = t0 + x[0];
+          float s1 = k1 == k0 ? s0 : t1;
+          s1 += x[1];
+          float s2 = k2 == k0 ? s0 : t2;
+          s2 = k2 == k1 ? s1 : s2;
+          s2 += x[2];
+          float s3 = k3 == k0 ? s0 : t3;
+          s3 = k3 == k1 ? s1 : s3;
+          s3 = k3 == k2 ? s2 : s3;
+          s3 += x[3];
+          own[k0 * 64] = s0;
+          own[k1 * 64] = s1;
+          own[k2 * 64] = s2;
+          own[k3 * 64] = s3;
+        }
+      }
+      id[0] = id[1];
+    }
+  }
+  __syncthreads();
+  float* part = a.part + (int64_t)chunk * a.rows * a.D;
+  if (col < a.D)
+#pragma unroll 4
+    for (int k = wave; k < a.rows; k += TABLE_WAVES) {
+      float sum = tab[0][k][lane];
+#pragma unroll
+      for (int w = 1; w < TABLE_WAVES; ++w) sum += tab[w][k][lane];
+      part[(int64_t)k * a.D + col] = sum;
+    }
+}
+template <typename TO>
+__global__ __launch_bounds__(512) void k_table_join(TableIn a) {
+  __shared__ float sh[8][64];
+  const int row = blockIdx.x / a.n_tiles, tile = blockIdx.x % a.n_tiles;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = tile * 64 + lane;
+  float sum = 0.f;
+  if (col < a.D) {
+    const float* p = a.part + (int64_t)row * a.D + col;
+#pragma unroll 8
+    for (int c = wave; c < a.n_chunks; c += 8) sum += p[(int64_t)c * a.rows * a.D];
+  }
+  sh[wave][lane] = sum;
+  __syncthreads();
+  if (wave > 0 || col >= a.D) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) sum += sh[w][lane];
+  put(reinterpret_cast<TO*>(a.d_table) + (int64_t)row * a.t_stride + col, sum * a.scale, a.accumulate);
+}
+
 // ------------------------------------------------------------------ host side
 // Sort: passes of 8 bits while they take no more passes than 11 bits would (a pass of 2048 bins costs twice one of 256: each
 // block reads the whole count table): one pass for up to 255 rows (the token outside is one more key), two below 65536 rows;
@@ -513,6 +648,20 @@ static int chunk_rows(int64_t n, int tiles) {
   while (r < 512 && n * tiles > (int64_t)r * 8192) r *= 2;
   return r;
 }
+// Blocks of the table sums: as many as the chip holds at once (a block takes rows + 1 KB of LDS), 32 rows a wave or more.
+static int64_t table_per_wave(int64_t n, int32_t rows, int32_t width) {
+  const int64_t tiles = (width + 63) / 64, held = 256 * (rows <= 32 ? 4 : rows <= 64 ? 2 : 1);
+  const int64_t chunks = tiles < held ? held / tiles : 1, waves = chunks * TABLE_WAVES;
+  const int64_t per = (n + waves - 1) / waves;
+  return per < 32 ? 32 : (per + 7) / 8 * 8;
+}
+static int64_t table_chunks(int64_t n, int32_t rows, int32_t width) {
+  const int64_t per = table_per_wave(n, rows, width) * TABLE_WAVES;
+  return (n + per - 1) / per;
+}
+// Measured against the sort (119 rows, us): 29 x 256 7 against 10, 29696 x 256 16 against 20, 29696 x 1024 32 against 39,
+// 600000 x 64 38 against 107, 600000 x 256 142 against 153; bf16 29696 x 1024 31 against 31.  (A batch's offsets are 32 bits.)
+static bool table_form(int64_t n, int32_t rows, int64_t d_stride) { return n > 0 && rows <= TABLE_ROWS && d_stride <= (1 << 24); }
 struct EmbedWs { uint32_t* key[2]; int32_t* pos[2]; int32_t* hist; int32_t* row_ptr; float* part; size_t bytes; };
 static EmbedWs embed_ws(void* base, int64_t n, int32_t rows, int32_t width) {
   char* p = (char*)base;
@@ -526,7 +675,8 @@ static EmbedWs embed_ws(void* base, int64_t n, int32_t rows, int32_t width) {
   w.row_ptr = (int32_t*)take(((size_t)rows + 1) * 4);
   // (half-precision tiles are the widest: fewest tiles, shortest chunks, most partial rows)
   const int64_t r = (int64_t)chunk_rows(n, (width + 511) / 512) * SUM_WAVES;
-  w.part = (float*)take((size_t)((n + r - 1) / r) * 2 * (size_t)width * 4);
+  const size_t parts = (size_t)((n + r - 1) / r) * 2, table = table_form(n, rows, 0) ? (size_t)table_chunks(n, rows, width) * rows : 0;
+  w.part = (float*)take((parts > table ? parts : table) * (size_t)width * 4);
   w.bytes = used;
   return w;
 }
@@ -566,6 +716,13 @@ template <int BITS> static int sort_tokens(const EmbedGrad& g, const EmbedWs& w,
   return passes;
 }
 
+template <typename T, typename TO> static void table_sums(const TableIn& a, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)a.n_chunks * a.n_tiles)), block(TABLE_WAVES * 64);
+  if (a.rows <= 32) hipLaunchKernelGGL((k_table_sums<T, 32>), grid, block, 0, s, a);
+  else if (a.rows <= 64) hipLaunchKernelGGL((k_table_sums<T, 64>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((k_table_sums<T, TABLE_ROWS>), grid, block, 0, s, a);
+  hipLaunchKernelGGL((k_table_join<TO>), dim3((unsigned)((int64_t)a.rows * a.n_tiles)), dim3(512), 0, s, a);
+}
 template <typename T, typename TO> static void segment_sums(SegIn a, hipStream_t s) {
   a.n_tiles = (a.D + 64 * Pack<T>::N - 1) / (64 * Pack<T>::N);
   a.R = chunk_rows(a.n, a.n_tiles);
@@ -583,6 +740,18 @@ template <typename T, typename TO> static void segment_sums(SegIn a, hipStream_t
 
 void embed_grad(const EmbedGrad& g, void* workspace, hipStream_t s) {
   const EmbedWs w = embed_ws(workspace, g.n, g.rows, g.width);
+  const bool wide = g.grad_dtype == LIGDIFF_F32;
+  if (table_form(g.n, g.rows, g.d_stride)) {
+    TableIn t;
+    t.d_out = g.d_out; t.d_stride = g.d_stride; t.tok = g.tok; t.n = g.n; t.rows = g.rows; t.D = g.width; t.scale = g.scale;
+    t.n_tiles = (g.width + 63) / 64; t.per_wave = table_per_wave(g.n, g.rows, g.width);
+    t.n_chunks = (int)table_chunks(g.n, g.rows, g.width); t.part = w.part;
+    t.d_table = g.d_table; t.t_stride = g.t_stride; t.accumulate = g.accumulate;
+    if (g.dtype == LIGDIFF_F32) table_sums<float, float>(t, s);
+    else if (g.dtype == LIGDIFF_BF16) { if (wide) table_sums<bf16_t, float>(t, s); else table_sums<bf16_t, bf16_t>(t, s); }
+    else { if (wide) table_sums<f16_t, float>(t, s); else table_sums<f16_t, f16_t>(t, s); }
+    return;
+  }
   SegIn a;
   a.have_ptr = false;
   int passes = 1;
@@ -596,7 +765,6 @@ void embed_grad(const EmbedGrad& g, void* workspace, hipStream_t s) {
   a.d_out = g.d_out; a.d_stride = g.d_stride; a.key = w.key[(passes - 1) & 1]; a.pos = w.pos[(passes - 1) & 1]; a.n = g.n;
   a.row_ptr = w.row_ptr; a.rows = g.rows; a.D = g.width; a.scale = g.scale; a.part = w.part;
   a.d_table = g.d_table; a.t_stride = g.t_stride; a.accumulate = g.accumulate;
-  const bool wide = g.grad_dtype == LIGDIFF_F32;
   if (g.dtype == LIGDIFF_F32) segment_sums<float, float>(a, s);
   else if (g.dtype == LIGDIFF_BF16) { if (wide) segment_sums<bf16_t, float>(a, s); else segment_sums<bf16_t, bf16_t>(a, s); }
   else { if (wide) segment_sums<f16_t, float>(a, s); else segment_sums<f16_t, f16_t>(a, s); }

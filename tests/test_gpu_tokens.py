@@ -111,6 +111,46 @@ def test_embed_grad(tk, dtype, T, V, D):
         assert torch.equal(got, tk.embed_tokens_grad(d, ids, V, 0.5))      # the same bits every time
 
 
+# tables of up to 32, 64 and 128 rows are added up in LDS, larger ones sorted: by one block up to 4096 positions
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("V", [32, 33, 64, 65, 128, 129, 200])
+def test_embed_grad_borders(tk, dtype, V):
+    g = gen(V)
+    for T, D in ((1, 64), (31, 65), (33, 256), (4096, 100), (4097, 40), (20001, 70), (2000, 1)):
+        d = torch.randn(T, D, device="cuda", generator=g, dtype=DTYPES[dtype])
+        ids = ids_of(T, V, g, 0.2)
+        d[(ids < 0) | (ids >= V)] = float("nan")          # rows of ignored tokens reach nothing
+        ids[::3] = V - 1                                  # runs and pairs of one token
+        ids[1::7] = V - 1
+        d = torch.where(d.isnan(), torch.zeros_like(d), d) if T < 4 else d
+        d[ids == V - 1] = d[ids == V - 1].nan_to_num(0.5)
+        want, slack = grad_oracle(d, ids, V, 0.5)
+        for view in (d, strided(d, 3, 1)[0]):
+            got = tk.embed_tokens_grad(view, ids, V, 0.5)
+            within(got, want, slack, (T, D))
+        assert torch.equal(got, tk.embed_tokens_grad(d, ids.int(), V, 0.5))
+        out, buf = strided(torch.randn(V, D, device="cuda", generator=g), 2, 1)
+        start = out.clone()
+        tk.embed_tokens_grad(d, ids, V, 0.5, out=out, accumulate=True)
+        within(out, start.double() + want, slack + U * (start.abs().double() + want.abs()), "accumulate")
+        assert (buf[:, 0] == 7).all() and (buf[:, -1] == 7).all()
+
+
+def test_embed_grad_far_rows(tk):
+    """Rows of the gradient 2^26 + 4 bytes apart and more (past 32-bit offsets), and one row for all of them (stride 0)."""
+    buf = torch.zeros(40 * ((1 << 24) + 1), device="cuda")
+    d = buf.view(40, -1)[:, :48]
+    d.copy_(torch.randn(40, 48, device="cuda", generator=gen(5)))
+    ids = torch.arange(40, device="cuda") % 7
+    for rows in (d, buf.view(40, -1)[:, 1:48], d[:1].expand(40, 48)):
+        want, slack = grad_oracle(rows, ids, 7, 1.0)
+        within(tk.embed_tokens_grad(rows, ids, 7), want, slack, "far apart")
+    near = buf[:40 * (1 << 24)].view(40, 1 << 24)[:, :48]       # the widest stride of the tables in LDS
+    near.copy_(torch.randn(40, 48, device="cuda", generator=gen(6)))
+    want, slack = grad_oracle(near, ids, 7, 1.0)
+    within(tk.embed_tokens_grad(near, ids, 7), want, slack, "2^24 apart")
+
+
 @pytest.mark.parametrize("dtype", list(DTYPES))
 def test_embed_grad_outputs_and_strides(tk, dtype):
     g = gen(3)
