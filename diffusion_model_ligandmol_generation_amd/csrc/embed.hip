@@ -7,6 +7,7 @@
 // records, small against the rows) and cut into chunks; a token whose positions lie in several chunks leaves one partial row
 // in each, and a last launch joins them.
 #include "embed.h"
+#include <algorithm>
 
 // ------------------------------------------------------------------ lookup
 // TPR lanes a row, four rows in flight per group: the token, then the row, then the store are dependent accesses.
@@ -91,16 +92,24 @@ struct SortPass {
   int32_t shift, per_block;            // per_block: a multiple of SORT_NT
   int32_t* hist;                       // [blocks][bins]
   int32_t* row_ptr; int32_t rows;      // one-pass sorts: block 0 writes the first position of every token, [rows + 1]
+  int32_t blocks;                      // that sort; those behind them clear a part of the table
+  u32x4* clear; int64_t n_clear;
 };
+// A sort keeps few compute units busy and waits for memory most of the time: the others write zeros to the table meanwhile.
+__device__ __forceinline__ void clear_part(const SortPass& a) {
+  const int64_t step = (int64_t)(gridDim.x - a.blocks) * blockDim.x;
+  for (int64_t i = (int64_t)(blockIdx.x - a.blocks) * blockDim.x + threadIdx.x; i < a.n_clear; i += step) a.clear[i] = u32x4{0, 0, 0, 0};
+}
 template <bool FIRST> __device__ __forceinline__ uint32_t sort_key(const SortPass& a, int64_t i) {
   if (!FIRST) return a.key_in[i];
   const int id = a.tok.at(i);
   return id < 0 ? (uint32_t)a.tok.n_rows : (uint32_t)id;
 }
-template <int BITS, bool FIRST>
+template <int BITS, bool FIRST, bool CLEAR>
 __global__ __launch_bounds__(SORT_NT) void k_sort_count(SortPass a) {
   constexpr int NB = 1 << BITS;
   __shared__ int cnt[NB];
+  if (CLEAR && (int)blockIdx.x >= a.blocks) return clear_part(a);
   for (int d = threadIdx.x; d < NB; d += SORT_NT) cnt[d] = 0;
   __syncthreads();
   const int64_t b0 = (int64_t)blockIdx.x * a.per_block;
@@ -112,11 +121,12 @@ __global__ __launch_bounds__(SORT_NT) void k_sort_count(SortPass a) {
 // Each block finds its own offsets from the count table (no scan launch): total and preceding blocks' counts of every digit,
 // a prefix sum over the digits, then one over its waves; a wave ranks 64 positions at a time by the lanes that hold the
 // same digit, so positions of equal digits keep their order.
-template <int BITS, bool FIRST>
+template <int BITS, bool FIRST, bool CLEAR>
 __global__ __launch_bounds__(SORT_NT) void k_sort_scatter(SortPass a) {
   constexpr int NB = 1 << BITS, K = NB > SORT_NT ? NB / SORT_NT : 1, LIVE = NB / K;
   __shared__ int cnt[SORT_WAVES][NB];
   __shared__ int wtot[SORT_WAVES];
+  if (CLEAR && (int)blockIdx.x >= a.blocks) return clear_part(a);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // this wave's first keys are on their way while the count table is read
   constexpr int PRE = 2;
@@ -133,7 +143,7 @@ __global__ __launch_bounds__(SORT_NT) void k_sort_scatter(SortPass a) {
   int total[K] = {}, before[K] = {};
   if (tid < LIVE) {
 #pragma unroll 8
-    for (int b = 0; b < (int)gridDim.x; ++b)
+    for (int b = 0; b < (CLEAR ? a.blocks : (int)gridDim.x); ++b)
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int h = a.hist[(int64_t)b * NB + tid * K + k];
@@ -218,6 +228,7 @@ __global__ __launch_bounds__(SORT_SMALL_NT) void k_sort_small(SortPass a) {
   __shared__ uint16_t pos[SORT_SMALL];
   __shared__ int cnt[WAVES][256];
   __shared__ int wtot[4];
+  if (blockIdx.x > 0) return clear_part(a);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = (int)a.n, w0 = wave * 64 * EACH;
   uint32_t k[EACH];
   uint16_t p[EACH];
@@ -294,7 +305,7 @@ struct SegIn {
   float scale;
   float* part;                               // [n_chunks][2][D], a chunk here SUM_WAVES * R positions
   void* d_table; int64_t t_stride;
-  bool accumulate;
+  bool accumulate, cleared;                  // cleared: the sort wrote zeros to the table
   int32_t zero_blocks;
 };
 #define SUM_WAVES 8
@@ -344,7 +355,7 @@ __global__ __launch_bounds__(SUM_WAVES * 64) void k_segment_sums(SegIn a) {
       ptr[k] = p;
     }
     __syncthreads();
-    if (a.accumulate) return;
+    if (a.accumulate || a.cleared) return;
     for (int k = wave; k < ZERO_ROWS && v0 + k < a.rows; k += SUM_WAVES) {
       if (ptr[k + 1] != ptr[k]) continue;
       TO* row = reinterpret_cast<TO*>(a.d_table) + (int64_t)(v0 + k) * a.t_stride;
@@ -494,7 +505,7 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void k_segment_join(SegIn a) {
 // ------------------------------------------------------------------ tables that fit into LDS
 // Up to TABLE_ROWS rows need no sort: a wave adds its rows of d_out to a table of its own in LDS, 64 columns wide, lane by lane and
 // in order; a row more takes the tokens without one.  The block joins its waves' tables and writes one part; k_table_join
-// adds the parts in order.  Four rows make one trip to LDS; read, add and write take a tenth of the time of LDS's float
+// adds the parts in order.  Four rows make one trip to LDS; read, add and write take a third of the time that LDS's float
 // atomics (29696 x 256 rows and 119 tokens: 52 us with atomics, 16 so, 20 sorted).  What bounds it at 119 rows, where one
 // block of four waves fits into a compute unit, is the instructions of its waves; many rows come at 4.2 TB/s.
 #define TABLE_ROWS 128
@@ -682,6 +693,15 @@ static EmbedWs embed_ws(void* base, int64_t n, int32_t rows, int32_t width) {
 }
 size_t embed_grad_workspace(int64_t n, int32_t rows, int32_t width) { return embed_ws(nullptr, n, rows, width).bytes; }
 
+// The table in 16-byte units if the sort's launches clear it: it has to be one aligned piece of memory, and where the sort takes
+// several launches of several blocks, most of its rows empty; else every row that is written twice costs more than the others
+// gain (bf16, us: 32000 x 1024 with 4096 positions 31 -> 28, 8192 35 -> 38, 65536 61 -> 69; 10^6 x 64 with 10^5 171 -> 152).
+static int64_t table_units(const EmbedGrad& g) {
+  const int64_t bytes = (int64_t)g.rows * g.width * (g.grad_dtype == LIGDIFF_F32 ? 4 : 2);
+  if (g.accumulate || g.n == 0 || g.t_stride != g.width || (reinterpret_cast<uintptr_t>(g.d_table) | bytes) % 16) return 0;
+  return g.n <= SORT_SMALL || g.rows / 8 >= g.n ? bytes / 16 : 0;
+}
+static int clear_blocks(int64_t units, int threads) { return (int)std::min<int64_t>((units + threads - 1) / threads, 1024); }
 // Sorts into key[0] / pos[0]; returns whether it wrote row_ptr.
 static bool sort_small(const EmbedGrad& g, const EmbedWs& w, hipStream_t s) {
   SortPass a{};
@@ -689,10 +709,12 @@ static bool sort_small(const EmbedGrad& g, const EmbedWs& w, hipStream_t s) {
   const int passes = sort_passes(g.tok.n_rows, 8);
   const bool ptr = passes == 1 && g.rows < 256;
   a.row_ptr = ptr ? w.row_ptr : nullptr;
-  if (passes == 1) hipLaunchKernelGGL(k_sort_small<1>, dim3(1), dim3(SORT_SMALL_NT), 0, s, a);
-  else if (passes == 2) hipLaunchKernelGGL(k_sort_small<2>, dim3(1), dim3(SORT_SMALL_NT), 0, s, a);
-  else if (passes == 3) hipLaunchKernelGGL(k_sort_small<3>, dim3(1), dim3(SORT_SMALL_NT), 0, s, a);
-  else hipLaunchKernelGGL(k_sort_small<4>, dim3(1), dim3(SORT_SMALL_NT), 0, s, a);
+  a.blocks = 1; a.clear = (u32x4*)g.d_table; a.n_clear = table_units(g);
+  const dim3 grid(1 + clear_blocks(a.n_clear, SORT_SMALL_NT));
+  if (passes == 1) hipLaunchKernelGGL(k_sort_small<1>, grid, dim3(SORT_SMALL_NT), 0, s, a);
+  else if (passes == 2) hipLaunchKernelGGL(k_sort_small<2>, grid, dim3(SORT_SMALL_NT), 0, s, a);
+  else if (passes == 3) hipLaunchKernelGGL(k_sort_small<3>, grid, dim3(SORT_SMALL_NT), 0, s, a);
+  else hipLaunchKernelGGL(k_sort_small<4>, grid, dim3(SORT_SMALL_NT), 0, s, a);
   return ptr;
 }
 template <int BITS> static int sort_tokens(const EmbedGrad& g, const EmbedWs& w, hipStream_t s) {
@@ -700,18 +722,31 @@ template <int BITS> static int sort_tokens(const EmbedGrad& g, const EmbedWs& w,
   a.tok = g.tok; a.n = g.n; a.per_block = sort_per_block(g.n, BITS); a.hist = w.hist; a.rows = g.rows;
   const int blocks = (int)((g.n + a.per_block - 1) / a.per_block);
   const int passes = sort_passes(g.tok.n_rows, BITS);
+  a.blocks = blocks;
+  const int64_t units = table_units(g), each = (units + 2 * passes - 1) / (2 * passes);
+  int64_t from = 0;
+  const auto clear = [&]() {    // the next part of the table; returns the launch's grid
+    a.clear = (u32x4*)g.d_table + from;
+    a.n_clear = std::min(each, units - from);
+    from += a.n_clear;
+    return dim3(blocks + clear_blocks(a.n_clear, SORT_NT));
+  };
+  const auto pass = [&](auto first) {
+    constexpr bool FIRST = decltype(first)::value;
+    const dim3 count = clear();
+    if (units) hipLaunchKernelGGL((k_sort_count<BITS, FIRST, true>), count, dim3(SORT_NT), 0, s, a);
+    else hipLaunchKernelGGL((k_sort_count<BITS, FIRST, false>), count, dim3(SORT_NT), 0, s, a);
+    const dim3 scatter = clear();
+    if (units) hipLaunchKernelGGL((k_sort_scatter<BITS, FIRST, true>), scatter, dim3(SORT_NT), 0, s, a);
+    else hipLaunchKernelGGL((k_sort_scatter<BITS, FIRST, false>), scatter, dim3(SORT_NT), 0, s, a);
+  };
   for (int p = 0; p < passes; ++p) {
     a.shift = p * BITS;
     a.key_in = w.key[(p + 1) & 1]; a.pos_in = w.pos[(p + 1) & 1];
     a.key_out = w.key[p & 1]; a.pos_out = w.pos[p & 1];
     a.row_ptr = passes == 1 && g.rows < (1 << BITS) ? w.row_ptr : nullptr;
-    if (p == 0) {
-      hipLaunchKernelGGL((k_sort_count<BITS, true>), dim3(blocks), dim3(SORT_NT), 0, s, a);
-      hipLaunchKernelGGL((k_sort_scatter<BITS, true>), dim3(blocks), dim3(SORT_NT), 0, s, a);
-    } else {
-      hipLaunchKernelGGL((k_sort_count<BITS, false>), dim3(blocks), dim3(SORT_NT), 0, s, a);
-      hipLaunchKernelGGL((k_sort_scatter<BITS, false>), dim3(blocks), dim3(SORT_NT), 0, s, a);
-    }
+    if (p == 0) pass(std::true_type());
+    else pass(std::false_type());
   }
   return passes;
 }
@@ -764,7 +799,7 @@ void embed_grad(const EmbedGrad& g, void* workspace, hipStream_t s) {
   }
   a.d_out = g.d_out; a.d_stride = g.d_stride; a.key = w.key[(passes - 1) & 1]; a.pos = w.pos[(passes - 1) & 1]; a.n = g.n;
   a.row_ptr = w.row_ptr; a.rows = g.rows; a.D = g.width; a.scale = g.scale; a.part = w.part;
-  a.d_table = g.d_table; a.t_stride = g.t_stride; a.accumulate = g.accumulate;
+  a.d_table = g.d_table; a.t_stride = g.t_stride; a.accumulate = g.accumulate; a.cleared = table_units(g) > 0;
   if (g.dtype == LIGDIFF_F32) segment_sums<float, float>(a, s);
   else if (g.dtype == LIGDIFF_BF16) { if (wide) segment_sums<bf16_t, float>(a, s); else segment_sums<bf16_t, bf16_t>(a, s); }
   else { if (wide) segment_sums<f16_t, float>(a, s); else segment_sums<f16_t, f16_t>(a, s); }

@@ -136,6 +136,24 @@ def test_embed_grad_borders(tk, dtype, V):
         assert (buf[:, 0] == 7).all() and (buf[:, -1] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("T,V,D", [(4096, 1000, 64), (4097, 40000, 16), (5000, 40001, 24), (5001, 40001, 24), (9000, 72000, 8), (9000, 5000000, 4)])
+def test_embed_grad_cleared(tk, dtype, T, V, D):
+    """Large tables are cleared beside the sort (aligned, in one piece, at least 8 rows a position), else behind it: no row
+    keeps what was in it, and nothing beyond the table is written."""
+    g = gen(T + V)
+    d = torch.randn(T, D, device="cuda", generator=g, dtype=DTYPES[dtype])
+    ids = ids_of(T, V, g, 0.1)
+    ids[:5] = torch.tensor([0, V - 1, V - 1, 1, 0], device="cuda")
+    want, slack = grad_oracle(d, ids, V, 1.0)
+    for lead in (0, 8, 3):
+        buf = torch.full((lead + V * D + 9,), 7.0, device="cuda", dtype=d.dtype)
+        out = buf[lead:lead + V * D].view(V, D)
+        tk.embed_tokens_grad(d, ids, V, out=out)
+        within(out, want, slack, lead)
+        assert (buf[:lead] == 7).all() and (buf[lead + V * D:] == 7).all()
+
+
 def test_embed_grad_far_rows(tk):
     """Rows of the gradient 2^26 + 4 bytes apart and more (past 32-bit offsets), and one row for all of them (stride 0)."""
     buf = torch.zeros(40 * ((1 << 24) + 1), device="cuda")
