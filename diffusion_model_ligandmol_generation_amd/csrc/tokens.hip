@@ -317,6 +317,21 @@ __device__ __forceinline__ void exponentials(u32x4 (&x)[NV], int nb, float m, fl
     }
   }
 }
+// Half-precision rows that start between two 32-bit words (odd strides): a pack across word borders comes at three quarters of the
+// rate, so blocks of one row read the words themselves, five a pack, and shift them.  The halves before and behind the pack
+// that come with them lie in words of the row's own ends.  (6006 rows of 32003 bf16: 101 us, 92 so.)
+template <typename T, int TPR> __device__ __forceinline__ bool between_words(const T* row) {
+  return sizeof(T) == 2 && TPR >= 256 && uniform((int)reinterpret_cast<uintptr_t>(row) & 2);
+}
+template <typename T> __device__ __forceinline__ u32x4 load_words(const T* p, uint32_t& last) {
+  typedef uint32_t words __attribute__((ext_vector_type(4), aligned(4)));
+  last = *reinterpret_cast<const uint32_t*>(p + 7);
+  return *reinterpret_cast<const words*>(p - 1);
+}
+__device__ __forceinline__ void shift_words(u32x4& x, uint32_t last) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = __builtin_amdgcn_alignbit(j < 3 ? x[j < 3 ? j + 1 : 3] : last, x[j], 16);
+}
 // Short rows are loaded one row ahead of their arithmetic: a wave has two rows' bytes under way.
 #define ROW_AHEAD(TPR, REGS, MODE) ((REGS) <= 8)
 // Waves a SIMD holds at once: what the registers of a row allow.
@@ -325,9 +340,12 @@ __device__ __forceinline__ void exponentials(u32x4 (&x)[NV], int nb, float m, fl
 // Rows that fit the registers of TPR lanes, NV packs a lane: the logits are read once, exponentiated once, and the policy
 // loss writes its gradient from the same registers.  TPR = 8 / 16 / 64: several rows a block and no barrier; 256 / 1024: one
 // row a block, whose waves take the maximum and sum of their own part and exchange the pair once.
-template <typename T, int TPR, int NV, int MODE, bool STAGE = false>
+// FORM: ROW_STAGED writes gradients of ragged short rows through LDS, ROW_WORDS reads rows between words.
+enum { ROW_PLAIN, ROW_STAGED, ROW_WORDS };
+template <typename T, int TPR, int NV, int MODE, int FORM = ROW_PLAIN>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)) void k_token_rows(TokenRows a, PolicyIn p, RowOut o) {
   constexpr int N = Pack<T>::N, NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR, NW = TPR / 64, GRP = TPR < 64 ? TPR : 64;
+  constexpr bool STAGE = FORM == ROW_STAGED, WORDS = FORM == ROW_WORDS;
   constexpr bool KEEP = MODE != TK_LOGP && sizeof(T) == 4;   // the exponentials take the logits' registers
   constexpr bool AHEAD = ROW_AHEAD(TPR, NV * 4, MODE);
   constexpr int STAGE_ROWS = 64 / (TPR < 64 ? TPR : 64), STAGE_V = TPR * NV * N + N;   // (a multiple of a pack)
@@ -354,16 +372,30 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
     if (MODE != TK_LOGP && c.seq < 0) c.id = -1;
     return c;
   };
+  static_assert(!(WORDS && AHEAD), "rows between words are shifted right behind their load");
   const auto load = [&](const RowScalars& c, int64_t t, u32x4 (&x)[NV], float& et, float& xt, float& A, int& len) {
     const T* row = reinterpret_cast<const T*>(a.x) + t * a.stride;
+    uint32_t last[WORDS ? NV : 1];
+    const bool words = WORDS && between_words<T, TPR>(row);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       x[k] = raw_minus_inf<T>();
+      if constexpr (WORDS) {
+        last[k] = x[k][0];
+        if (words) {
+          if (r + k * TPR < nb) x[k] = load_words(row + (int64_t)(r + k * TPR) * N, last[k]);
+          continue;
+        }
+      }
       if (r + k * TPR < nb) x[k] = load_raw(row + (int64_t)(r + k * TPR) * N);
     }
     et = -__builtin_inff();
     if (r < tail) et = (float)row[nb * N + r];
     xt = (float)row[c.id];
+    if constexpr (WORDS)
+      if (words)
+#pragma unroll
+        for (int k = 0; k < NV; ++k) shift_words(x[k], last[k]);
     if constexpr (MODE != TK_LOGP) {
       A = p.adv[p.adv_per_token ? t : (int64_t)c.seq];
       len = !p.per_seq_mean ? 1 : MODE == TK_SMALL ? small_len[t] : p.seq_len[c.seq];
@@ -496,30 +528,29 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
 template <typename T, int TPR>
 __device__ __forceinline__ void row_gradient(const TokenRows& a, const T* row, T* d, int id, int r, float M, float inv_s, float g) {
   constexpr int N = Pack<T>::N;
-  const int V = a.V, nb = V / N, tail = V - nb * N;
+  // rows between words: packs from the second element on, the first goes to lane 0 beside the tail
+  const int shift = between_words<T, TPR>(row), V = a.V, nb = (V - shift) / N, tail = V - nb * N;
   const bool off = g == 0.f || inv_s == 0.f, far = far_out(M, a.c);
   const float mc = far ? 0.f : M * a.c, q = -g * inv_s;
-  const int it = id / N;
+  const int at = id - shift, it = at / N;   // (-1 is in no pack)
   if (off) {
-    const float z[N] = {};
-    for (int i = r; i < nb; i += TPR) store_pack(d + (int64_t)i * N, z);
-    if (r < tail) d[nb * N + r] = (T)0.f;
+    row_zero(d, V, r, TPR);
     return;
   }
 #pragma unroll 4
   for (int i = r; i < nb; i += TPR) {
     float v[N];
-    load_pack(row + (int64_t)i * N, v);
+    load_pack(row + shift + (int64_t)i * N, v);
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = q * __builtin_amdgcn_exp2f(fmaf(far ? shifted(v[j], M) : v[j], a.c, -mc));
     if (i == it) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] += j == id - it * N ? g : 0.f;
+      for (int j = 0; j < N; ++j) v[j] += j == at - it * N ? g : 0.f;
     }
-    store_pack(d + (int64_t)i * N, v);
+    store_pack(d + shift + (int64_t)i * N, v);
   }
   if (r < tail) {
-    const int v = nb * N + r;
+    const int v = shift && r == 0 ? 0 : nb * N + r;
     const float x = (float)row[v];
     d[v] = (T)(q * __builtin_amdgcn_exp2f(fmaf(far ? shifted(x, M) : x, a.c, -mc)) + (v == id ? g : 0.f));
   }
@@ -549,6 +580,7 @@ __global__ __launch_bounds__(1024) void k_token_rows_long(TokenRows a, PolicyIn 
       continue;
     }
     const T* row = reinterpret_cast<const T*>(a.x) + t * a.stride;
+    const bool words = between_words<T, NT>(row);
     const float xt = (float)row[id];
     double w = 0.0;
     float A = 0.f;
@@ -559,8 +591,16 @@ __global__ __launch_bounds__(1024) void k_token_rows_long(TokenRows a, PolicyIn 
     float m = -__builtin_inff(), s = 0.f;   // of this lane: s relative to m
     for (int i = r; i < nb + (r < tail ? NT : 0); i += NT) {
       float v[N];
-      if (i < nb) load_pack(row + (int64_t)i * N, v);
-      else {   // one element of the tail
+      if (i < nb) {
+        u32x4 x;
+        if (words) {
+          uint32_t last;
+          x = load_words(row + (int64_t)i * N, last);
+          shift_words(x, last);
+        } else x = load_raw(row + (int64_t)i * N);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = raw_get<T>(x, j);
+      } else {   // one element of the tail
 #pragma unroll
         for (int j = 0; j < N; ++j) v[j] = -__builtin_inff();
         v[0] = (float)row[nb * N + r];
@@ -894,12 +934,23 @@ static int row_grid(int64_t groups, int most) { return (int)(groups < most ? gro
 #define TK_GRID_CAP 2048
 // Rows next to each other that end inside cache lines.
 static bool ragged_lines(int32_t V, int64_t d_stride, size_t size) { return d_stride == V && (V * size) % 128 != 0; }
-template <typename T, int TPR, int NV, int MODE, bool STAGE = false>
+template <typename T, int TPR, int NV, int MODE, int FORM = ROW_PLAIN>
 static int launch_rows_as(const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
   constexpr int NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR;
   const int grid = row_grid((a.n + RPB - 1) / RPB, TK_GRID_CAP * 256 / NT);
-  hipLaunchKernelGGL((k_token_rows<T, TPR, NV, MODE, STAGE>), dim3(grid), dim3(NT), 0, s, a, p, o);
+  hipLaunchKernelGGL((k_token_rows<T, TPR, NV, MODE, FORM>), dim3(grid), dim3(NT), 0, s, a, p, o);
   return grid;
+}
+// Rows of more than 512 packs, one a block, that fit its registers; 0: too long.
+template <typename T, int MODE, int FORM> static int launch_long_rows(int packs, const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
+  if (packs <= 1024) return launch_rows_as<T, 256, 4, MODE, FORM>(a, p, o, s);
+  if (packs <= 2048) return launch_rows_as<T, 256, 8, MODE, FORM>(a, p, o, s);
+  if (packs <= 4096) return launch_rows_as<T, 1024, 4, MODE, FORM>(a, p, o, s);
+  if (packs <= 8192) return launch_rows_as<T, 1024, 8, MODE, FORM>(a, p, o, s);
+  if constexpr (MODE == TK_POLICY) {
+    if (packs <= 16384) return launch_rows_as<T, 1024, 16, MODE, FORM>(a, p, o, s);
+  }
+  return 0;
 }
 // A batch of at most SMALL_ROWS short rows is one launch of one block: three launches take longer than its two rounds.
 static bool rows_of_8_lanes(int dtype, int32_t V) { return V / (dtype == LIGDIFF_F32 ? 4 : 8) <= 64; }
@@ -924,8 +975,8 @@ static int launch_rows(const TokenRows& a, const PolicyIn& p, const RowOut& o, h
     // (through LDS: 119 fp32 a row 69 us against 86 for 147 MB, 200 fp32 61 against 72, 500 bf16 70 against 76; but 30 fp32 57
     // against 52 and 90 bf16 78 against 74: rows of two lines at most are as well written directly)
     if (packs <= 64 && (size_t)a.V * sizeof(T) > 256 && o.d && ragged_lines(a.V, o.d_stride, sizeof(T))) {
-      if (packs <= 32) return launch_rows_as<T, 8, 4, MODE, true>(a, p, o, s);
-      return launch_rows_as<T, 8, 8, MODE, true>(a, p, o, s);
+      if (packs <= 32) return launch_rows_as<T, 8, 4, MODE, ROW_STAGED>(a, p, o, s);
+      return launch_rows_as<T, 8, 8, MODE, ROW_STAGED>(a, p, o, s);
     }
   }
   if (packs <= 16) return launch_rows_as<T, 8, 2, MODE>(a, p, o, s);
@@ -934,12 +985,13 @@ static int launch_rows(const TokenRows& a, const PolicyIn& p, const RowOut& o, h
   if (packs <= 128) return launch_rows_as<T, 16, 8, MODE>(a, p, o, s);
   if (packs <= 256) return launch_rows_as<T, 64, 4, MODE>(a, p, o, s);
   if (packs <= 512) return launch_rows_as<T, 64, 8, MODE>(a, p, o, s);
-  if (packs <= 1024) return launch_rows_as<T, 256, 4, MODE>(a, p, o, s);
-  if (packs <= 2048) return launch_rows_as<T, 256, 8, MODE>(a, p, o, s);
-  if (packs <= 4096) return launch_rows_as<T, 1024, 4, MODE>(a, p, o, s);
-  if (packs <= 8192) return launch_rows_as<T, 1024, 8, MODE>(a, p, o, s);
-  if constexpr (MODE == TK_POLICY) {
-    if (packs <= 16384) return launch_rows_as<T, 1024, 16, MODE>(a, p, o, s);
+  // half-precision rows some of which start between words (aligned rows would take 13% longer with the check)
+  if (sizeof(T) == 2 && ((a.stride & 1) || (reinterpret_cast<uintptr_t>(a.x) & 2))) {
+    const int grid = launch_long_rows<T, MODE, sizeof(T) == 2 ? ROW_WORDS : ROW_PLAIN>(packs, a, p, o, s);
+    if (grid) return grid;
+  } else {
+    const int grid = launch_long_rows<T, MODE, ROW_PLAIN>(packs, a, p, o, s);
+    if (grid) return grid;
   }
   const int grid = row_grid(a.n, TK_GRID_CAP);
   hipLaunchKernelGGL((k_token_rows_long<T, MODE>), dim3(grid), dim3(1024), 0, s, a, p, o);
