@@ -651,7 +651,10 @@ __global__ __launch_bounds__(256) void k_token_grad(TokenRows a, LossTail f, con
   constexpr int FLAT_V = (FLAT + 1) * Pack<T>::N;
   __shared__ __attribute__((aligned(16))) T stage[FLAT ? 4 * ROWS * FLAT_V : 1];
   T* const mine = stage + (FLAT ? (threadIdx.x >> 6) * ROWS * FLAT_V : 0);
-  for (int64_t base = (int64_t)blockIdx.x * RPB; base < a.n; base += (int64_t)blocks * RPB) {
+  for (int64_t from = (int64_t)blockIdx.x * RPB; from < a.n; from += (int64_t)blocks * RPB) {
+    // long rows from the last one back: a preference step has just read them, and the last ones may still be in the last-level
+    // cache (6007 rows of 32003 bf16 251 us against 259; without effect on batches many times its size)
+    const int64_t base = TPR == 256 ? a.n - 1 - from : from;
     const int64_t t = base + threadIdx.x / TPR;
     if (t < a.n) {
       const int id = a.tok.at(t);
