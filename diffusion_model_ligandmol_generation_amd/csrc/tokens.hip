@@ -13,18 +13,18 @@ struct TokenRows {
   int64_t n;           // rows
   int32_t V;
   TokenView tok;
-  float c;             // log2(e) / temperature: exp(x / temperature) = exp2(c x)
+  float c, c_lo;       // log2(e) / temperature = c + c_lo, 0 < c_lo <= the last place of c: exp(x / temperature) = exp2((c + c_lo) x)
   double inv_t;        // 1 / temperature
 };
 
-// exp((x - m) / temperature) of a row with maximum m is exp2(c x - mc), mc = c m: one fused multiply-add, rounded once, also
-// for logits far from 0.  mc is a rounded number, but the same one in every element and in logp, where it cancels exactly;
-// so does c, whose rounding only means a temperature that is off by 2^-25.  The largest exponent is mc's rounding error, at
-// most |mc| 2^-24: below 1 as long as |mc| < 2^24.  Rows further out (masked with -1e10 or the type's lowest value, very low
-// temperatures), where that error could overflow the exponential or lose it, are shifted by m first, and their mc is 0.
-__device__ __forceinline__ bool far_out(float m, float c) { return !(fabsf(m) * c < 16777216.f); }
-__device__ __forceinline__ float shifted(float x, float m) { return x == m ? 0.f : x - m; }   // (+inf - +inf is not asked for)
-
+// exp((x - m) / temperature) of a row with maximum m is exp2(exponent(x)).  x - m is exact where it matters (near m), the product
+// is rounded once.  One constant would do for the exponentials, but its rounding is a temperature that is off by up to 2^-25:
+// the same error 1.3e-8 (z - E[z]) in every log-probability, which sums over a sequence add up (29 atoms: twice the error
+// of the plain form).  Both parts are above 0, so that a masked -inf stays -inf.
+__device__ __forceinline__ float exponent(const TokenRows& a, float x, float m) {
+  const float d = x - m;
+  return fmaf(d, a.c, d * a.c_lo);
+}
 
 // log(s) of the softmax sum, in 64 bits: losses use differences of log-probabilities of two policies, which are small
 // against the log-probabilities.  s = 2^k f with f in [sqrt(1/2), sqrt(2)), z = (f - 1) / (f + 1),
@@ -120,8 +120,8 @@ template <int MODE>
 __device__ __forceinline__ float row_epilogue(const TokenRows& a, const PolicyIn& p, const RowOut& o, int64_t t, const RowScalars& c,
                                               float xt, float M, float S, float inv_s, bool writer, float A, double w, double* acc) {
   // a row of -inf only has no distribution: S = 0, logp = -inf, no gradient
-  const double z = far_out(M, a.c) ? ((double)xt - (double)M) * a.c : fma((double)xt, (double)a.c, -(double)(M * a.c));
-  const double lp = S == 0.f ? -__builtin_inf() : fma(z, 0.69314718055994530942, -log_of_sum(S));
+  const double z = ((double)xt - (double)M) * a.inv_t;
+  const double lp = S == 0.f ? -__builtin_inf() : z - log_of_sum(S);
   float g = 0.f, coef = 0.f;
   if constexpr (MODE != TK_LOGP) {
     const float rho = p.old_logp ? expf((float)(lp - (double)c.old)) : lp == lp ? 1.0f : (float)lp;
@@ -262,30 +262,22 @@ __global__ __launch_bounds__(256) void k_policy_final(const double* __restrict__
   }
 }
 
-// What a wave's sum, relative to its own maximum m, counts in a row with maximum M.
-__device__ __forceinline__ float part_factor(float m, float M, float c) {
-#pragma clang fp contract(off)   // both products are the rounded numbers that the exponentials used
-  if (m == -__builtin_inff()) return 0.f;
-  const float mc = m * c, Mc = M * c;
-  const bool far_m = far_out(m, c), far_M = far_out(M, c);
-  if (__builtin_expect(far_m || far_M, 0))   // (a shifted one has no rounded product)
-    return __builtin_amdgcn_exp2f(shifted(m, M) * c + (far_M ? 0.f : __builtin_fmaf(M, c, -Mc)) - (far_m ? 0.f : __builtin_fmaf(m, c, -mc)));
-  return __builtin_amdgcn_exp2f(mc - Mc);
-}
+// What a sum relative to a maximum m counts in a row with maximum M (m = -inf: nothing).
+__device__ __forceinline__ float part_factor(const TokenRows& a, float m, float M) { return __builtin_amdgcn_exp2f(exponent(a, m, M)); }
 // The maximum and sum of a row from those of its 4 or 16 waves (0 and 0 for a row of -inf only).
-template <int NW> __device__ __forceinline__ void join_waves(const float2* sh, float c, float& M, float& S) {
+template <int NW> __device__ __forceinline__ void join_waves(const TokenRows& a, const float2* sh, float& M, float& S) {
   const float2 v = sh[threadIdx.x & (NW - 1)];
   M = v.x;
   M = fmaxf(M, dpp_move<0xB1>(M));
   M = fmaxf(M, dpp_move<0x4E>(M));
   if (NW == 16) { M = fmaxf(M, dpp_move<0x141>(M)); M = fmaxf(M, dpp_move<0x140>(M)); }
   if (M == -__builtin_inff()) M = 0.f;
-  S = v.y * part_factor(v.x, M, c);
+  S = v.y * part_factor(a, v.x, M);
   S += dpp_move<0xB1>(S);
   S += dpp_move<0x4E>(S);
   if (NW == 16) { S += dpp_move<0x141>(S); S += dpp_move<0x140>(S); }
 }
-// exp2(c x - mc) of a lane's packs, handed on one pack at a time.  Half-precision packs stay packed until then (the compiler
+// The exponentials of a lane's packs, handed on one pack at a time.  Half-precision packs stay packed until then (the compiler
 // would keep the values that it unpacked for the maximum, twice the registers): the policy loss exponentiates them a second
 // time for its gradient rather than hold 32-bit results, which halves the rows in flight.
 __device__ __forceinline__ void set_pack(u32x4& x, const float (&v)[4]) {
@@ -293,28 +285,17 @@ __device__ __forceinline__ void set_pack(u32x4& x, const float (&v)[4]) {
   for (int j = 0; j < 4; ++j) x[j] = __float_as_uint(v[j]);
 }
 template <typename T, int NV, int TPR, typename F>
-__device__ __forceinline__ void exponentials(u32x4 (&x)[NV], int nb, float m, float mc, float c, bool far, F&& take) {
+__device__ __forceinline__ void exponentials(const TokenRows& a, u32x4 (&x)[NV], int nb, float m, F&& take) {
   constexpr int N = Pack<T>::N;
-  if (__builtin_expect(far, 0)) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      if (sizeof(T) == 2) asm volatile("" : "+v"(x[k]));
-      float e[N];
+  for (int k = 0; k < NV; ++k) {
+    if (k > 0 && k * TPR >= nb) break;   // no lane has a pack here
+    if (sizeof(T) == 2) asm volatile("" : "+v"(x[k]));
+    float e[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) e[j] = __builtin_amdgcn_exp2f(shifted(raw_get<T>(x[k], j), m) * c);
-      take(k, e);
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      if (k > 0 && k * TPR >= nb) break;   // no lane has a pack here
-      if (sizeof(T) == 2) asm volatile("" : "+v"(x[k]));
-      float e[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(raw_get<T>(x[k], j), c, -mc));
-      take(k, e);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    for (int j = 0; j < N; ++j) e[j] = __builtin_amdgcn_exp2f(exponent(a, raw_get<T>(x[k], j), m));
+    take(k, e);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 // Half-precision rows that start between two 32-bit words (odd strides): a pack across word borders comes at three quarters of the
@@ -446,25 +427,23 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
       for (int j = 0; j < N; ++j) m = fmaxf(m, raw_get<T>(x[k], j));
     }
     m = group_max<GRP>(m);
-    // this wave's own part: e = exp2(c x - mc)
-    const bool none = m == -__builtin_inff(), far = !none && far_out(m, a.c);
-    const float mc = none || far ? 0.f : m * a.c;
-    float s;
-    if (__builtin_expect(far, 0)) s = et = __builtin_amdgcn_exp2f(shifted(et, m) * a.c);
-    else s = et = __builtin_amdgcn_exp2f(fmaf(et, a.c, -mc));
-    exponentials<T, NV, TPR>(x, nb, m, mc, a.c, far, [&](int k, float (&e)[N]) {
+    // this wave's own part, relative to its own maximum
+    const bool none = m == -__builtin_inff();
+    if (none) m = 0.f;
+    float s = et = __builtin_amdgcn_exp2f(exponent(a, et, m));
+    exponentials<T, NV, TPR>(a, x, nb, m, [&](int k, float (&e)[N]) {
 #pragma unroll
       for (int j = 0; j < N; ++j) s += e[j];
       if constexpr (KEEP) set_pack(x[k], e);
     });
     s = group_sum<GRP>(s);
-    float M = none ? 0.f : m, S = s, f = 1.0f;
+    float M = m, S = s, f = 1.0f;
     if constexpr (NW > 1) {
       // (the buffers alternate between rows: a wave that runs ahead writes the other one)
-      if ((threadIdx.x & 63) == 0) sh[parity][threadIdx.x >> 6] = make_float2(m, s);
+      if ((threadIdx.x & 63) == 0) sh[parity][threadIdx.x >> 6] = make_float2(none ? -__builtin_inff() : m, s);
       __syncthreads();
-      join_waves<NW>(sh[parity], a.c, M, S);
-      f = part_factor(m, M, a.c);
+      join_waves<NW>(a, sh[parity], M, S);
+      f = none ? 0.f : part_factor(a, m, M);
       parity ^= 1;
     }
     float inv_s = S == 0.f ? 0.f : 1.0f / S;
@@ -503,7 +482,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
             out(k, e);
           }
         } else {
-          exponentials<T, NV, TPR>(x, nb, m, mc, a.c, far, out);
+          exponentials<T, NV, TPR>(a, x, nb, m, out);
         }
         if (r < tail) d[nb * N + r] = (T)(q * et + (nb * N + r == id ? g : 0.f));
       };
@@ -530,8 +509,8 @@ __device__ __forceinline__ void row_gradient(const TokenRows& a, const T* row, T
   constexpr int N = Pack<T>::N;
   // rows between words: packs from the second element on, the first goes to lane 0 beside the tail
   const int shift = between_words<T, TPR>(row), V = a.V, nb = (V - shift) / N, tail = V - nb * N;
-  const bool off = g == 0.f || inv_s == 0.f, far = far_out(M, a.c);
-  const float mc = far ? 0.f : M * a.c, q = -g * inv_s;
+  const bool off = g == 0.f || inv_s == 0.f;
+  const float q = -g * inv_s;
   const int at = id - shift, it = at / N;   // (-1 is in no pack)
   if (off) {
     row_zero(d, V, r, TPR);
@@ -542,7 +521,7 @@ __device__ __forceinline__ void row_gradient(const TokenRows& a, const T* row, T
     float v[N];
     load_pack(row + shift + (int64_t)i * N, v);
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = q * __builtin_amdgcn_exp2f(fmaf(far ? shifted(v[j], M) : v[j], a.c, -mc));
+    for (int j = 0; j < N; ++j) v[j] = q * __builtin_amdgcn_exp2f(exponent(a, v[j], M));
     if (i == it) {
 #pragma unroll
       for (int j = 0; j < N; ++j) v[j] += j == at - it * N ? g : 0.f;
@@ -552,7 +531,7 @@ __device__ __forceinline__ void row_gradient(const TokenRows& a, const T* row, T
   if (r < tail) {
     const int v = shift && r == 0 ? 0 : nb * N + r;
     const float x = (float)row[v];
-    d[v] = (T)(q * __builtin_amdgcn_exp2f(fmaf(far ? shifted(x, M) : x, a.c, -mc)) + (v == id ? g : 0.f));
+    d[v] = (T)(q * __builtin_amdgcn_exp2f(exponent(a, x, M)) + (v == id ? g : 0.f));
   }
 }
 
@@ -609,20 +588,19 @@ __global__ __launch_bounds__(1024) void k_token_rows_long(TokenRows a, PolicyIn 
 #pragma unroll
       for (int j = 1; j < N; ++j) mx = fmaxf(mx, v[j]);
       if (mx > m) {
-        s *= part_factor(m, mx, a.c);
+        s *= part_factor(a, m, mx);
         m = mx;
       }
-      const bool none = m == -__builtin_inff(), far = !none && far_out(m, a.c);
-      const float mc = none || far ? 0.f : m * a.c;
+      const float base = m == -__builtin_inff() ? 0.f : m;
 #pragma unroll
-      for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f(fmaf(far ? shifted(v[j], m) : v[j], a.c, -mc));
+      for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f(exponent(a, v[j], base));
     }
     const float wm = group_max<64>(m);
-    s = group_sum<64>(s * part_factor(m, wm == -__builtin_inff() ? 0.f : wm, a.c));
+    s = group_sum<64>(s * part_factor(a, m, wm == -__builtin_inff() ? 0.f : wm));
     if ((threadIdx.x & 63) == 0) sh[parity][threadIdx.x >> 6] = make_float2(wm, s);
     __syncthreads();
     float M, S;
-    join_waves<NW>(sh[parity], a.c, M, S);
+    join_waves<NW>(a, sh[parity], M, S);
     parity ^= 1;
     const float inv_s = S == 0.f ? 0.f : 1.0f / S;
     const float g = row_epilogue<MODE>(a, p, o, t, c, xt, M, S, inv_s, r == 0, A, w, acc[0]);
@@ -1040,7 +1018,10 @@ static int fill_rows(TokenRows* r, const ligdiff_token_args* a) {
   if (a->n_tokens > 0 && (!a->logits || !a->tokens)) return LIGDIFF_ERR_ARG;
   r->x = a->logits; r->stride = a->row_stride; r->n = a->n_tokens; r->V = a->vocab;
   r->tok = TokenView{a->tokens, a->token_bytes, a->vocab};
-  r->c = (float)(TK_LOG2E / (double)a->temperature);
+  const double c = TK_LOG2E / (double)a->temperature;
+  r->c = (float)c;
+  if ((double)r->c >= c) r->c = nextafterf(r->c, 0.f);
+  r->c_lo = (float)(c - (double)r->c);
   r->inv_t = 1.0 / (double)a->temperature;
   return LIGDIFF_OK;
 }
