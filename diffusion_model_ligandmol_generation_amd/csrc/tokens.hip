@@ -264,18 +264,20 @@ __global__ __launch_bounds__(256) void k_policy_final(const double* __restrict__
 
 // What a sum relative to a maximum m counts in a row with maximum M (m = -inf: nothing).
 __device__ __forceinline__ float part_factor(const TokenRows& a, float m, float M) { return __builtin_amdgcn_exp2f(exponent(a, m, M)); }
-// The maximum and sum of a row from those of its 4 or 16 waves (0 and 0 for a row of -inf only).
+// The maximum and sum of a row from those of its 4, 8 or 16 waves (0 and 0 for a row of -inf only).
 template <int NW> __device__ __forceinline__ void join_waves(const TokenRows& a, const float2* sh, float& M, float& S) {
   const float2 v = sh[threadIdx.x & (NW - 1)];
   M = v.x;
   M = fmaxf(M, dpp_move<0xB1>(M));
   M = fmaxf(M, dpp_move<0x4E>(M));
-  if (NW == 16) { M = fmaxf(M, dpp_move<0x141>(M)); M = fmaxf(M, dpp_move<0x140>(M)); }
+  if (NW >= 8) M = fmaxf(M, dpp_move<0x141>(M));
+  if (NW == 16) M = fmaxf(M, dpp_move<0x140>(M));
   if (M == -__builtin_inff()) M = 0.f;
   S = v.y * part_factor(a, v.x, M);
   S += dpp_move<0xB1>(S);
   S += dpp_move<0x4E>(S);
-  if (NW == 16) { S += dpp_move<0x141>(S); S += dpp_move<0x140>(S); }
+  if (NW >= 8) S += dpp_move<0x141>(S);
+  if (NW == 16) S += dpp_move<0x140>(S);
 }
 // The exponentials of a lane's packs, handed on one pack at a time.  Half-precision packs stay packed until then (the compiler
 // would keep the values that it unpacked for the maximum, twice the registers): the policy loss exponentiates them a second
@@ -314,13 +316,13 @@ __device__ __forceinline__ void shift_words(u32x4& x, uint32_t last) {
   for (int j = 0; j < 4; ++j) x[j] = __builtin_amdgcn_alignbit(j < 3 ? x[j < 3 ? j + 1 : 3] : last, x[j], 16);
 }
 // Short rows are loaded one row ahead of their arithmetic: a wave has two rows' bytes under way.
-#define ROW_AHEAD(TPR, REGS, MODE) ((REGS) <= 8)
+#define ROW_AHEAD(REGS) ((REGS) <= 8)
 // Waves a SIMD holds at once: what the registers of a row allow.
 #define ROW_WAVES(TPR, REGS, MODE) ((MODE) == TK_LOGP ? ((REGS) <= 16 ? 8 : (REGS) <= 32 ? 6 : 4) : (TPR) == 1024 ? ((REGS) <= 16 ? 8 : 4) : (REGS) <= 8 ? 6 : (REGS) <= 16 ? 5 : 4)
 
 // Rows that fit the registers of TPR lanes, NV packs a lane: the logits are read once, exponentiated once, and the policy
-// loss writes its gradient from the same registers.  TPR = 8 / 16 / 64: several rows a block and no barrier; 256 / 1024: one
-// row a block, whose waves take the maximum and sum of their own part and exchange the pair once.
+// loss writes its gradient from the same registers.  TPR = 8 / 16 / 64: several rows a block and no barrier; 256 / 512 / 1024:
+// one row a block, whose waves take the maximum and sum of their own part and exchange the pair once.
 // FORM: ROW_STAGED writes gradients of ragged short rows through LDS, ROW_WORDS reads rows between words.
 enum { ROW_PLAIN, ROW_STAGED, ROW_WORDS };
 template <typename T, int TPR, int NV, int MODE, int FORM = ROW_PLAIN>
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
   constexpr int N = Pack<T>::N, NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR, NW = TPR / 64, GRP = TPR < 64 ? TPR : 64;
   constexpr bool STAGE = FORM == ROW_STAGED, WORDS = FORM == ROW_WORDS;
   constexpr bool KEEP = MODE != TK_LOGP && sizeof(T) == 4;   // the exponentials take the logits' registers
-  constexpr bool AHEAD = ROW_AHEAD(TPR, NV * 4, MODE);
+  constexpr bool AHEAD = ROW_AHEAD(NV * 4);
   constexpr int STAGE_ROWS = 64 / (TPR < 64 ? TPR : 64), STAGE_V = TPR * NV * N + N;   // (a multiple of a pack)
   __shared__ __attribute__((aligned(16))) T stage[STAGE ? NT / 64 * STAGE_ROWS * STAGE_V : 1];
   __shared__ float2 sh[2][NW > 1 ? NW : 1];
@@ -922,27 +924,32 @@ static int launch_rows_as(const TokenRows& a, const PolicyIn& p, const RowOut& o
   hipLaunchKernelGGL((k_token_rows<T, TPR, NV, MODE, FORM>), dim3(grid), dim3(NT), 0, s, a, p, o);
   return grid;
 }
-// Rows of more than 512 packs, one a block, that fit its registers; 0: too long.
+// Rows of more than 1024 packs, one a block, that fit its registers; 0: too long.
 template <typename T, int MODE, int FORM> static int launch_long_rows(int packs, const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
-  if (packs <= 1024) return launch_rows_as<T, 256, 4, MODE, FORM>(a, p, o, s);
-  if (packs <= 2048) return launch_rows_as<T, 256, 8, MODE, FORM>(a, p, o, s);
-  if (packs <= 4096) return launch_rows_as<T, 1024, 4, MODE, FORM>(a, p, o, s);
-  if (packs <= 8192) return launch_rows_as<T, 1024, 8, MODE, FORM>(a, p, o, s);
+  if (packs <= 2048) return launch_rows_as<T, 256, 12, MODE, FORM>(a, p, o, s);
   if constexpr (MODE == TK_POLICY) {
+    if (packs <= 4096) return launch_rows_as<T, 512, 8, MODE, FORM>(a, p, o, s);
+  } else {
+    if (packs <= 4096) return launch_rows_as<T, 256, 16, MODE, FORM>(a, p, o, s);
+  }
+  if (packs <= 6144) return launch_rows_as<T, 512, 12, MODE, FORM>(a, p, o, s);
+  if constexpr (MODE == TK_POLICY) {
+    if (packs <= 12288) return launch_rows_as<T, 1024, 12, MODE, FORM>(a, p, o, s);
     if (packs <= 16384) return launch_rows_as<T, 1024, 16, MODE, FORM>(a, p, o, s);
   }
   return 0;
 }
 // A batch of at most SMALL_ROWS short rows is one launch of one block: three launches take longer than its two rounds.
 static bool rows_of_8_lanes(int dtype, int32_t V) { return V / (dtype == LIGDIFF_F32 ? 4 : 8) <= 64; }
-// The fewest lanes whose registers hold a row, and the fewest packs a lane: 8 lanes up to 64 packs, 16 up to 128, a wave up to 512,
-// 256 lanes up to 2048, 1024 up to 8192 (32768 fp32 or 65536 half-precision logits).  More lanes than that wait for each
-// other more often, hold fewer rows under way and do the work per row (64-bit log, ratio, KL term) for fewer rows at a time.
-// Measured on 268 MB of fp32 logits, log-probabilities / policy loss with gradient, us: 32 packs 8 lanes 43/113, 16 lanes 48/124,
-// 64 lanes 154/292; 64 packs 8 lanes 40/111, 16 lanes 42/112; 128 packs 16 lanes 41/110, 64 lanes 49/125, 256 lanes 168/345; 512 packs 64 lanes 41/112, 256 lanes 52/127; 2048 packs
-// 256 lanes 42/111, 1024 lanes 53/113; 8192 packs 1024 lanes 44/114, reading twice 45/167.  So beyond 8192 packs the
-// log-probabilities stream the row (one read in either form: 12000 packs 45 against 47) and the policy loss keeps it up to
-// 16384 packs (134 against 171).  Returns the number of blocks.
+// Few lanes with many packs each (up to 16: 64 registers) before more lanes: more lanes wait for each other more often, hold fewer
+// rows under way, have lanes without a pack in their last round, and do the work per row (64-bit log, ratio, KL term) for
+// fewer rows at a time.  Measured, log-probabilities / policy loss with gradient, us.  268 MB of fp32 logits: 32 packs 8 lanes
+// 43/113, 16 lanes 48/124, 64 lanes 154/292; 64 packs 8 lanes 40/111, 16 lanes 42/112; 128 packs 16 lanes 41/110, 64 lanes
+// 49/125.  419 MB of bf16 logits: 300 packs 64 lanes x 12 91/178, 256 x 4 185/330; 1024 packs 64 x 16 82/178, 256 x 4 89/176,
+// 256 x 8 91/172; 2500 packs 256 x 16 85/183, 512 x 8 91/179, 1024 x 4 111/203; 4000 packs 256 x 16 79/180, 512 x 8 86/175,
+// 1024 x 4 87/177; 5000 packs 512 x 12 81/176, 1024 x 6 99/188, reading twice 88/277; 7500 packs 1024 x 12 96/186, reading twice
+// 83/265.  So beyond 6144 packs the log-probabilities stream the row (one read in either form), and the policy loss keeps it
+// up to 16384 packs (215 against 260).  fp32 differs by less and in the same direction.  Returns the number of blocks.
 template <typename T, int MODE>
 static int launch_rows(const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
   const int packs = a.V / Pack<T>::N;
@@ -965,7 +972,8 @@ static int launch_rows(const TokenRows& a, const PolicyIn& p, const RowOut& o, h
   if (packs <= 64) return launch_rows_as<T, 8, 8, MODE>(a, p, o, s);
   if (packs <= 128) return launch_rows_as<T, 16, 8, MODE>(a, p, o, s);
   if (packs <= 256) return launch_rows_as<T, 64, 4, MODE>(a, p, o, s);
-  if (packs <= 512) return launch_rows_as<T, 64, 8, MODE>(a, p, o, s);
+  if (packs <= 768) return launch_rows_as<T, 64, 12, MODE>(a, p, o, s);
+  if (packs <= 1024) return launch_rows_as<T, 64, 16, MODE>(a, p, o, s);
   // half-precision rows some of which start between words (aligned rows would take 13% longer with the check)
   if (sizeof(T) == 2 && ((a.stride & 1) || (reinterpret_cast<uintptr_t>(a.x) & 2))) {
     const int grid = launch_long_rows<T, MODE, sizeof(T) == 2 ? ROW_WORDS : ROW_PLAIN>(packs, a, p, o, s);
