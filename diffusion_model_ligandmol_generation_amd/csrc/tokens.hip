@@ -300,9 +300,11 @@ __device__ __forceinline__ void exponentials(const TokenRows& a, u32x4 (&x)[NV],
     __builtin_amdgcn_sched_barrier(0);
   }
 }
-// Half-precision rows that start between two 32-bit words (odd strides): a pack across word borders comes at three quarters of the
-// rate, so blocks of one row read the words themselves, five a pack, and shift them.  The halves before and behind the pack
-// that come with them lie in words of the row's own ends.  (6006 rows of 32003 bf16: 101 us, 92 so.)
+// Half-precision rows that start between two 32-bit words (odd strides): packs across word borders come slower.  Where many
+// blocks of few lanes hold rows in registers it hardly shows; the kernels that stream long rows go around it: the gradient
+// takes its packs from the second element on, the sums read whole words, five a pack, and shift them (an order of their own
+// would change the result with the stride).  The halves before and behind the pack that come with the words lie in words of
+// the row's own ends.  (preference of 6007 rows of 32003 bf16 281 us without, 261 with them.)
 template <typename T, int TPR> __device__ __forceinline__ bool between_words(const T* row) {
   return sizeof(T) == 2 && TPR >= 256 && uniform((int)reinterpret_cast<uintptr_t>(row) & 2);
 }
@@ -323,12 +325,10 @@ __device__ __forceinline__ void shift_words(u32x4& x, uint32_t last) {
 // Rows that fit the registers of TPR lanes, NV packs a lane: the logits are read once, exponentiated once, and the policy
 // loss writes its gradient from the same registers.  TPR = 8 / 16 / 64: several rows a block and no barrier; 256 / 512 / 1024:
 // one row a block, whose waves take the maximum and sum of their own part and exchange the pair once.
-// FORM: ROW_STAGED writes gradients of ragged short rows through LDS, ROW_WORDS reads rows between words.
-enum { ROW_PLAIN, ROW_STAGED, ROW_WORDS };
-template <typename T, int TPR, int NV, int MODE, int FORM = ROW_PLAIN>
+// STAGE: gradients of ragged short rows are written through LDS.
+template <typename T, int TPR, int NV, int MODE, bool STAGE = false>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)) void k_token_rows(TokenRows a, PolicyIn p, RowOut o) {
   constexpr int N = Pack<T>::N, NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR, NW = TPR / 64, GRP = TPR < 64 ? TPR : 64;
-  constexpr bool STAGE = FORM == ROW_STAGED, WORDS = FORM == ROW_WORDS;
   constexpr bool KEEP = MODE != TK_LOGP && sizeof(T) == 4;   // the exponentials take the logits' registers
   constexpr bool AHEAD = ROW_AHEAD(NV * 4);
   constexpr int STAGE_ROWS = 64 / (TPR < 64 ? TPR : 64), STAGE_V = TPR * NV * N + N;   // (a multiple of a pack)
@@ -355,30 +355,16 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
     if (MODE != TK_LOGP && c.seq < 0) c.id = -1;
     return c;
   };
-  static_assert(!(WORDS && AHEAD), "rows between words are shifted right behind their load");
   const auto load = [&](const RowScalars& c, int64_t t, u32x4 (&x)[NV], float& et, float& xt, float& A, int& len) {
     const T* row = reinterpret_cast<const T*>(a.x) + t * a.stride;
-    uint32_t last[WORDS ? NV : 1];
-    const bool words = WORDS && between_words<T, TPR>(row);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       x[k] = raw_minus_inf<T>();
-      if constexpr (WORDS) {
-        last[k] = x[k][0];
-        if (words) {
-          if (r + k * TPR < nb) x[k] = load_words(row + (int64_t)(r + k * TPR) * N, last[k]);
-          continue;
-        }
-      }
       if (r + k * TPR < nb) x[k] = load_raw(row + (int64_t)(r + k * TPR) * N);
     }
     et = -__builtin_inff();
     if (r < tail) et = (float)row[nb * N + r];
     xt = (float)row[c.id];
-    if constexpr (WORDS)
-      if (words)
-#pragma unroll
-        for (int k = 0; k < NV; ++k) shift_words(x[k], last[k]);
     if constexpr (MODE != TK_LOGP) {
       A = p.adv[p.adv_per_token ? t : (int64_t)c.seq];
       len = !p.per_seq_mean ? 1 : MODE == TK_SMALL ? small_len[t] : p.seq_len[c.seq];
@@ -917,39 +903,28 @@ static int row_grid(int64_t groups, int most) { return (int)(groups < most ? gro
 #define TK_GRID_CAP 2048
 // Rows next to each other that end inside cache lines.
 static bool ragged_lines(int32_t V, int64_t d_stride, size_t size) { return d_stride == V && (V * size) % 128 != 0; }
-template <typename T, int TPR, int NV, int MODE, int FORM = ROW_PLAIN>
+template <typename T, int TPR, int NV, int MODE, bool STAGE = false>
 static int launch_rows_as(const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
   constexpr int NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR;
   const int grid = row_grid((a.n + RPB - 1) / RPB, TK_GRID_CAP * 256 / NT);
-  hipLaunchKernelGGL((k_token_rows<T, TPR, NV, MODE, FORM>), dim3(grid), dim3(NT), 0, s, a, p, o);
+  hipLaunchKernelGGL((k_token_rows<T, TPR, NV, MODE, STAGE>), dim3(grid), dim3(NT), 0, s, a, p, o);
   return grid;
-}
-// Rows of more than 1024 packs, one a block, that fit its registers; 0: too long.
-template <typename T, int MODE, int FORM> static int launch_long_rows(int packs, const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
-  if (packs <= 2048) return launch_rows_as<T, 256, 12, MODE, FORM>(a, p, o, s);
-  if constexpr (MODE == TK_POLICY) {
-    if (packs <= 4096) return launch_rows_as<T, 512, 8, MODE, FORM>(a, p, o, s);
-  } else {
-    if (packs <= 4096) return launch_rows_as<T, 256, 16, MODE, FORM>(a, p, o, s);
-  }
-  if (packs <= 6144) return launch_rows_as<T, 512, 12, MODE, FORM>(a, p, o, s);
-  if constexpr (MODE == TK_POLICY) {
-    if (packs <= 12288) return launch_rows_as<T, 1024, 12, MODE, FORM>(a, p, o, s);
-    if (packs <= 16384) return launch_rows_as<T, 1024, 16, MODE, FORM>(a, p, o, s);
-  }
-  return 0;
 }
 // A batch of at most SMALL_ROWS short rows is one launch of one block: three launches take longer than its two rounds.
 static bool rows_of_8_lanes(int dtype, int32_t V) { return V / (dtype == LIGDIFF_F32 ? 4 : 8) <= 64; }
 // Few lanes with many packs each (up to 16: 64 registers) before more lanes: more lanes wait for each other more often, hold fewer
 // rows under way, have lanes without a pack in their last round, and do the work per row (64-bit log, ratio, KL term) for
-// fewer rows at a time.  Measured, log-probabilities / policy loss with gradient, us.  268 MB of fp32 logits: 32 packs 8 lanes
-// 43/113, 16 lanes 48/124, 64 lanes 154/292; 64 packs 8 lanes 40/111, 16 lanes 42/112; 128 packs 16 lanes 41/110, 64 lanes
-// 49/125.  419 MB of bf16 logits: 300 packs 64 lanes x 12 91/178, 256 x 4 185/330; 1024 packs 64 x 16 82/178, 256 x 4 89/176,
-// 256 x 8 91/172; 2500 packs 256 x 16 85/183, 512 x 8 91/179, 1024 x 4 111/203; 4000 packs 256 x 16 79/180, 512 x 8 86/175,
-// 1024 x 4 87/177; 5000 packs 512 x 12 81/176, 1024 x 6 99/188, reading twice 88/277; 7500 packs 1024 x 12 96/186, reading twice
-// 83/265.  So beyond 6144 packs the log-probabilities stream the row (one read in either form), and the policy loss keeps it
-// up to 16384 packs (215 against 260).  fp32 differs by less and in the same direction.  Returns the number of blocks.
+// fewer rows at a time.  Measured on 419 MB, lanes x packs, log-probabilities / policy loss with gradient, us.
+//   fp32: 24 packs 8x4 77/186, 8x8 93/168; 48 packs 8x8 81/169, 8x16 72, 16x4 74/181; 96 packs 8x16 72/184, 16x8 80/167, 16x12 74/167;
+//     192 packs 16x16 72/182, 16x12 74/169, 64x4 76/186; 1024 packs 64x16 76/171, 256x4 74/169; 2048 packs 256x12 76/168, 1024x4 91/171;
+//     5000 packs 512x12 72/173, 1024x6 83/170, twice read 81/244; 8192 packs 1024x12 78/170, twice read 74/236
+//   bf16: 24 packs 8x4 88/194, 8x8 99/196; 48 packs 8x8 86/174, 8x16 81/181; 96 packs 8x16 76/194, 16x8 85/173, 16x12 80/173, 64x4
+//     137/265; 192 packs 16x16 75/191, 16x12 78/176, 64x4 90/187; 300 packs 64x12 91/178, 256x4 185/330; 1024 packs 64x16 82/178, 256x4
+//     89/176; 2500 packs 256x16 85/183, 512x8 91/179, 1024x4 111/203; 4000 packs 256x16 79/180, 512x8 86/175, 1024x4 87/177;
+//     5000 packs 512x12 81/176, 1024x6 99/188, twice read 88/277; 7500 packs 1024x12 96/186, twice read 83/265; 16384 packs 1024x16
+//     95/215, twice read 84/260
+// So beyond 6144 packs the log-probabilities stream the row (they need one read in either form), and the policy loss keeps it up
+// to 16384 packs.  Returns the number of blocks.
 template <typename T, int MODE>
 static int launch_rows(const TokenRows& a, const PolicyIn& p, const RowOut& o, hipStream_t s) {
   const int packs = a.V / Pack<T>::N;
@@ -962,25 +937,34 @@ static int launch_rows(const TokenRows& a, const PolicyIn& p, const RowOut& o, h
   if constexpr (MODE == TK_POLICY) {
     // (through LDS: 119 fp32 a row 69 us against 86 for 147 MB, 200 fp32 61 against 72, 500 bf16 70 against 76; but 30 fp32 57
     // against 52 and 90 bf16 78 against 74: rows of two lines at most are as well written directly)
+    const bool few = packs <= (sizeof(T) == 4 ? 16 : 24);
     if (packs <= 64 && (size_t)a.V * sizeof(T) > 256 && o.d && ragged_lines(a.V, o.d_stride, sizeof(T))) {
-      if (packs <= 32) return launch_rows_as<T, 8, 4, MODE, ROW_STAGED>(a, p, o, s);
-      return launch_rows_as<T, 8, 8, MODE, ROW_STAGED>(a, p, o, s);
+      if (sizeof(T) == 2 && packs <= 32) return launch_rows_as<T, 8, 4, MODE, true>(a, p, o, s);
+      return launch_rows_as<T, 8, 8, MODE, true>(a, p, o, s);
     }
+    if (packs <= 16) return launch_rows_as<T, 8, 2, MODE>(a, p, o, s);
+    if (few) return launch_rows_as<T, 8, 4, MODE>(a, p, o, s);
+    if (packs <= 64) return launch_rows_as<T, 8, 8, MODE>(a, p, o, s);
+    if (packs <= 192) return launch_rows_as<T, 16, 12, MODE>(a, p, o, s);
+    if (packs <= 256) return launch_rows_as<T, 64, 4, MODE>(a, p, o, s);
+  } else {
+    if (packs <= 16) return launch_rows_as<T, 8, 2, MODE>(a, p, o, s);
+    if (packs <= 32) return launch_rows_as<T, 8, 4, MODE>(a, p, o, s);
+    if (packs <= 128) return launch_rows_as<T, 8, 16, MODE>(a, p, o, s);
+    if (packs <= 256) return launch_rows_as<T, 16, 16, MODE>(a, p, o, s);
   }
-  if (packs <= 16) return launch_rows_as<T, 8, 2, MODE>(a, p, o, s);
-  if (packs <= 32) return launch_rows_as<T, 8, 4, MODE>(a, p, o, s);
-  if (packs <= 64) return launch_rows_as<T, 8, 8, MODE>(a, p, o, s);
-  if (packs <= 128) return launch_rows_as<T, 16, 8, MODE>(a, p, o, s);
-  if (packs <= 256) return launch_rows_as<T, 64, 4, MODE>(a, p, o, s);
   if (packs <= 768) return launch_rows_as<T, 64, 12, MODE>(a, p, o, s);
   if (packs <= 1024) return launch_rows_as<T, 64, 16, MODE>(a, p, o, s);
-  // half-precision rows some of which start between words (aligned rows would take 13% longer with the check)
-  if (sizeof(T) == 2 && ((a.stride & 1) || (reinterpret_cast<uintptr_t>(a.x) & 2))) {
-    const int grid = launch_long_rows<T, MODE, sizeof(T) == 2 ? ROW_WORDS : ROW_PLAIN>(packs, a, p, o, s);
-    if (grid) return grid;
+  if (packs <= 2048) return launch_rows_as<T, 256, 12, MODE>(a, p, o, s);
+  if constexpr (MODE == TK_POLICY) {
+    if (packs <= 4096) return launch_rows_as<T, 512, 8, MODE>(a, p, o, s);
   } else {
-    const int grid = launch_long_rows<T, MODE, ROW_PLAIN>(packs, a, p, o, s);
-    if (grid) return grid;
+    if (packs <= 4096) return launch_rows_as<T, 256, 16, MODE>(a, p, o, s);
+  }
+  if (packs <= 6144) return launch_rows_as<T, 512, 12, MODE>(a, p, o, s);
+  if constexpr (MODE == TK_POLICY) {
+    if (packs <= 12288) return launch_rows_as<T, 1024, 12, MODE>(a, p, o, s);
+    if (packs <= 16384) return launch_rows_as<T, 1024, 16, MODE>(a, p, o, s);
   }
   const int grid = row_grid(a.n, TK_GRID_CAP);
   hipLaunchKernelGGL((k_token_rows_long<T, MODE>), dim3(grid), dim3(1024), 0, s, a, p, o);
