@@ -21,9 +21,9 @@ struct TokenRows {
 // is rounded once.  One constant would do for the exponentials, but its rounding is a temperature that is off by up to 2^-25:
 // the same error 1.3e-8 (z - E[z]) in every log-probability, which sums over a sequence add up (29 atoms: twice the error
 // of the plain form).  Both parts are above 0, so that a masked -inf stays -inf.
+__device__ __forceinline__ float scaled(const TokenRows& a, float d) { return fmaf(d, a.c, d * a.c_lo); }
 __device__ __forceinline__ float exponent(const TokenRows& a, float x, float m) {
-  const float d = x - m;
-  return fmaf(d, a.c, d * a.c_lo);
+  return scaled(a, x - m);
 }
 
 // log(s) of the softmax sum, in 64 bits: losses use differences of log-probabilities of two policies, which are small
@@ -279,6 +279,17 @@ template <int NW> __device__ __forceinline__ void join_waves(const TokenRows& a,
   if (NW >= 8) S += dpp_move<0x141>(S);
   if (NW == 16) S += dpp_move<0x140>(S);
 }
+// The maximum of a pack and m; fp16 in packed instructions.
+template <typename T> __device__ __forceinline__ float max_pack(const u32x4& x, float m) {
+  if constexpr (std::is_same<T, f16_t>::value) {
+    f16x2 v = __builtin_elementwise_max(__builtin_bit_cast(f16x2, (uint32_t)x[0]), __builtin_bit_cast(f16x2, (uint32_t)x[1]));
+    v = __builtin_elementwise_max(v, __builtin_elementwise_max(__builtin_bit_cast(f16x2, (uint32_t)x[2]), __builtin_bit_cast(f16x2, (uint32_t)x[3])));
+    return fmaxf(m, fmaxf((float)v[0], (float)v[1]));
+  }
+#pragma unroll
+  for (int j = 0; j < Pack<T>::N; ++j) m = fmaxf(m, raw_get<T>(x, j));
+  return m;
+}
 // The exponentials of a lane's packs, handed on one pack at a time.  Half-precision packs stay packed until then (the compiler
 // would keep the values that it unpacked for the maximum, twice the registers): the policy loss exponentiates them a second
 // time for its gradient rather than hold 32-bit results, which halves the rows in flight.
@@ -289,13 +300,15 @@ __device__ __forceinline__ void set_pack(u32x4& x, const float (&v)[4]) {
 template <typename T, int NV, int TPR, typename F>
 __device__ __forceinline__ void exponentials(const TokenRows& a, u32x4 (&x)[NV], int nb, float m, F&& take) {
   constexpr int N = Pack<T>::N;
+  float one = 1.f;   // (not known to the compiler: fp16 converts and subtracts in one instruction, a mixed fma)
+  if (std::is_same<T, f16_t>::value) asm volatile("" : "+s"(one));
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     if (k > 0 && k * TPR >= nb) break;   // no lane has a pack here
     if (sizeof(T) == 2) asm volatile("" : "+v"(x[k]));
     float e[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) e[j] = __builtin_amdgcn_exp2f(exponent(a, raw_get<T>(x[k], j), m));
+    for (int j = 0; j < N; ++j) e[j] = __builtin_amdgcn_exp2f(scaled(a, std::is_same<T, f16_t>::value ? fmaf(raw_get<T>(x[k], j), one, -m) : raw_get<T>(x[k], j) - m));
     take(k, e);
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -411,8 +424,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if (k > 0 && k * TPR >= nb) break;
-#pragma unroll
-      for (int j = 0; j < N; ++j) m = fmaxf(m, raw_get<T>(x[k], j));
+      m = max_pack<T>(x[k], m);
     }
     m = group_max<GRP>(m);
     // this wave's own part, relative to its own maximum
