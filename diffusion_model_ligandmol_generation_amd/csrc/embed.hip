@@ -10,7 +10,8 @@
 #include <algorithm>
 
 // ------------------------------------------------------------------ lookup
-// TPR lanes a row, four rows in flight per group: the token, then the row, then the store are dependent accesses.
+// TPR lanes a row, four rows in flight per group: the token, then the row, then the store are dependent accesses.  29696 rows of
+// 256 fp32 8.5 us, 65536 rows of 1024 bf16 of a table of 32000 33-44 us (the table in the last-level cache or not).
 template <typename T, int TPR>
 __global__ __launch_bounds__(256) void k_embed(const T* __restrict__ table, int64_t row_stride, TokenView tok, int64_t n, int32_t D,
                                                float scale, T* __restrict__ out, int64_t out_stride) {
@@ -82,6 +83,7 @@ extern "C" int ligdiff_embed(const void* table, int32_t dtype, int64_t n_rows, i
 }
 
 // ------------------------------------------------------------------ stable radix sort of the positions by token
+// Bound by latency: 65536 positions take 22 us in two passes of two launches, 4096 or fewer about 7 us in one launch.
 #define SORT_NT 512
 #define SORT_WAVES (SORT_NT / 64)
 struct SortPass {
@@ -331,6 +333,7 @@ template <typename TO, int N> __device__ __forceinline__ void put_columns(TO* p,
 // of tokens that do not occur.  The other blocks: SUM_WAVES chunks of R sorted positions and 64 packs of columns, a wave a chunk.  A wave
 // writes the tokens that lie inside its chunk; the first and the last, which may go on in the neighbours', meet in LDS, and
 // only what goes on beyond the block's chunks leaves it as a partial row: slot 0 the block's first token, slot 1 its last.
+// 65536 rows of 1024 bf16 in random order, table of 32000: 49 us, 4.1 TB/s.
 template <typename T, typename TO>
 __global__ __launch_bounds__(SUM_WAVES * 64) void k_segment_sums(SegIn a) {
   constexpr int N = Pack<T>::N, U = 8, NT = SUM_WAVES * 64;
