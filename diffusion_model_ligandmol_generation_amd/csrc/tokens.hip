@@ -61,7 +61,7 @@ __device__ __forceinline__ void kl_terms(float q, float& em1, float& kl) {
     em1 = q + kl;
   } else {
     em1 = expf(q) - 1.0f;
-    kl = em1 - q;
+    kl = em1 < __builtin_inff() ? em1 - q : em1;   // (q = inf: infinite, and NaN stays NaN)
   }
 }
 
@@ -93,8 +93,7 @@ struct RowOut {
   int64_t d_stride;
 };
 
-// What a row contributes once its maximum M and sum S are known, the same in every lane of the row; returns the gradient's
-// factor d loss / d logp * grad_scale / temperature.
+// What is known of a row besides its logits; loaded one row ahead, so that a row costs one memory latency.
 struct RowScalars { int id, seq; float old, ref; };
 // A value that all lanes of the wave share, in a scalar register.
 __device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
@@ -116,6 +115,8 @@ template <int MODE> __device__ __forceinline__ RowScalars row_scalars(const Toke
   return r;
 }
 
+// What a row contributes once its maximum M and sum S are known, the same in every lane of the row; returns the gradient's
+// factor d loss / d logp * grad_scale / temperature.
 template <int MODE>
 __device__ __forceinline__ float row_epilogue(const TokenRows& a, const PolicyIn& p, const RowOut& o, int64_t t, const RowScalars& c,
                                               float xt, float M, float S, float inv_s, bool writer, float A, double w, double* acc) {
@@ -132,7 +133,7 @@ __device__ __forceinline__ float row_epilogue(const TokenRows& a, const PolicyIn
     float em1 = 0.f, kl = 0.f;
     if (p.ref_logp) {
       kl_terms((float)((double)c.ref - lp), em1, kl);
-      slope -= p.kl_coef * em1;
+      if (p.kl_coef != 0.f) slope -= p.kl_coef * em1;   // (an infinite term that does not count reaches nothing)
     }
     if (rho != rho) slope = rho;   // fminf drops a NaN
     if (writer) {
@@ -239,7 +240,7 @@ template <int RPB> __device__ __forceinline__ void policy_result(const PolicyIn&
     for (int g = 0; g < RPB; ++g)
 #pragma unroll
       for (int k = 0; k < 3; ++k) v[k] += acc[g][k];
-    p.result[0] = (float)(v[0] + (double)p.kl_coef * v[1]);
+    p.result[0] = (float)(p.kl_coef != 0.f ? v[0] + (double)p.kl_coef * v[1] : v[0]);
     p.result[1] = (float)v[0];
     p.result[2] = (float)v[1];
     p.result[3] = (float)v[2];
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(256) void k_policy_final(const double* __restrict__
 #pragma unroll
   for (int k = 0; k < 3; ++k) v[k] = block_sum<256>(v[k], red);
   if (threadIdx.x == 0) {
-    result[0] = (float)(v[0] + kl_coef * v[1]);
+    result[0] = (float)(kl_coef != 0.0 ? v[0] + kl_coef * v[1] : v[0]);
     result[1] = (float)v[0];
     result[2] = (float)v[1];
     result[3] = (float)v[2];

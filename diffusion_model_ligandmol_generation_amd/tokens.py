@@ -17,6 +17,7 @@ from collections import namedtuple
 from functools import lru_cache
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import PolicyArgs, PreferenceArgs, TokenArgs, check
@@ -150,6 +151,7 @@ class _EmbedTokens(torch.autograd.Function):
         return _embed(tokens, table, scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_out):
         return None, embed_tokens_grad(d_out, ctx.saved_tensors[0], ctx.rows, ctx.scale), None
 
@@ -243,6 +245,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return logp
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         logits, tokens, stats = ctx.saved_tensors
         return _logprob_grad(logits, tokens, ctx.temperature, stats, g.float().contiguous()), None, None
@@ -307,6 +310,7 @@ class _PreferenceLoss(torch.autograd.Function):
         return loss, log_ratio, margin
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g, *_):
         logits, tokens, slope, stats, row_seq = ctx.saved_tensors
         return _logprob_grad(logits, tokens, ctx.temperature, stats, slope, row_seq, g.float().contiguous()), None, None, None, None
@@ -384,6 +388,7 @@ class _PolicyLoss(torch.autograd.Function):
         return loss, rest, logp
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g, *_):
         logits, tokens, stats, coef = ctx.saved_tensors
         return (_logprob_grad(logits, tokens, ctx.temperature, stats, coef, None, g.float().contiguous()),) + (None,) * 6

@@ -675,6 +675,35 @@ def test_two_backwards_of_one_graph(tk):
         loss.backward()
 
 
+def test_no_second_derivative(tk):
+    """Second derivatives are refused, not silently left out."""
+    g = gen(22)
+    x = torch.randn(64, 119, device="cuda", generator=g, requires_grad=True)
+    table = torch.randn(119, 16, device="cuda", generator=g, requires_grad=True)
+    ids, ptr, adv = ids_of(64, 119, g), cuts(64, 4, g), torch.ones(4, device="cuda")
+    for leaf, loss in ((x, tk.policy_loss(x, ids, ptr, adv).loss), (x, tk.preference_loss(x, ids, ptr).loss),
+                       (x, tk.token_logprobs(x, ids).square().sum()), (table, tk.embed_tokens(ids, table).square().sum())):
+        first, = torch.autograd.grad(loss, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+            first.sum().backward()
+
+
+@pytest.mark.parametrize("T", [40, 200])
+def test_infinite_kl_without_weight(tk, T):
+    """kl_coef 0 with a reference: the term is returned, and an infinite one reaches neither loss nor gradient."""
+    g = gen(23)
+    x, ids = torch.randn(T, 119, device="cuda", generator=g), ids_of(T, 119, g)
+    ids[7] = 3
+    x[7, 3] = float("-inf")                   # chosen under an older policy, masked now
+    old = torch.full((T,), -4.8, device="cuda")
+    ref = -4.8 + 0.1 * torch.randn(T, device="cuda", generator=g)
+    adv = torch.randn(T, device="cuda", generator=g)
+    with_ref = tk.policy_loss_and_grad(x, ids, None, adv, old, ref, "token", kl_coef=0.0)
+    without = tk.policy_loss_and_grad(x, ids, None, adv, old, None, "token", kl_coef=0.0)
+    assert with_ref.kl == float("inf") and with_ref.loss.isfinite() and with_ref.d_logits.isfinite().all()
+    assert torch.equal(with_ref.loss, without.loss) and torch.equal(with_ref.d_logits, without.d_logits)
+
+
 def test_captured_and_replayed(tk):
     """All operators in one graph, replayed on new inputs with eager work in between: every replay has the eager bits."""
     g = gen(11)
