@@ -704,6 +704,28 @@ def test_infinite_kl_without_weight(tk, T):
     assert torch.equal(with_ref.loss, without.loss) and torch.equal(with_ref.d_logits, without.d_logits)
 
 
+def test_offsets_past_32_bits(tk):
+    """Rows 2^25 elements apart: the last ones lie past 2^32 elements and bytes, of logits, tables and their gradients."""
+    g = gen(24)
+    T, V = 140, 119
+    buf = torch.empty(T << 25, dtype=torch.bfloat16, device="cuda")
+    x = buf.view(T, 1 << 25)[:, 5:5 + V]
+    x.copy_(torch.randn(T, V, device="cuda", generator=g))
+    ids, ptr, adv = ids_of(T, V, g), cuts(T, 6, g), torch.randn(6, device="cuda", generator=g)
+    near = x.contiguous()
+    assert torch.equal(tk.token_logprobs(x, ids), tk.token_logprobs(near, ids))
+    for f in (lambda y: tk.policy_loss_and_grad(y, ids, ptr, adv, kl_coef=0.0), lambda y: tk.preference_loss_and_grad(y, ids, ptr)):
+        assert all(torch.equal(a, b) for a, b in zip(f(x), f(near)))
+    tokens = torch.randint(0, T, (500,), device="cuda", generator=g)
+    tokens[:2] = T - 1
+    assert torch.equal(tk.embed_tokens(tokens, x, 0.5), tk.embed_tokens(tokens, near, 0.5))
+    assert torch.equal(tk.embed_tokens_grad(x, ids, V), tk.embed_tokens_grad(near, ids, V))
+    up = torch.randn(500, V, device="cuda", generator=g).bfloat16()
+    want = tk.embed_tokens_grad(up, tokens, T)
+    tk.embed_tokens_grad(up, tokens, T, out=x)
+    assert torch.equal(x, want)
+
+
 def test_captured_and_replayed(tk):
     """All operators in one graph, replayed on new inputs with eager work in between: every replay has the eager bits."""
     g = gen(11)
