@@ -726,6 +726,23 @@ def test_offsets_past_32_bits(tk):
     assert torch.equal(x, want)
 
 
+def test_shares_of_two_ranks(tk):
+    """Two halves of a batch with the whole batch's counts as denominators: losses add up, gradients are the whole one's
+    (factors that are rounded once more or less: 4 u)."""
+    g = gen(25)
+    T, V, S = 2000, 119, 40
+    x, ids, adv = torch.randn(T, V, device="cuda", generator=g), ids_of(T, V, g, 0.1), torch.randn(S, device="cuda", generator=g)
+    ptr, old = torch.arange(0, T + 1, 50, device="cuda"), -4.8 + 0.2 * torch.randn(T, device="cuda", generator=g)
+    n = int(((ids >= 0) & (ids < V)).sum())
+    for aggregate, total in (("token", n), ("sequence", S)):
+        whole = tk.policy_loss_and_grad(x, ids, ptr, adv, old, old, kl_coef=0.1, aggregate=aggregate)
+        parts = [tk.policy_loss_and_grad(x[a:a + 1000], ids[a:a + 1000], ptr[:21], adv[a // 50:a // 50 + 20], old[a:a + 1000],
+                                         old[a:a + 1000], kl_coef=0.1, aggregate=aggregate, denominator=total) for a in (0, 1000)]
+        within(parts[0].loss + parts[1].loss, whole.loss.double(), 4 * U * (parts[0].loss.abs() + parts[1].loss.abs()).double(), "loss")
+        want = whole.d_logits.double()
+        within(torch.cat([p.d_logits for p in parts]), want, 4 * U * want.abs(), "d_logits")
+
+
 def test_captured_and_replayed(tk):
     """All operators in one graph, replayed on new inputs with eager work in between: every replay has the eager bits."""
     g = gen(11)

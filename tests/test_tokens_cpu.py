@@ -130,3 +130,36 @@ def test_no_cpu_path():
                  lambda: tk.token_logprobs(x.requires_grad_(), ids)):
         with pytest.raises(RuntimeError, match="HIP device"):
             call()
+
+
+def _count_worker(rank, world, port, q):
+    import os
+    import torch.distributed as dist
+    from types import SimpleNamespace
+    from diffusion_model_ligandmol_generation_amd.train import ResearchAccurateTrainer
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    me = SimpleNamespace(group=dist.group.WORLD, count_group=dist.group.WORLD)
+    q.put(ResearchAccurateTrainer._sum_over_ranks(me, 10 ** 9 + rank, 3 - rank))
+    dist.destroy_process_group()
+
+
+def test_counts_over_ranks():
+    """The denominators of the fine-tuning steps are the counts of all ranks (two gloo processes)."""
+    import socket
+    from types import SimpleNamespace
+    import torch.multiprocessing as mp
+    from diffusion_model_ligandmol_generation_amd.train import ResearchAccurateTrainer
+    assert ResearchAccurateTrainer._sum_over_ranks(SimpleNamespace(group=None), 7) == (7,)
+    with socket.socket() as sock:
+        sock.bind(("127.0.0.1", 0))
+        port = sock.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_count_worker, args=(r, 2, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = [q.get(timeout=120) for _ in procs]
+    for p in procs:
+        p.join(60)
+    assert got == [(2 * 10 ** 9 + 1, 5)] * 2 and all(p.exitcode == 0 for p in procs)
