@@ -315,10 +315,10 @@ __device__ __forceinline__ void exponentials(const TokenRows& a, u32x4 (&x)[NV],
   }
 }
 // Half-precision rows that start between two 32-bit words (odd strides): packs across word borders come slower.  Where many
-// blocks of few lanes hold rows in registers it hardly shows; the kernels that stream long rows go around it: the gradient
-// takes its packs from the second element on, the sums read whole words, five a pack, and shift them (an order of their own
-// would change the result with the stride).  The halves before and behind the pack that come with the words lie in words of
-// the row's own ends.  (The gradient of 6007 rows of 32003 bf16 137 us, 147 across the borders.)
+// blocks of few lanes hold rows in registers it shows less (rows of 32003 bf16 127 us, of 32004 115); the kernel that streams
+// longer rows reads whole words, five a pack, and shifts them (another partition of the row would be another order of its sum,
+// which would then change with the stride).  The halves before and behind the pack that come with the words lie in words of
+// the row's own ends.  (Log-probabilities of 1601 rows of 120001 bf16 94 us without, 86 with them.)
 template <typename T, int TPR> __device__ __forceinline__ bool between_words(const T* row) {
   return sizeof(T) == 2 && TPR >= 256 && uniform((int)reinterpret_cast<uintptr_t>(row) & 2);
 }
@@ -508,11 +508,13 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)
 template <typename T, int TPR>
 __device__ __forceinline__ void row_gradient(const TokenRows& a, const T* row, T* d, int id, int r, float M, float inv_s, float g) {
   constexpr int N = Pack<T>::N;
-  // rows between words: packs from the second element on, the first goes to lane 0 beside the tail
-  const int shift = between_words<T, TPR>(row), V = a.V, nb = (V - shift) / N, tail = V - nb * N;
+  // long rows: packs from the first cache line of the gradient on, which a wave then writes whole; the elements before and
+  // behind them go to a lane each (preference of 6007 rows of 32003 bf16 284 -> 276 us, 20000 of 8201 fp32 415 -> 403)
+  const int V = a.V, head = TPR >= 256 ? uniform((int)(-reinterpret_cast<uintptr_t>(d) & 127) / (int)sizeof(T)) : 0;
+  const int shift = head < V ? head : V, nb = (V - shift) / N, edges = V - nb * N;
   const bool off = g == 0.f || inv_s == 0.f;
   const float q = -g * inv_s;
-  const int at = id - shift, it = at / N;   // (-1 is in no pack)
+  const int at = id - shift, it = at < 0 ? -1 : at / N;   // (an element before the packs is in none)
   if (off) {
     row_zero(d, V, r, TPR);
     return;
@@ -529,8 +531,8 @@ __device__ __forceinline__ void row_gradient(const TokenRows& a, const T* row, T
     }
     store_pack(d + shift + (int64_t)i * N, v);
   }
-  if (r < tail) {
-    const int v = shift && r == 0 ? 0 : nb * N + r;
+  if (r < edges) {
+    const int v = r < shift ? r : nb * N + r;
     const float x = (float)row[v];
     d[v] = (T)(q * __builtin_amdgcn_exp2f(exponent(a, x, M)) + (v == id ? g : 0.f));
   }
