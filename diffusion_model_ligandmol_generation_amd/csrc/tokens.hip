@@ -334,14 +334,14 @@ __device__ __forceinline__ void shift_words(u32x4& x, uint32_t last) {
 // Short rows are loaded one row ahead of their arithmetic: a wave has two rows' bytes under way.
 #define ROW_AHEAD(REGS) ((REGS) <= 8)
 // Waves a SIMD holds at once: what the registers of a row allow.
-#define ROW_WAVES(TPR, REGS, MODE) ((MODE) == TK_LOGP ? ((REGS) <= 16 ? 8 : (REGS) <= 32 ? 6 : 4) : (TPR) == 1024 ? ((REGS) <= 16 ? 8 : 4) : (REGS) <= 8 ? 6 : (REGS) <= 16 ? 5 : 4)
+#define ROW_WAVES(REGS, MODE) ((REGS) > 16 ? 4 : (MODE) == TK_LOGP ? 8 : (REGS) <= 8 ? 6 : 5)
 
 // Rows that fit the registers of TPR lanes, NV packs a lane: the logits are read once, exponentiated once, and the policy
 // loss writes its gradient from the same registers.  TPR = 8 / 16 / 64: several rows a block and no barrier; 256 / 512 / 1024:
 // one row a block, whose waves take the maximum and sum of their own part and exchange the pair once.
 // STAGE: gradients of ragged short rows are written through LDS.
 template <typename T, int TPR, int NV, int MODE, bool STAGE = false>
-__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(TPR, NV * 4, MODE)) void k_token_rows(TokenRows a, PolicyIn p, RowOut o) {
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(NV * 4, MODE)) void k_token_rows(TokenRows a, PolicyIn p, RowOut o) {
   constexpr int N = Pack<T>::N, NT = TPR <= 64 ? 256 : TPR, RPB = NT / TPR, NW = TPR / 64, GRP = TPR < 64 ? TPR : 64;
   constexpr bool KEEP = MODE != TK_LOGP && sizeof(T) == 4;   // the exponentials take the logits' registers
   constexpr bool AHEAD = ROW_AHEAD(NV * 4);
