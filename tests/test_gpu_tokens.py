@@ -560,6 +560,31 @@ def test_policy_borders(tk, dtype, T, V):
         within(got.d_logits, want["d"] * scale, slack, "d_logits")
 
 
+# one pack on either side of every border between numbers of lanes and packs a lane
+PACKS = [24, 25, 33, 129, 192, 193, 257, 769, 1024, 1025, 2048, 2049, 4096, 4097, 6144, 6145, 12288, 12289, 16384, 16385]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("packs", PACKS)
+def test_rows_at_borders(tk, dtype, packs):
+    V = packs * (4 if dtype == "fp32" else 8) + 1          # and one element behind the packs
+    T = 300 if packs < 600 else 9
+    case = (T, V, 4, False, True, True, 0.2, 0.2, 0.1, "sequence", 1.0, None, True)
+    x, ids, ptr, adv, old, ref = policy_inputs(case, dtype)
+    scale = 64.0 if dtype == "fp16" else 1.0
+    off = LOGP + max(0, V / 1024 - 64) * U                 # (a lane of the longest rows adds up more than 64 terms)
+    want = policy_oracle(x, ids, ptr, adv, False, old, ref, 0.2, 0.2, 0.1, "sequence", 1.0, None)
+    slack = policy_slack(want, scale, 1.0) * (off / LOGP)
+    for y in (x, strided(x, 3, 1)[0]):
+        within(tk.token_logprobs(y, ids), logp_oracle(x, ids)[0], off, "log-probabilities")
+        got = tk.policy_loss_and_grad(y, ids, ptr, adv, old, ref, "sequence", 0.2, 0.2, 0.1, "sequence", 1.0, None, scale)
+        within(got.logp[want["on"]], want["logp"][want["on"]], off, "logp")
+        within(got.d_logits, want["d"] * scale, slack, "d_logits")
+        leaf = y.detach().requires_grad_()
+        (tk.policy_loss(leaf, ids, ptr, adv, old, ref, "sequence", 0.2, 0.2, 0.1, "sequence").loss * scale).backward()
+        within(leaf.grad, want["d"] * scale, slack, "autograd")
+
+
 @pytest.mark.parametrize("T,P", [(1023, 1024), (1024, 1024), (1024, 1025), (1025, 1), (1025, 1025), (3000, 1500), (64, 32), (65, 32)])
 def test_preference_borders(tk, T, P):
     """One chunk of rows and up to 1024 pairs go in fewer launches: the same formula on both sides."""
