@@ -845,11 +845,12 @@ __device__ __forceinline__ double pair_loss(const PrefIn& a, int64_t pr, double 
   const double ratio0 = sum0 * share0, ratio1 = sum1 * share1, gap = ratio0 - ratio1;
   double loss, slope;
   if (a.kind == LIGDIFF_PREFERENCE_SIGMOID) {
-    // -(1 - e) log sigmoid(z) - e log sigmoid(-z) = log(1 + exp(-z)) + e z
-    const double z = (double)a.beta * gap, x = exp(-fabs(z));
-    loss = log1p(x) + (z < 0.0 ? -z : 0.0) + (double)a.smooth * z;
+    // -(1 - e) log sigmoid(z) - e log sigmoid(-z) = log(1 + exp(-|z|)) + (z < 0 ? -(1 - e) z : e z).  The margin may be infinite
+    // (a chosen id without probability): then x = 0 and the other term is the loss, 0 for z = inf and e = 0, else inf.
+    const double z = (double)a.beta * gap, e = (double)a.smooth, x = exp(-fabs(z));
+    loss = log1p(x) + (z < 0.0 ? -(1.0 - e) * z : e != 0.0 ? e * z : 0.0);
     const double sig = z >= 0.0 ? 1.0 / (1.0 + x) : x / (1.0 + x);
-    slope = (double)a.beta * (sig - 1.0 + (double)a.smooth);
+    slope = (double)a.beta * (sig - 1.0 + e);
   } else {
     const double z = gap - 0.5 / (double)a.beta;
     loss = z * z;

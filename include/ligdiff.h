@@ -642,7 +642,8 @@ int ligdiff_token_logprob_grad(const ligdiff_token_args* args, const float* stat
  *   sigmoid: -(1 - e) log sigmoid(beta d) - e log sigmoid(-beta d)  (e = label_smoothing);  ipo: (d - 1 / (2 beta))^2
  *   loss = sum over pairs / denominator
  * seq_ptr [2 n_pairs + 1] int32, ascending, first position of each sequence (mol_ptr of a packed batch); a sequence may
- * be empty (r = 0); positions outside every sequence take no part. */
+ * be empty (r = 0); positions outside every sequence take no part.  A chosen id without probability makes its margin
+ * infinite: the sigmoid loss of the pair is then 0 (d = inf, e = 0) or inf, its gradient is finite. */
 enum ligdiff_preference_kind { LIGDIFF_PREFERENCE_SIGMOID = 0, LIGDIFF_PREFERENCE_IPO = 1 };
 typedef struct ligdiff_preference_args {
   const int32_t* seq_ptr;

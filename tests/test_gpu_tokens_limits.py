@@ -1,0 +1,75 @@
+"""GPU: the token operators where a value has no bound or a size has no room: infinite margins of the
+preference loss.  Against plain 64-bit forms; the tolerances of single values are
+those of test_gpu_tokens.py (U half a step of fp32, LOGP the error of a log-probability)."""
+import pytest
+import torch
+
+from test_gpu_tokens import LOGP, U, gen, ids_of, logp_oracle, owner_of, seq_sum, tk, within  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ infinite margins
+# (up to 1024 rows and pairs one block computes the loss, beyond that several)
+@pytest.mark.parametrize("T,P", [(64, 8), (1024, 30), (1025, 30), (5000, 1100)])
+@pytest.mark.parametrize("e", [0.0, 0.1])
+@pytest.mark.parametrize("side", ["preferred", "other", "both", "neither"])
+def test_infinite_margins(tk, T, P, e, side):
+    """A chosen id whose logit is -inf has log-probability -inf.  In the sequence that is not preferred it makes the margin +inf:
+    the pair's loss is 0 without label smoothing and inf with it; in the preferred one -inf, and the loss is inf.  The
+    gradient is finite: its factor beta (sigmoid(z) - 1 + e) is."""
+    g = gen(T + P)
+    beta = 0.3
+    ptr = torch.linspace(0, T, 2 * P + 1, device="cuda").long().int()
+    x, ids = torch.randn(T, 119, device="cuda", generator=g), ids_of(T, 119, g)
+    owner = owner_of(ptr, T)
+    mask = lambda s: (owner == s).nonzero()[0, 0]   # noqa: E731  (the sequence's first row)
+    if side in ("other", "both"):
+        t = mask(P + 3)
+        x[t, ids[t]] = float("-inf")
+    if side in ("preferred", "both"):
+        t = mask(5)
+        x[t, ids[t]] = float("-inf")
+    lp, p, _ = logp_oracle(x, ids)
+    r = seq_sum(lp, owner, 2 * P)
+    z = beta * (r[:P] - r[P:])
+    sp = torch.nn.functional.softplus
+    each = (1 - e) * sp(-z) + (e * sp(z) if e else 0.0)
+    want = each.mean()
+    assert want.isinf() == (side in ("preferred", "both") or (side == "other" and e > 0)) and not want.isnan()
+    n = torch.bincount(owner, minlength=2 * P).double()
+    slack = beta * ((n + 1) * (LOGP + U)).sum() / P
+    got = tk.preference_loss_and_grad(x, ids, ptr, beta=beta, label_smoothing=e)
+    within(got.loss, want, slack if want.isfinite() else 0.0, "loss")
+    assert got.d_logits.isfinite().all()
+    coef = beta * (torch.sigmoid(z) - 1 + e) / P
+    if side in ("other", "both"):
+        assert got.margin[3] == float("inf") and coef[3] == beta * e / P
+        if e == 0:
+            assert not got.d_logits[owner == 3].any() and not got.d_logits[owner == P + 3].any()
+    if side in ("preferred", "both"):
+        assert got.margin[5] == float("-inf")
+        rows = owner == 5
+        d = -p[rows]
+        d[torch.arange(int(rows.sum()), device="cuda"), ids[rows]] += 1
+        d *= coef[5]
+        within(got.d_logits[rows], d, 3 * LOGP * beta / P * (p[rows] + 1e-3) + 4 * U * d.abs(), "d_logits")
+    leaf = x.clone().requires_grad_()
+    loss = tk.preference_loss(leaf, ids, ptr, beta=beta, label_smoothing=e).loss
+    assert torch.equal(loss, got.loss)
+    loss.backward()
+    within(leaf.grad, got.d_logits.double(), 4 * U * got.d_logits.abs().double(), "autograd")
+
+
+def test_nan_margin_is_the_loss(tk):
+    """NaN in a sequence, and -inf on both sides of a pair, leave the pair's loss undefined: NaN."""
+    x, ids = torch.zeros(8, 9, device="cuda"), torch.zeros(8, dtype=torch.int64, device="cuda")
+    ptr = torch.tensor([0, 2, 4, 6, 8], device="cuda")
+    for bad in ("nan", "inf - inf"):
+        y = x.clone()
+        if bad == "nan":
+            y[1, 5] = float("nan")
+        else:
+            y[1, 0] = y[5, 0] = float("-inf")
+        for e in (0.0, 0.2):
+            assert tk.preference_loss(y, ids, ptr, label_smoothing=e).loss.isnan()
