@@ -268,12 +268,29 @@ class ResearchAccurateTrainer:
             logits, _ = self._atom_type_logits(model, batch, draws)
             return token_logprobs(logits, self._atom_types(batch, self.device), temperature), draws
 
-    def _fine_tune_update(self, logits, result):
-        """Backward pass from the gradient of the logits, gradient sum over the ranks, clipping and optimiser step."""
+    @staticmethod
+    def _check_rate(lr):
+        if lr is not None and not 0.0 <= float(lr) < float("inf"):
+            raise ValueError("lr must be a finite number, at least 0")
+
+    def _fine_tune_update(self, logits, result, lr):
+        """Backward pass from the gradient of the logits, gradient sum over the ranks, clipping and optimiser step at rate
+        ``lr`` (None: see ``preference_step``)."""
         self.optimizer.zero_grad()
         logits.backward(result.d_logits)
         self._allreduce_gradients()
-        self.optimizer.clip_and_step(self.model, max_norm=1.0)
+        groups = self.optimizer.param_groups
+        rates = [g["lr"] for g in groups]
+        try:
+            for g in groups:
+                if lr is not None:
+                    g["lr"] = float(lr)
+                elif g["lr"] == 0:      # the schedule of train_research_validated counts epochs and starts at 0
+                    g["lr"] = g.get("initial_lr", g["lr"])
+            self.optimizer.clip_and_step(self.model, max_norm=1.0)
+        finally:
+            for g, rate in zip(groups, rates):
+                g["lr"] = rate
         self.step_count += 1
 
     def _sum_over_ranks(self, *values):
@@ -286,28 +303,33 @@ class ResearchAccurateTrainer:
         return tuple(t.tolist())
 
     def preference_step(self, batch, draws, ref_logp=None, beta=0.1, label_smoothing=0.0, kind="sigmoid", average=False,
-                        temperature=1.0):
+                        temperature=1.0, lr=None):
         """One optimiser step on pairs of ligands: of the 2 P molecules of the batch, number p is preferred over number
         P + p (``tokens.preference_loss`` on ``atom_pred`` and ``batch.atom_types``).  ``draws`` and ``ref_logp`` come from
         ``atom_type_logprobs(batch, model=reference)``.  Under data parallelism each rank brings its own pairs and the
-        loss is the mean over all of them.  Returns tokens.PreferenceGrad (this rank's share of the loss)."""
+        loss is the mean over all of them.  ``lr``: the step's learning rate; None: the optimiser's, or, where the epoch
+        schedule holds that at 0 (before the first epoch), the one the trainer was built with.  Returns tokens.PreferenceGrad
+        (this rank's share of the loss)."""
         from .tokens import preference_loss_and_grad
+        self._check_rate(lr)
         types = self._atom_types(batch, self.device)
         draws = self._fine_tune_draws(batch, draws)
         logits, graph = self._atom_type_logits(self.model, batch, draws)
         pairs, = self._sum_over_ranks(graph.n_mols // 2)
         r = preference_loss_and_grad(logits, types, graph.mol_ptr, ref_logp, beta, label_smoothing, kind, average, temperature,
                                      denominator=pairs if self.group is not None else None)
-        self._fine_tune_update(logits, r)
+        self._fine_tune_update(logits, r, lr)
         return r
 
     def policy_step(self, batch, draws, advantage, old_logp=None, ref_logp=None, advantage_per="sequence", clip_low=0.2,
-                    clip_high=0.2, kl_coef=0.0, aggregate="token", temperature=1.0):
+                    clip_high=0.2, kl_coef=0.0, aggregate="token", temperature=1.0, lr=None):
         """One optimiser step on rewards (``tokens.policy_loss`` on ``atom_pred`` and ``batch.atom_types``): ``advantage`` has
         one value for each molecule (or atom), ``old_logp`` are the log-probabilities under the policy that chose the
         types, ``ref_logp`` those under the reference, both from ``atom_type_logprobs`` with the same ``draws``.  Under data
-        parallelism the mean goes over all ranks' atoms / molecules.  Returns tokens.PolicyGrad (this rank's share)."""
+        parallelism the mean goes over all ranks' atoms / molecules.  ``lr`` as in ``preference_step``.  Returns
+        tokens.PolicyGrad (this rank's share)."""
         from .tokens import policy_loss_and_grad
+        self._check_rate(lr)
         types = self._atom_types(batch, self.device)
         draws = self._fine_tune_draws(batch, draws)
         logits, graph = self._atom_type_logits(self.model, batch, draws)
@@ -317,7 +339,7 @@ class ResearchAccurateTrainer:
             denominator, = self._sum_over_ranks(own)
         r = policy_loss_and_grad(logits, types, graph.mol_ptr, advantage, old_logp, ref_logp, advantage_per, clip_low, clip_high,
                                  kl_coef, aggregate, temperature, denominator=denominator)
-        self._fine_tune_update(logits, r)
+        self._fine_tune_update(logits, r, lr)
         return r
 
     # ------------------------------------------------------------------ optimisation step

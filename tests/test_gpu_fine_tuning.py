@@ -1,0 +1,55 @@
+"""GPU: the trainer's fine-tuning steps as a program uses them: a trainer as it is built, its learning rate."""
+import pytest
+import torch
+
+from test_gpu_atom_types import fine_tune_batch, model_of, trainer_of
+
+pytestmark = pytest.mark.gpu
+
+SIZES = [9, 14, 20, 29]
+
+
+def weights(tr):
+    return {n: p.detach().clone() for n, p in tr.model.named_parameters()}
+
+
+def largest_move(tr, before):
+    return max(float((p.detach() - before[n]).abs().max()) for n, p in tr.model.named_parameters())
+
+
+def steps_of(tr, d, draws, logp, **kw):
+    adv = torch.tensor([1.0, -0.5, 0.2, -0.7], device="cuda")
+    return (lambda: tr.policy_step(d, draws, adv, logp, logp, kl_coef=0.05, **kw), lambda: tr.preference_step(d, draws, logp, **kw))
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_new_trainer_learns(which):
+    """A trainer as it is built: its epoch schedule starts at 0, a fine-tuning step takes the rate it was built with.  AdamW's
+    first step moves a weight by the rate at most (and the decay, 1e-5 of it per unit of weight), and most by nearly that."""
+    d = fine_tune_batch(SIZES, 8)
+    tr = trainer_of(model_of(), lr=3e-4)
+    logp, draws = tr.atom_type_logprobs(d)
+    before = weights(tr)
+    steps_of(tr, d, draws, logp)[which]()
+    assert 0.9 * 3e-4 <= largest_move(tr, before) <= 1.01 * 3e-4
+    assert tr.optimizer.param_groups[0]["lr"] == 0.0 and tr.step_count == 1      # the epoch schedule goes on as it was
+    assert tr.optimizer.last_path == "fused"
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_learning_rates(which):
+    d = fine_tune_batch(SIZES, 9)
+    for given, scheduled, want in ((1e-3, None, 1e-3), (None, 5e-5, 5e-5), (1e-5, 5e-5, 1e-5), (0.0, 5e-5, 0.0)):
+        tr = trainer_of(model_of())
+        if scheduled is not None:
+            tr.optimizer.param_groups[0]["lr"] = scheduled
+        logp, draws = tr.atom_type_logprobs(d)
+        before = weights(tr)
+        steps_of(tr, d, draws, logp, lr=given)[which]()
+        assert 0.9 * want <= largest_move(tr, before) <= 1.01 * want, (given, scheduled)
+        assert tr.optimizer.param_groups[0]["lr"] == (scheduled or 0.0)
+    before = weights(tr)
+    for bad in (-1e-4, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="lr"):
+            steps_of(tr, d, draws, logp, lr=bad)[which]()
+    assert largest_move(tr, before) == 0.0 and tr.step_count == 1
