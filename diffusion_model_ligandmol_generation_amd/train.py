@@ -287,7 +287,7 @@ class ResearchAccurateTrainer:
                     g["lr"] = float(lr)
                 elif g["lr"] == 0:      # the schedule of train_research_validated counts epochs and starts at 0
                     g["lr"] = g.get("initial_lr", g["lr"])
-            self.optimizer.clip_and_step(self.model, max_norm=1.0)
+            self._clip_and_step()
         finally:
             for g, rate in zip(groups, rates):
                 g["lr"] = rate
@@ -353,17 +353,21 @@ class ResearchAccurateTrainer:
         from .parallel import allreduce_flat
         allreduce_flat([p.grad for p in self.model.parameters() if p.grad is not None], self.group)
 
+    def _clip_and_step(self):
+        """train.py:196-197: two launches over the flat gradient buffer, or any other optimiser's own step."""
+        if hasattr(self.optimizer, "clip_and_step"):
+            self.optimizer.clip_and_step(self.model, max_norm=1.0)
+        else:
+            torch.nn.utils.clip_grad_norm_(self.model.parameters(), max_norm=1.0)
+            self.optimizer.step()
+
     def train_step(self, batch, draws=None):
         """train.py:187-200 for one batch (one shard of the global batch under data parallelism)."""
         self.optimizer.zero_grad()
         loss_dict = self._compute_research_exact_loss(batch, training=True, draws=draws)
         loss_dict["total_loss"].backward()
         self._allreduce_gradients()
-        if hasattr(self.optimizer, "clip_and_step"):      # train.py:196-197 as two launches over the flat gradient buffer
-            self.optimizer.clip_and_step(self.model, max_norm=1.0)
-        else:
-            torch.nn.utils.clip_grad_norm_(self.model.parameters(), max_norm=1.0)
-            self.optimizer.step()
+        self._clip_and_step()
         self.step_count += 1
         return loss_dict
 

@@ -53,3 +53,22 @@ def test_learning_rates(which):
         with pytest.raises(ValueError, match="lr"):
             steps_of(tr, d, draws, logp, lr=bad)[which]()
     assert largest_move(tr, before) == 0.0 and tr.step_count == 1
+
+
+def test_any_optimiser():
+    """As train_step: an optimiser without a fused clip and step gets torch's clipping and its own step; the same update."""
+    d = fine_tune_batch(SIZES, 10)
+    moved = []
+    for plain in (False, True):
+        tr = trainer_of(model_of(), lr=1e-4)
+        if plain:
+            tr.optimizer = torch.optim.AdamW(tr.model.parameters(), lr=1e-4, weight_decay=1e-5)
+        logp, draws = tr.atom_type_logprobs(d, moved[0][1] if moved else None)
+        before = weights(tr)
+        for f in steps_of(tr, d, draws, logp):
+            f()
+        moved.append(({n: p.detach() - before[n] for n, p in tr.model.named_parameters()}, draws))
+        assert tr.step_count == 2
+    for n, want in moved[0][0].items():
+        # (a move of a rate's size from a gradient near 0 may take either sign: compared as a whole, as the other gradients are)
+        assert float((moved[1][0][n] - want).norm()) <= 1e-3 * float(want.norm()) + 1e-9, n
