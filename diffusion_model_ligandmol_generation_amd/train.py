@@ -88,6 +88,10 @@ class ResearchAccurateTrainer:
         progress = (step - self.warmup_steps) / max(1, 50000 - self.warmup_steps)
         return 0.5 * (1 + math.cos(math.pi * min(progress, 1.0)))
 
+    def _shared_dropout_seed(self):
+        """The dropout key of the present step under data parallelism: the same on every rank."""
+        return (self.dp_seed_base + self.step_count) & ((1 << 62) - 1)
+
     # ------------------------------------------------------------------ loss step
     def _compute_research_exact_loss(self, batch, training=True, draws=None):
         """train.py:267-452.  Returns the reference's dict: total_loss (differentiable), the
@@ -160,7 +164,6 @@ class ResearchAccurateTrainer:
             allc = torch.stack(allc)
             n_atoms_g, n_mols_g = int(allc[:, 0].sum()), int(allc[:, 1].sum())
             mol_off, atom_off = int(allc[:self.rank, 1].sum()), int(allc[:self.rank, 0].sum())
-            shared_seed = (self.dp_seed_base + self.step_count) & ((1 << 62) - 1)   # the same key on every rank
 
         class _Data:
             pass
@@ -173,7 +176,7 @@ class ResearchAccurateTrainer:
         if "dropout_seed" in draws:
             d.dropout_seed = int(draws["dropout_seed"])
         elif self.group is not None:
-            d.dropout_seed = shared_seed
+            d.dropout_seed = self._shared_dropout_seed()
         # the consistency module's outputs reach no loss term here (train.py:519, :543, :559, :583), so the
         # training step does not spend an O(sum n^2) pass and an [N,N] tensor on them
         d.skip_consistency = not getattr(self, "run_consistency", False)
@@ -205,14 +208,18 @@ class ResearchAccurateTrainer:
 
     # ------------------------------------------------------------------ fine-tuning on atom types
     def _fine_tune_draws(self, batch, draws):
-        """The random numbers of one noised forward pass: given ones, or new ones on the trainer's device.  Reference,
-        sampling and trained policy are compared at the same noise, so one set goes to all of them."""
+        """The random numbers of one noised forward pass: given ones, or new ones on the trainer's device; ``dropout_seed``, the
+        key of the dropout masks of a model in train mode, among them.  Reference, sampling and trained policy are compared at
+        the same noise and masks, so one set goes to all of them."""
         draws = dict(draws or {})
         n_mols = int(batch.batch.max()) + 1 if getattr(batch, "batch", None) is not None else 1
         if "u" not in draws:
             draws["u"] = torch.rand(n_mols, device=self.device)
         if "noise" not in draws:
             draws["noise"] = torch.randn(batch.pos.shape, device=self.device)
+        if "dropout_seed" not in draws:
+            draws["dropout_seed"] = (self._shared_dropout_seed() if self.group is not None
+                                     else int(torch.randint(0, 1 << 62, (1,), dtype=torch.int64).item()))
         return draws
 
     def _atom_type_logits(self, model, batch, draws):
@@ -244,8 +251,7 @@ class ResearchAccurateTrainer:
         d = _Data()
         d.x, d.pos, d.edge_index, d.batch, d._ligdiff_graph = batch.x.to(dev), pre_pos, batch.edge_index, batch.batch, graph
         d.skip_consistency = True
-        if "dropout_seed" in draws:
-            d.dropout_seed = int(draws["dropout_seed"])
+        d.dropout_seed = int(draws["dropout_seed"])
         props = getattr(batch, "properties", None)
         return model(d, c_noise, None if props is None else props.to(dev).float())[0], graph
 
@@ -258,9 +264,9 @@ class ResearchAccurateTrainer:
 
     def atom_type_logprobs(self, batch, draws=None, model=None, temperature=1.0):
         """(logp [N], draws): log-probabilities that ``model`` (the trainer's own by default; a frozen copy as the
-        reference) gives to ``batch.atom_types`` at the noise of ``draws``, without gradient.  Hand the same draws and the
-        returned values to ``preference_step`` / ``policy_step``.  Dropout follows the model's mode: ``model.eval()`` (gradients
-        flow all the same), or a ``dropout_seed`` in the draws, keeps its noise out of the ratios."""
+        reference) gives to ``batch.atom_types`` at the noise of ``draws``, without gradient.  Hand the returned draws and values
+        to ``preference_step`` / ``policy_step``: they hold the key of the dropout masks too, so that a model in train mode
+        scores and is trained under the same masks (``model.eval()`` has none; gradients flow all the same)."""
         from .tokens import token_logprobs
         model = self.model if model is None else model
         draws = self._fine_tune_draws(batch, draws)

@@ -1,4 +1,4 @@
-"""GPU: the trainer's fine-tuning steps as a program uses them: a trainer as it is built, its learning rate."""
+"""GPU: the trainer's fine-tuning steps as a program uses them: a trainer as it is built, its learning rate, dropout."""
 import pytest
 import torch
 
@@ -72,3 +72,30 @@ def test_any_optimiser():
     for n, want in moved[0][0].items():
         # (a move of a rate's size from a gradient near 0 may take either sign: compared as a whole, as the other gradients are)
         assert float((moved[1][0][n] - want).norm()) <= 1e-3 * float(want.norm()) + 1e-9, n
+
+
+def dropout_model():
+    from diffusion_model_ligandmol_generation_amd import ResearchAccurateDiffusionModel
+    torch.manual_seed(0)
+    return ResearchAccurateDiffusionModel().cuda().train()
+
+
+def test_dropout_is_in_the_draws():
+    """A model in train mode scores and is trained under the same masks: the ratio to itself is 1 at every position (to the
+    rtol 1e-4 / atol 2e-5 that two forms of the network agree to), so that nothing is clipped and the KL term is 0."""
+    d = fine_tune_batch(SIZES, 11)
+    tr = trainer_of(dropout_model())
+    adv = torch.tensor([1.0, -0.5, 0.2, -0.7], device="cuda")
+    logp, draws = tr.atom_type_logprobs(d)
+    r = tr.policy_step(d, draws, adv, logp, logp, kl_coef=0.05, lr=0.0)
+    torch.testing.assert_close(r.logp, logp, rtol=1e-4, atol=2e-5)
+    assert r.clip_fraction == 0 and r.kl < 1e-6
+    again, kept = tr.atom_type_logprobs(d, draws)
+    assert torch.equal(again, logp) and kept["dropout_seed"] == draws["dropout_seed"]
+    other, fresh = tr.atom_type_logprobs(d, {k: draws[k] for k in ("u", "noise")})      # another key: other masks
+    assert fresh["dropout_seed"] != draws["dropout_seed"] and float((other - logp).abs().max()) > 1e-3
+    r = tr.preference_step(d, draws, logp, lr=0.0)
+    assert float(r.margin.abs().max()) < 29 * 4e-4      # two sums of up to 29 differences
+    tr.model.eval()
+    still, _ = tr.atom_type_logprobs(d, draws)
+    assert float((still - logp).abs().max()) > 1e-3     # (and in eval mode there are none)
