@@ -92,6 +92,33 @@ class ResearchAccurateTrainer:
         """The dropout key of the present step under data parallelism: the same on every rank."""
         return (self.dp_seed_base + self.step_count) & ((1 << 62) - 1)
 
+    def _batch_properties(self, batch, n_mols, pilot=True):
+        """(properties [n_mols,15] or None, whether the PILOT loss family sees them), train.py:327-343: a 1-D vector is one row,
+        one row is every molecule's, rows too many are left out.  Without that loss (``pilot`` False) only the model reads
+        them, and a row of another width for each molecule leaves nothing open."""
+        if getattr(batch, "properties", None) is None:
+            return None, True
+        properties = batch.properties.to(self.device).float()
+        each = properties.dim() == 2 and properties.shape[0] == n_mols
+        if properties.dim() == 1:
+            properties = properties.unsqueeze(0)
+        if properties.shape[0] != n_mols:
+            properties = properties.repeat(n_mols, 1) if properties.shape[0] == 1 else properties[:n_mols]
+        if properties.shape[1] == 15:
+            return properties, True
+        if not self.reference_collate_quirk and (pilot or not each):
+            raise ValueError("batch.properties must be [B,15]; the reference's own loaders deliver [14 B] "
+                             "(data_utils.py:904-914 + PyG collate), which train.py:327-343 turns into one "
+                             "row for every molecule with the PILOT loss skipped: pass "
+                             "reference_collate_quirk=True to the trainer to get exactly that")
+        if properties.shape[1] < 8:
+            raise ValueError("batch.properties needs at least the 8 columns the PILOT encoders read")
+        # F.mse_loss(prop_pred [B,15], properties [B,w]) raises inside the try block of train.py:388-397:
+        # the family contributes nothing; the model reads columns 0..7 only (model1.py:342-345)
+        p15 = properties.new_zeros(n_mols, 15)
+        p15[:, :8] = properties[:, :8]
+        return p15, False
+
     # ------------------------------------------------------------------ loss step
     def _compute_research_exact_loss(self, batch, training=True, draws=None):
         """train.py:267-452.  Returns the reference's dict: total_loss (differentiable), the
@@ -126,28 +153,8 @@ class ResearchAccurateTrainer:
                                           float(edm.sigma_min), float(edm.sigma_max), float(edm.sigma_data),
                                           _ptr(coef), _ptr(c_noise), _ptr(noisy), _ptr(pre_pos), _stream()),
                   "ligdiff_edm_prepare")
-        properties = None
-        pilot_loss = True
-        if hasattr(batch, "properties") and batch.properties is not None:              # train.py:327-343
-            properties = batch.properties.to(dev).float()
-            if properties.dim() == 1:
-                properties = properties.unsqueeze(0)
-            if properties.shape[0] != B:
-                properties = properties.repeat(B, 1) if properties.shape[0] == 1 else properties[:B]
-            if properties.shape[1] != 15:
-                if not self.reference_collate_quirk:
-                    raise ValueError("batch.properties must be [B,15]; the reference's own loaders deliver [14 B] "
-                                     "(data_utils.py:904-914 + PyG collate), which train.py:327-343 turns into one "
-                                     "row for every molecule with the PILOT loss skipped: pass "
-                                     "reference_collate_quirk=True to the trainer to get exactly that")
-                if properties.shape[1] < 8:
-                    raise ValueError("batch.properties needs at least the 8 columns the PILOT encoders read")
-                # F.mse_loss(prop_pred [B,15], properties [B,w]) raises inside the try block of train.py:388-397:
-                # the family contributes nothing; the model reads columns 0..7 only (model1.py:342-345)
-                pilot_loss = False
-                p15 = properties.new_zeros(B, 15)
-                p15[:, :8] = properties[:, :8]
-                properties = p15
+        properties, pilot_loss = self._batch_properties(batch, B)
+        if properties is not None:
             if training:
                 null_rand = draws["null_rand"].to(dev) if "null_rand" in draws else torch.rand(B, device=dev)
                 properties = properties.clone()
@@ -252,8 +259,7 @@ class ResearchAccurateTrainer:
         d.x, d.pos, d.edge_index, d.batch, d._ligdiff_graph = batch.x.to(dev), pre_pos, batch.edge_index, batch.batch, graph
         d.skip_consistency = True
         d.dropout_seed = int(draws["dropout_seed"])
-        props = getattr(batch, "properties", None)
-        return model(d, c_noise, None if props is None else props.to(dev).float())[0], graph
+        return model(d, c_noise, self._batch_properties(batch, B, pilot=False)[0])[0], graph
 
     @staticmethod
     def _atom_types(batch, device):

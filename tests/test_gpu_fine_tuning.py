@@ -1,4 +1,5 @@
-"""GPU: the trainer's fine-tuning steps as a program uses them: a trainer as it is built, its learning rate, dropout."""
+"""GPU: the trainer's fine-tuning steps as a program uses them: a trainer as it is built, its learning rate, dropout, the
+forms of a batch's properties."""
 import pytest
 import torch
 
@@ -99,3 +100,36 @@ def test_dropout_is_in_the_draws():
     tr.model.eval()
     still, _ = tr.atom_type_logprobs(d, draws)
     assert float((still - logp).abs().max()) > 1e-3     # (and in eval mode there are none)
+
+
+def test_properties_as_in_train_step():
+    """Properties in every form that train_step takes: a vector, one row, rows too many, the reference loader's [14 B] behind its
+    flag; the network reads the first 8 columns.  Scoring and steps see the same ones."""
+    d, B = fine_tune_batch(SIZES, 12), len(SIZES)
+    g = torch.Generator().manual_seed(3)
+    full, loader = torch.randn(B, 15, generator=g), torch.randn(14 * B, generator=g)
+    tr = trainer_of(model_of())
+    draws = None
+
+    def score(tr, props):
+        nonlocal draws
+        d.properties = props
+        logp, draws = tr.atom_type_logprobs(d, draws)
+        for f in steps_of(tr, d, draws, logp, lr=0.0):
+            f()
+        return logp
+
+    none = score(tr, None)
+    want, one = score(tr, full), score(tr, full[:1].repeat(B, 1))
+    assert not torch.equal(want, none) and not torch.equal(want, one)
+    for props, same in ((full[0], one), (full[:1], one), (torch.cat([full, full]), want), (full.cuda(), want), (full.double(), want),
+                        (full[:, :8], want), (full[:, :14], want)):
+        assert torch.equal(score(tr, props), same), tuple(props.shape)
+    for bad in (loader, full[:, :7], full[:2]):
+        d.properties = bad
+        for f in (lambda: tr.atom_type_logprobs(d, draws), *steps_of(tr, d, draws, want)):
+            with pytest.raises(ValueError, match="properties"):
+                f()
+    row = torch.zeros(B, 15)
+    row[:, :8] = loader[:8]
+    assert torch.equal(score(trainer_of(model_of(), reference_collate_quirk=True), loader), score(tr, row))
