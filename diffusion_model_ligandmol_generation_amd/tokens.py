@@ -195,26 +195,28 @@ def embed_tokens_grad(d_out, tokens, n_rows, scale=1.0, out=None, accumulate=Fal
 
 
 # ------------------------------------------------------------------------------------------------ log-probabilities
-def _token_args(logits, tokens, temperature):
-    """(struct, rows, ids, n, V): the tensors must outlive the call."""
+def _check_rows(logits, tokens, temperature):
     _check_float(logits, "logits")
     if logits.dim() < 2 or logits.shape[-1] < 1:
         raise ValueError("logits must be [..., vocabulary]")
-    dev = logits.device
-    _check_ids(tokens, dev)
+    _check_ids(tokens, logits.device)
     if tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
-    temperature = float(temperature)
-    if not 1e-20 <= temperature <= 1e20:
+    if not 1e-20 <= float(temperature) <= 1e20:
         raise ValueError("temperature must be between 1e-20 and 1e20")
+
+
+def _token_args(logits, tokens, temperature):
+    """(struct, rows, ids, n, V) of checked tensors, which must outlive the call."""
     V = logits.shape[-1]
     rows, n, stride = _rows(logits, V)
     ids = tokens.contiguous()
     return TokenArgs(rows.data_ptr(), ids.data_ptr(), stride, n, V, _DTYPES[rows.dtype], _TOKEN_BYTES[ids.dtype],
-                     temperature), rows, ids, n, V
+                     float(temperature)), rows, ids, n, V
 
 
 def _logprob(logits, tokens, temperature, want_stats):
+    _check_rows(logits, tokens, temperature)
     a, rows, ids, n, V = _token_args(logits, tokens, temperature)
     dev = logits.device
     logp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
@@ -260,8 +262,9 @@ def token_logprobs(logits, tokens, temperature=1.0):
 
 
 # ------------------------------------------------------------------------------------------------ preference loss
-def _preference(logits, tokens, seq_ptr, ref_logp, beta, label_smoothing, kind, average, temperature, denominator, grad_scale,
-                want_grad):
+def _preference_inputs(logits, tokens, seq_ptr, ref_logp, beta, label_smoothing, kind, temperature, denominator, grad_scale):
+    """Checks what a preference loss is given, of the logits only where they are and their type and shape:
+    (seq_ptr, ref_logp, denominator, grad_scale) as the library takes them."""
     if kind not in _lib.PREFERENCE_KINDS:
         raise ValueError(f"kind must be one of {sorted(_lib.PREFERENCE_KINDS)}")
     beta, label_smoothing = float(beta), float(label_smoothing)
@@ -269,14 +272,21 @@ def _preference(logits, tokens, seq_ptr, ref_logp, beta, label_smoothing, kind, 
         raise ValueError("beta must be positive and label_smoothing in [0, 0.5)")
     if kind != "sigmoid" and label_smoothing:
         raise ValueError("label_smoothing belongs to the sigmoid loss")
-    a, rows, ids, n, V = _token_args(logits, tokens, temperature)
+    _check_rows(logits, tokens, temperature)
     dev = logits.device
     ptr = _ptr_vector(seq_ptr, dev)
     if ptr.numel() % 2 != 1:
         raise ValueError("seq_ptr must hold an even number of sequences: the preferred ones, then the others in the same order")
-    P = (ptr.numel() - 1) // 2
-    ref = None if ref_logp is None else _vector(ref_logp, n, dev, "ref_logp")
-    denominator, grad_scale = _denominator(denominator), _finite_scale(grad_scale, "grad_scale")
+    ref = None if ref_logp is None else _vector(ref_logp, tokens.numel(), dev, "ref_logp")
+    return ptr, ref, _denominator(denominator), _finite_scale(grad_scale, "grad_scale")
+
+
+def _preference(logits, tokens, seq_ptr, ref_logp, beta, label_smoothing, kind, average, temperature, denominator, grad_scale,
+                want_grad):
+    ptr, ref, denominator, grad_scale = _preference_inputs(logits, tokens, seq_ptr, ref_logp, beta, label_smoothing, kind,
+                                                           temperature, denominator, grad_scale)
+    a, rows, ids, n, V = _token_args(logits, tokens, temperature)
+    dev, P = logits.device, (ptr.numel() - 1) // 2
     lib = _lib.load()
     nbytes = _workspace_bytes("ligdiff_preference_workspace_bytes", n, P)
     f32 = dict(dtype=torch.float32, device=dev)
@@ -293,7 +303,7 @@ def _preference(logits, tokens, seq_ptr, ref_logp, beta, label_smoothing, kind, 
             slope, stats, row_seq = torch.empty(2 * P, **f32), torch.empty(n, 2, **f32), torch.empty(n, dtype=torch.int32, device=dev)
             saved = (slope.data_ptr(), stats.data_ptr(), row_seq.data_ptr())
         q = PreferenceArgs(ptr.data_ptr(), None if ref is None else ref.data_ptr(), P, _lib.PREFERENCE_KINDS[kind],
-                           1 if average else 0, beta, label_smoothing, denominator, grad_scale, loss.data_ptr(),
+                           1 if average else 0, float(beta), float(label_smoothing), denominator, grad_scale, loss.data_ptr(),
                            log_ratio.data_ptr(), margin.data_ptr(), *saved,
                            None if d is None else d.data_ptr(), V, ws.data_ptr(), nbytes)
         check(lib.ligdiff_preference_loss(C.byref(a), C.byref(q), stream), "ligdiff_preference_loss")
@@ -342,24 +352,34 @@ def preference_loss_and_grad(logits, tokens, seq_ptr, ref_logp=None, beta=0.1, l
 
 
 # ------------------------------------------------------------------------------------------------ policy loss
-def _policy(logits, tokens, seq_ptr, advantage, old_logp, ref_logp, advantage_per, clip_low, clip_high, kl_coef, aggregate,
-            temperature, denominator, grad_scale, want_grad, want_saved):
+def _policy_inputs(logits, tokens, seq_ptr, advantage, old_logp, ref_logp, advantage_per, clip_low, clip_high, kl_coef, aggregate,
+                   temperature, denominator, grad_scale):
+    """Checks what a policy loss is given, of the logits only where they are and their type and shape:
+    (seq_ptr, number of sequences, advantage, old_logp, ref_logp, denominator, grad_scale) as the library takes them."""
     if aggregate not in _lib.POLICY_MEANS:
         raise ValueError(f"aggregate must be one of {sorted(_lib.POLICY_MEANS)}")
     clip_low, clip_high, kl_coef = float(clip_low), float(clip_high), float(kl_coef)
     if not 0.0 <= clip_low <= 1.0 or not 0.0 <= clip_high <= 3e38 or not 0.0 <= kl_coef <= 3e38:
         raise ValueError("clip_low must be in [0, 1], clip_high and kl_coef at least 0")
-    a, rows, ids, n, V = _token_args(logits, tokens, temperature)
-    dev = logits.device
+    _check_rows(logits, tokens, temperature)
+    dev, n = logits.device, tokens.numel()
     ptr = None if seq_ptr is None else _ptr_vector(seq_ptr, dev)
     S = 1 if ptr is None else ptr.numel() - 1
     if advantage_per not in ("sequence", "token"):
         raise ValueError("advantage_per must be 'sequence' or 'token'")
-    per_token = advantage_per == "token"
-    adv = _vector(advantage, n if per_token else S, dev, "advantage")
+    adv = _vector(advantage, n if advantage_per == "token" else S, dev, "advantage")
     old = None if old_logp is None else _vector(old_logp, n, dev, "old_logp")
     ref = None if ref_logp is None else _vector(ref_logp, n, dev, "ref_logp")
-    denominator, grad_scale = _denominator(denominator), _finite_scale(grad_scale, "grad_scale")
+    return ptr, S, adv, old, ref, _denominator(denominator), _finite_scale(grad_scale, "grad_scale")
+
+
+def _policy(logits, tokens, seq_ptr, advantage, old_logp, ref_logp, advantage_per, clip_low, clip_high, kl_coef, aggregate,
+            temperature, denominator, grad_scale, want_grad, want_saved):
+    ptr, S, adv, old, ref, denominator, grad_scale = _policy_inputs(logits, tokens, seq_ptr, advantage, old_logp, ref_logp,
+                                                                    advantage_per, clip_low, clip_high, kl_coef, aggregate,
+                                                                    temperature, denominator, grad_scale)
+    a, rows, ids, n, V = _token_args(logits, tokens, temperature)
+    dev = logits.device
     mean = _lib.POLICY_MEANS[aggregate]
     lib = _lib.load()
     nbytes = _workspace_bytes("ligdiff_policy_workspace_bytes", n, S, mean)
@@ -370,8 +390,8 @@ def _policy(logits, tokens, seq_ptr, advantage, old_logp, ref_logp, advantage_pe
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         d = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
         q = PolicyArgs(None if ptr is None else ptr.data_ptr(), adv.data_ptr(), None if old is None else old.data_ptr(),
-                       None if ref is None else ref.data_ptr(), S, 1 if per_token else 0, mean, clip_low, clip_high, kl_coef,
-                       denominator, grad_scale, result.data_ptr(), logp.data_ptr(), stats.data_ptr() if want_saved else None,
+                       None if ref is None else ref.data_ptr(), S, 1 if advantage_per == "token" else 0, mean, float(clip_low), float(clip_high),
+                       float(kl_coef), denominator, grad_scale, result.data_ptr(), logp.data_ptr(), stats.data_ptr() if want_saved else None,
                        coef.data_ptr() if want_saved else None, None if d is None else d.data_ptr(), V, ws.data_ptr(), nbytes)
         check(lib.ligdiff_policy_loss(C.byref(a), C.byref(q), stream), "ligdiff_policy_loss")
     return result, logp, stats, coef, d

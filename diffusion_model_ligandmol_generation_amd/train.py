@@ -20,7 +20,7 @@ from . import _lib
 from ._lib import check
 from .autograd import packed_graph_of
 from .backward import EDMLossFunction, _Ctx
-from .engine import _ptr, _stream
+from .engine import _ptr, _stream, node_features
 
 LOSS_TERMS = ("edm_coordinate", "edm_preconditioning", "pilot_property", "dit_attention", "dit_adaptive_norm",
               "e3_coordinate", "e3_rotation", "e3_translation")
@@ -229,11 +229,9 @@ class ResearchAccurateTrainer:
                                      else int(torch.randint(0, 1 << 62, (1,), dtype=torch.int64).item()))
         return draws
 
-    def _atom_type_logits(self, model, batch, draws):
-        """``atom_pred`` [N,119] of ``model`` on the batch with its coordinates noised as in the training step
-        (train.py:286-312), and the packed graph."""
+    def _fine_tune_inputs(self, batch, draws):
+        """Checks the batch and the draws of a noised forward pass: (graph, node input, pos, u, noise, properties)."""
         dev = self.device
-        eng = model.engine()
         pos = batch.pos.to(dev).float().contiguous()
         if getattr(batch, "batch", None) is None:
             batch.batch = torch.zeros(pos.shape[0], dtype=torch.long, device=dev)
@@ -242,8 +240,17 @@ class ResearchAccurateTrainer:
         graph = packed_graph_of(batch)
         N, B = graph.n_atoms, graph.n_mols
         u, noise = draws["u"].to(dev).float().contiguous(), draws["noise"].to(dev).float().contiguous()
-        if u.shape != (B,) or noise.shape != (N, 3):
-            raise ValueError("draws must hold u [B] and noise [N,3]")
+        if pos.shape != (N, 3) or u.shape != (B,) or noise.shape != (N, 3):
+            raise ValueError("pos must be [N,3], and draws hold u [B] and noise [N,3]")
+        return graph, node_features(batch.x.to(dev), N)[0], pos, u, noise, self._batch_properties(batch, B, pilot=False)[0]
+
+    def _atom_type_logits(self, model, batch, draws, inputs=None):
+        """``atom_pred`` [N,119] of ``model`` on the batch with its coordinates noised as in the training step
+        (train.py:286-312), and the packed graph.  ``inputs``: the batch as ``_fine_tune_inputs`` gives it."""
+        dev = self.device
+        eng = model.engine()
+        graph, x, pos, u, noise, properties = self._fine_tune_inputs(batch, draws) if inputs is None else inputs
+        N, B = graph.n_atoms, graph.n_mols
         edm = model.edm_preconditioning
         coef, c_noise = torch.empty(B, 4, device=dev), torch.empty(B, device=dev)
         noisy, pre_pos = torch.empty_like(pos), torch.empty_like(pos)
@@ -256,10 +263,14 @@ class ResearchAccurateTrainer:
             pass
 
         d = _Data()
-        d.x, d.pos, d.edge_index, d.batch, d._ligdiff_graph = batch.x.to(dev), pre_pos, batch.edge_index, batch.batch, graph
+        d.x, d.pos, d.edge_index, d.batch, d._ligdiff_graph = x, pre_pos, batch.edge_index, batch.batch, graph
         d.skip_consistency = True
         d.dropout_seed = int(draws["dropout_seed"])
-        return model(d, c_noise, self._batch_properties(batch, B, pilot=False)[0])[0], graph
+        return model(d, c_noise, properties)[0], graph
+
+    def _logits_like(self, graph):
+        """What a loss needs to know of logits that are still to come: their shape, type and device."""
+        return torch.empty(1, 119, device=self.device).expand(graph.n_atoms, 119)
 
     @staticmethod
     def _atom_types(batch, device):
@@ -314,6 +325,25 @@ class ResearchAccurateTrainer:
         dist.all_reduce(t, group=self.count_group)
         return tuple(t.tolist())
 
+    def _over_ranks(self, look):
+        """``look()`` checks the arguments of a step on this rank and returns its (atoms, count): (count of all ranks, atoms of the
+        ranks before this one), exchanged between the host processes.  A rank whose arguments are refused raises its
+        error and the others a RuntimeError, before any of them waits for a gradient."""
+        if self.group is None:
+            return look()[1], 0
+        error, atoms, count = None, 0, 0
+        try:
+            atoms, count = look()
+        except Exception as e:      # whatever it is, the other ranks hear of it
+            error = e
+        later = [atoms if r > self.rank else 0 for r in range(self.world)]
+        total, refused, *before = self._sum_over_ranks(count, error is not None, *later)
+        if error is not None:
+            raise error
+        if refused:
+            raise RuntimeError(f"{int(refused)} of {self.world} ranks refused the arguments of this step")
+        return total, int(before[self.rank])
+
     def preference_step(self, batch, draws, ref_logp=None, beta=0.1, label_smoothing=0.0, kind="sigmoid", average=False,
                         temperature=1.0, lr=None):
         """One optimiser step on pairs of ligands: of the 2 P molecules of the batch, number p is preferred over number
@@ -322,13 +352,22 @@ class ResearchAccurateTrainer:
         loss is the mean over all of them.  ``lr``: the step's learning rate; None: the optimiser's, or, where the epoch
         schedule holds that at 0 (before the first epoch), the one the trainer was built with.  Returns tokens.PreferenceGrad
         (this rank's share of the loss)."""
-        from .tokens import preference_loss_and_grad
-        self._check_rate(lr)
-        types = self._atom_types(batch, self.device)
-        draws = self._fine_tune_draws(batch, draws)
-        logits, graph = self._atom_type_logits(self.model, batch, draws)
-        pairs, = self._sum_over_ranks(graph.n_mols // 2)
-        r = preference_loss_and_grad(logits, types, graph.mol_ptr, ref_logp, beta, label_smoothing, kind, average, temperature,
+        from .tokens import _preference_inputs, preference_loss_and_grad
+        draws, inputs = dict(draws or {}), []
+
+        def look():
+            self._check_rate(lr)
+            draws.update(self._fine_tune_draws(batch, draws))
+            inputs[:] = self._fine_tune_inputs(batch, draws)
+            graph = inputs[0]
+            _preference_inputs(self._logits_like(graph), self._atom_types(batch, self.device), graph.mol_ptr, ref_logp, beta,
+                               label_smoothing, kind, temperature, None, 1.0)
+            return graph.n_atoms, graph.n_mols // 2
+
+        pairs, _ = self._over_ranks(look)
+        logits, graph = self._atom_type_logits(self.model, batch, draws, inputs)
+        r = preference_loss_and_grad(logits, self._atom_types(batch, self.device), graph.mol_ptr, ref_logp, beta,
+                                     label_smoothing, kind, average, temperature,
                                      denominator=pairs if self.group is not None else None)
         self._fine_tune_update(logits, r, lr)
         return r
@@ -340,17 +379,26 @@ class ResearchAccurateTrainer:
         types, ``ref_logp`` those under the reference, both from ``atom_type_logprobs`` with the same ``draws``.  Under data
         parallelism the mean goes over all ranks' atoms / molecules.  ``lr`` as in ``preference_step``.  Returns
         tokens.PolicyGrad (this rank's share)."""
-        from .tokens import policy_loss_and_grad
-        self._check_rate(lr)
-        types = self._atom_types(batch, self.device)
-        draws = self._fine_tune_draws(batch, draws)
-        logits, graph = self._atom_type_logits(self.model, batch, draws)
-        denominator = None
-        if self.group is not None:
-            own = graph.n_mols if aggregate == "sequence" else int(((types >= 0) & (types < logits.shape[1])).sum())
-            denominator, = self._sum_over_ranks(own)
-        r = policy_loss_and_grad(logits, types, graph.mol_ptr, advantage, old_logp, ref_logp, advantage_per, clip_low, clip_high,
-                                 kl_coef, aggregate, temperature, denominator=denominator)
+        from .tokens import _policy_inputs, policy_loss_and_grad
+        draws, inputs = dict(draws or {}), []
+
+        def look():
+            self._check_rate(lr)
+            draws.update(self._fine_tune_draws(batch, draws))
+            inputs[:] = self._fine_tune_inputs(batch, draws)
+            graph = inputs[0]
+            like, types = self._logits_like(graph), self._atom_types(batch, self.device)
+            _policy_inputs(like, types, graph.mol_ptr, advantage, old_logp, ref_logp, advantage_per, clip_low, clip_high, kl_coef,
+                           aggregate, temperature, None, 1.0)
+            if self.group is None:      # (the library counts)
+                return graph.n_atoms, None
+            return graph.n_atoms, graph.n_mols if aggregate == "sequence" else int(((types >= 0) & (types < like.shape[1])).sum())
+
+        denominator, _ = self._over_ranks(look)
+        logits, graph = self._atom_type_logits(self.model, batch, draws, inputs)
+        r = policy_loss_and_grad(logits, self._atom_types(batch, self.device), graph.mol_ptr, advantage, old_logp, ref_logp,
+                                 advantage_per, clip_low, clip_high, kl_coef, aggregate, temperature,
+                                 denominator=denominator)
         self._fine_tune_update(logits, r, lr)
         return r
 
