@@ -265,7 +265,8 @@ class ResearchAccurateTrainer:
         d = _Data()
         d.x, d.pos, d.edge_index, d.batch, d._ligdiff_graph = x, pre_pos, batch.edge_index, batch.batch, graph
         d.skip_consistency = True
-        d.dropout_seed = int(draws["dropout_seed"])
+        # (as in the training step: masks are keyed by seed and global atom)
+        d.dropout_seed, d.atom_offset = int(draws["dropout_seed"]), int(draws.get("atom_offset", 0))
         return model(d, c_noise, properties)[0], graph
 
     def _logits_like(self, graph):
@@ -283,10 +284,20 @@ class ResearchAccurateTrainer:
         """(logp [N], draws): log-probabilities that ``model`` (the trainer's own by default; a frozen copy as the
         reference) gives to ``batch.atom_types`` at the noise of ``draws``, without gradient.  Hand the returned draws and values
         to ``preference_step`` / ``policy_step``: they hold the key of the dropout masks too, so that a model in train mode
-        scores and is trained under the same masks (``model.eval()`` has none; gradients flow all the same)."""
+        scores and is trained under the same masks (``model.eval()`` has none; gradients flow all the same).  Under data
+        parallelism every rank calls it on its part of the batch, and the masks are those of the whole batch."""
         from .tokens import token_logprobs
         model = self.model if model is None else model
-        draws = self._fine_tune_draws(batch, draws)
+        draws = dict(draws or {})
+
+        def look():
+            draws.update(self._fine_tune_draws(batch, draws))
+            return self._fine_tune_inputs(batch, draws)[0].n_atoms, 0
+
+        if self.group is not None and model.training and "atom_offset" not in draws:
+            _, draws["atom_offset"] = self._over_ranks(look)
+        else:
+            draws.update(self._fine_tune_draws(batch, draws))
         with torch.no_grad():
             logits, _ = self._atom_type_logits(model, batch, draws)
             return token_logprobs(logits, self._atom_types(batch, self.device), temperature), draws
@@ -364,7 +375,8 @@ class ResearchAccurateTrainer:
                                label_smoothing, kind, temperature, None, 1.0)
             return graph.n_atoms, graph.n_mols // 2
 
-        pairs, _ = self._over_ranks(look)
+        pairs, offset = self._over_ranks(look)
+        draws.setdefault("atom_offset", offset)
         logits, graph = self._atom_type_logits(self.model, batch, draws, inputs)
         r = preference_loss_and_grad(logits, self._atom_types(batch, self.device), graph.mol_ptr, ref_logp, beta,
                                      label_smoothing, kind, average, temperature,
@@ -394,7 +406,8 @@ class ResearchAccurateTrainer:
                 return graph.n_atoms, None
             return graph.n_atoms, graph.n_mols if aggregate == "sequence" else int(((types >= 0) & (types < like.shape[1])).sum())
 
-        denominator, _ = self._over_ranks(look)
+        denominator, offset = self._over_ranks(look)
+        draws.setdefault("atom_offset", offset)
         logits, graph = self._atom_type_logits(self.model, batch, draws, inputs)
         r = policy_loss_and_grad(logits, self._atom_types(batch, self.device), graph.mol_ptr, advantage, old_logp, ref_logp,
                                  advantage_per, clip_low, clip_high, kl_coef, aggregate, temperature,
