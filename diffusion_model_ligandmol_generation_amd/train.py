@@ -409,9 +409,10 @@ class ResearchAccurateTrainer:
         denominator, offset = self._over_ranks(look)
         draws.setdefault("atom_offset", offset)
         logits, graph = self._atom_type_logits(self.model, batch, draws, inputs)
+        # (no position on any rank: every share is 0, whatever it is divided by)
         r = policy_loss_and_grad(logits, self._atom_types(batch, self.device), graph.mol_ptr, advantage, old_logp, ref_logp,
                                  advantage_per, clip_low, clip_high, kl_coef, aggregate, temperature,
-                                 denominator=denominator)
+                                 denominator=None if denominator is None else max(denominator, 1))
         self._fine_tune_update(logits, r, lr)
         return r
 

@@ -68,6 +68,8 @@ def all_steps(group, mols):
                                       aggregate=aggregate))
     bp, dp, _, old_p = batch_of(pairs_of(mols))
     run("preference", model_of(), lambda tr: tr.preference_step(bp, dp, old_p, beta=0.3, label_smoothing=0.1))
+    b.atom_types = torch.full_like(b.atom_types, -1)
+    run("nothing", model_of(), lambda tr: tr.policy_step(b, draws, adv, old))
     return out
 
 
@@ -104,3 +106,4 @@ def test_two_ranks_equal_one_process():
             for n, t in grads.items():
                 off = float((torch.from_numpy(got[r][name][1][n]) - t).norm())
                 assert off <= 1e-4 * float(t.norm()) + 1e-9, (name, r, n, off, float(t.norm()))
+    assert want["nothing"][0] == 0 and not any(t.any() for t in want["nothing"][1].values())
