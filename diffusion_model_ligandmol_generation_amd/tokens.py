@@ -10,13 +10,15 @@ All run in the HIP library on the current stream of the tensors' device; there i
 fp32, bf16 or fp16 with rows any distance apart; ids are int32 or int64.  An id outside the vocabulary (-1 by custom) is an
 ignored position: a row of zeros, log-probability 0, no part in a loss.  The losses come in two forms: differentiable
 (``loss.backward()``), and ``*_and_grad``, which returns the gradient of the logits beside the loss - a training step that
-owns its backward pass hands it on with ``logits.backward(d_logits)`` and saves reading the logits again.
+owns its backward pass hands it on with ``logits.backward(d_logits)`` and saves reading the logits again.  Second and
+forward-mode derivatives are refused.
 The reference has no counterpart (one-hot types, no loss on the distribution of ``atom_pred``)."""
 import ctypes as C
 from collections import namedtuple
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -59,11 +61,18 @@ def _workspace_bytes(entry, *sizes):
     return getattr(_lib.load(), entry)(*sizes)
 
 
+def _check_tangent(t, name):
+    """A tangent would be lost without a word: the kernels read the values only."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{name} carries a tangent: forward-mode derivatives are not implemented")
+
+
 def _check_float(t, name):
     if not t.is_cuda:
         raise RuntimeError(f"{name} must live on a HIP device: the hot path has no CPU implementation")
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name} must be fp32, bf16 or fp16, got {t.dtype}")
+    _check_tangent(t, name)
 
 
 def _check_ids(tokens, device, name="tokens"):
@@ -91,6 +100,7 @@ def _vector(t, n, device, name):
         raise ValueError(f"{name} lives on {t.device}, the logits on {device}")
     if t.numel() != n:
         raise ValueError(f"{name} has {t.numel()} elements, expected {n}")
+    _check_tangent(t, name)
     if t.dtype != torch.float32:
         if t.dtype not in _DTYPES and t.dtype != torch.float64:
             raise ValueError(f"{name} must be a floating-point tensor, got {t.dtype}")
@@ -184,6 +194,8 @@ def embed_tokens_grad(d_out, tokens, n_rows, scale=1.0, out=None, accumulate=Fal
         raise ValueError(f"out must be [{n_rows}, {D}] on {dev}, of d_out's type or fp32")
     elif (D > 1 and out.stride(1) != 1) or (n_rows > 1 and out.stride(0) < D):
         raise ValueError("out must have rows of unit stride that do not overlap")
+    else:
+        _check_tangent(out, "out")
     lib = _lib.load()
     nbytes = _workspace_bytes("ligdiff_embed_grad_workspace_bytes", n, n_rows, D)
     with _on(dev) as stream:

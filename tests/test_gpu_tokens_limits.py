@@ -1,5 +1,5 @@
 """GPU: the token operators where a value has no bound or a size has no room: infinite margins of the
-preference loss.  Against plain 64-bit forms; the tolerances of single values are
+preference loss; and derivatives that they do not have.  Against plain 64-bit forms; the tolerances of single values are
 those of test_gpu_tokens.py (U half a step of fp32, LOGP the error of a log-probability)."""
 import pytest
 import torch
@@ -73,3 +73,33 @@ def test_nan_margin_is_the_loss(tk):
             y[1, 0] = y[5, 0] = float("-inf")
         for e in (0.0, 0.2):
             assert tk.preference_loss(y, ids, ptr, label_smoothing=e).loss.isnan()
+
+
+# ------------------------------------------------------------------------------------------------ other derivatives
+def test_no_tangent_is_lost(tk):
+    """Forward-mode derivatives are refused in every input that has values, and so are torch.func's transforms."""
+    import torch.autograd.forward_ad as fw
+    g = gen(31)
+    x, table = torch.randn(12, 9, device="cuda", generator=g), torch.randn(9, 6, device="cuda", generator=g)
+    ids, ptr = ids_of(12, 9, g), torch.tensor([0, 3, 6, 9, 12], device="cuda")
+    lp, adv, up = torch.randn(12, device="cuda"), torch.randn(4, device="cuda"), torch.randn(12, 6, device="cuda")
+    calls = [(x, lambda y: tk.token_logprobs(y, ids)), (table, lambda y: tk.embed_tokens(ids, y)), (up, lambda y: tk.embed_tokens_grad(y, ids, 9)),
+             (torch.zeros(9, 6, device="cuda"), lambda y: tk.embed_tokens_grad(up, ids, 9, out=y))]
+    for f in (tk.preference_loss, tk.preference_loss_and_grad):
+        calls += [(x, lambda y, f=f: f(y, ids, ptr, lp)), (lp, lambda y, f=f: f(x, ids, ptr, y))]
+    for f in (tk.policy_loss, tk.policy_loss_and_grad):
+        calls += [(x, lambda y, f=f: f(y, ids, ptr, adv, lp, lp)), (adv, lambda y, f=f: f(x, ids, ptr, y, lp, lp)),
+                  (lp, lambda y, f=f: f(x, ids, ptr, adv, y, lp)), (lp, lambda y, f=f: f(x, ids, ptr, adv, lp, y))]
+    for i, (t, f) in enumerate(calls):
+        with fw.dual_level():
+            f(t.clone())                            # no tangent: as ever
+            for leaf in (t.clone(), t.clone().requires_grad_()):
+                with pytest.raises(NotImplementedError):
+                    print(i, f(fw.make_dual(leaf, torch.ones_like(t))))
+        with pytest.raises(NotImplementedError, match="tangent"):
+            torch.func.jvp(lambda y: f(y) if torch.is_tensor(f(y)) else f(y).loss, (t,), (t,))
+        f(t.clone())
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda y: tk.token_logprobs(y, ids))(x.expand(3, 12, 9))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda y: tk.token_logprobs(y, ids).sum())(x)
