@@ -26,6 +26,7 @@ from ._lib import PolicyArgs, PreferenceArgs, TokenArgs, check
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _TOKEN_BYTES = {torch.int32: 4, torch.int64: 8}
+_INT_MAX = 0x7fffffff      # what the library's 32-bit sizes hold (a larger number would arrive as its low half)
 
 PreferenceLoss = namedtuple("PreferenceLoss", "loss log_ratio margin")
 PreferenceGrad = namedtuple("PreferenceGrad", "loss log_ratio margin d_logits")
@@ -109,7 +110,7 @@ def _vector(t, n, device, name):
 
 
 def _ptr_vector(seq_ptr, device, name="seq_ptr"):
-    if seq_ptr.dtype not in _TOKEN_BYTES or seq_ptr.dim() != 1 or seq_ptr.numel() < 2:
+    if seq_ptr.dtype not in _TOKEN_BYTES or seq_ptr.dim() != 1 or not 2 <= seq_ptr.numel() <= _INT_MAX:
         raise ValueError(f"{name} must be a 1-D int32 tensor of first positions, one more than there are sequences")
     if seq_ptr.device != device:
         raise ValueError(f"{name} lives on {seq_ptr.device}, the logits on {device}")
@@ -138,8 +139,8 @@ def _denominator(value):
 # ------------------------------------------------------------------------------------------------ embedding
 def _embed(tokens, table, scale):
     _check_float(table, "table")
-    if table.dim() != 2 or table.numel() == 0:
-        raise ValueError("table must be [rows, width] and not empty")
+    if table.dim() != 2 or table.numel() == 0 or table.shape[1] > _INT_MAX:
+        raise ValueError("table must be [rows, width], not empty and less than 2^31 wide")
     dev = table.device
     _check_ids(tokens, dev)
     scale = _finite_scale(scale, "scale")
@@ -182,8 +183,8 @@ def embed_tokens_grad(d_out, tokens, n_rows, scale=1.0, out=None, accumulate=Fal
     _check_ids(tokens, dev)
     scale, n_rows = _finite_scale(scale, "scale"), int(n_rows)
     D = d_out.shape[-1] if d_out.dim() else 0
-    if n_rows < 1 or D < 1 or d_out.shape[:-1] != tokens.shape:
-        raise ValueError("d_out must be [*tokens.shape, width] with width and n_rows at least 1")
+    if n_rows < 1 or not 1 <= D <= _INT_MAX or d_out.shape[:-1] != tokens.shape:
+        raise ValueError("d_out must be [*tokens.shape, width] with width (below 2^31) and n_rows at least 1")
     rows, n, stride = _rows(d_out, D)
     ids = tokens.contiguous()
     if out is None:
@@ -209,8 +210,8 @@ def embed_tokens_grad(d_out, tokens, n_rows, scale=1.0, out=None, accumulate=Fal
 # ------------------------------------------------------------------------------------------------ log-probabilities
 def _check_rows(logits, tokens, temperature):
     _check_float(logits, "logits")
-    if logits.dim() < 2 or logits.shape[-1] < 1:
-        raise ValueError("logits must be [..., vocabulary]")
+    if logits.dim() < 2 or not 1 <= logits.shape[-1] <= _INT_MAX:
+        raise ValueError("logits must be [..., vocabulary] with fewer than 2^31 ids")
     _check_ids(tokens, logits.device)
     if tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")

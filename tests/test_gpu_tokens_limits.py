@@ -1,5 +1,5 @@
 """GPU: the token operators where a value has no bound or a size has no room: infinite margins of the
-preference loss; and derivatives that they do not have.  Against plain 64-bit forms; the tolerances of single values are
+preference loss; derivatives that they do not have; sizes beyond 32 bits.  Against plain 64-bit forms; the tolerances of single values are
 those of test_gpu_tokens.py (U half a step of fp32, LOGP the error of a log-probability)."""
 import pytest
 import torch
@@ -103,3 +103,19 @@ def test_no_tangent_is_lost(tk):
         torch.func.vmap(lambda y: tk.token_logprobs(y, ids))(x.expand(3, 12, 9))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda y: tk.token_logprobs(y, ids).sum())(x)
+
+
+# ------------------------------------------------------------------------------------------------ sizes beyond 32 bits
+@pytest.mark.parametrize("size", [1 << 31, (1 << 32) + 5])
+def test_sizes_that_do_not_fit(tk, size):
+    """Sizes that the library holds in 32 bits are refused beyond them (2^32 + 5 would arrive as 5).  The tensors are one element
+    each, expanded."""
+    one, ids = torch.ones(1, 1, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+    wide, ptr = one.expand(1, size), torch.zeros(1, dtype=torch.int32, device="cuda").expand(size | 1)
+    adv = torch.ones(1, device="cuda")
+    for call in (lambda: tk.token_logprobs(wide, ids), lambda: tk.embed_tokens(ids, wide), lambda: tk.embed_tokens_grad(wide, ids, 3),
+                 lambda: tk.policy_loss(wide, ids, None, adv), lambda: tk.preference_loss(wide, ids, ptr[:3]),
+                 lambda: tk.preference_loss(one, ids, ptr), lambda: tk.policy_loss(one, ids, ptr, adv.expand(size)),
+                 lambda: tk.policy_loss_and_grad(one, ids, ptr, adv, advantage_per="token")):
+        with pytest.raises(ValueError):
+            call()
