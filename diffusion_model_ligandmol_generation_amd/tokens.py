@@ -111,11 +111,11 @@ def _vector(t, n, device, name):
 
 def _ptr_vector(seq_ptr, device, name="seq_ptr"):
     if seq_ptr.dtype not in _TOKEN_BYTES or seq_ptr.dim() != 1 or not 2 <= seq_ptr.numel() <= _INT_MAX:
-        raise ValueError(f"{name} must be a 1-D int32 tensor of first positions, one more than there are sequences")
+        raise ValueError(f"{name} must be a 1-D int32 or int64 tensor of first positions, one more than there are sequences")
     if seq_ptr.device != device:
         raise ValueError(f"{name} lives on {seq_ptr.device}, the logits on {device}")
-    if seq_ptr.dtype != torch.int32:
-        seq_ptr = seq_ptr.to(torch.int32)
+    if seq_ptr.dtype != torch.int32:   # (offsets beyond every position stay so)
+        seq_ptr = seq_ptr.clamp(-_INT_MAX - 1, _INT_MAX).to(torch.int32)
     return seq_ptr.contiguous()
 
 

@@ -119,3 +119,20 @@ def test_sizes_that_do_not_fit(tk, size):
                  lambda: tk.policy_loss_and_grad(one, ids, ptr, adv, advantage_per="token")):
         with pytest.raises(ValueError):
             call()
+
+
+def test_offsets_beyond_every_position(tk):
+    """First positions before 0 and behind the last position, also such as 32 bits do not hold: the sequences reach as far as the
+    positions do."""
+    g = gen(33)
+    T = 1500
+    x, ids, adv = torch.randn(T, 9, device="cuda", generator=g), ids_of(T, 9, g, 0.1), torch.randn(2, device="cuda", generator=g)
+    of = lambda *v: torch.tensor(v, device="cuda")   # noqa: E731
+    for n in (T, 50):                                # (several chunks, and one block)
+        want_p = tk.policy_loss_and_grad(x[:n], ids[:n], of(0, 20, n).int(), adv, kl_coef=0.0, aggregate="sequence")
+        want_q = tk.preference_loss_and_grad(x[:n], ids[:n], of(0, 20, n).int())
+        for ptr in (of(0, 20, n), of(-5, 20, n + 9), of(0, 20, 1 << 31), of(0, 20, (1 << 32) + 3), of(-(1 << 31) - 1, 20, 1 << 40),
+                    of(-(1 << 62), 20, (1 << 62) + 25), of(-(1 << 31), 20, (1 << 31) - 1).int()):
+            for got, want in ((tk.policy_loss_and_grad(x[:n], ids[:n], ptr, adv, kl_coef=0.0, aggregate="sequence"), want_p),
+                              (tk.preference_loss_and_grad(x[:n], ids[:n], ptr), want_q)):
+                assert all(torch.equal(a, b) for a, b in zip(got, want)), ptr.tolist()
