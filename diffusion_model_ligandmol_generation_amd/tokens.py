@@ -131,8 +131,8 @@ def _denominator(value):
     if value is None:
         return 0.0
     value = float(value)
-    if not 0.0 < value <= 3e38:
-        raise ValueError("denominator must be positive")
+    if not 2.0 ** -126 <= value <= 3e38:   # (what fp32 rounds to 0 would ask for the count)
+        raise ValueError("denominator must be positive, and a normal number of fp32")
     return value
 
 

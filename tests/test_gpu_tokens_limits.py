@@ -136,3 +136,17 @@ def test_offsets_beyond_every_position(tk):
             for got, want in ((tk.policy_loss_and_grad(x[:n], ids[:n], ptr, adv, kl_coef=0.0, aggregate="sequence"), want_p),
                               (tk.preference_loss_and_grad(x[:n], ids[:n], ptr), want_q)):
                 assert all(torch.equal(a, b) for a, b in zip(got, want)), ptr.tolist()
+
+
+def test_denominators_at_the_ends(tk):
+    """The smallest and largest normal numbers of fp32 divide; what rounds to 0 there is refused (0 asks for the count)."""
+    g = gen(34)
+    x, ids, ptr = torch.randn(4, 9, device="cuda", generator=g), ids_of(4, 9, g), torch.tensor([0, 2, 4], device="cuda")
+    adv = torch.ones(2, device="cuda")
+    for f in (lambda d: tk.preference_loss(x, ids, ptr, denominator=d), lambda d: tk.policy_loss(x, ids, ptr, adv, denominator=d)):
+        one = f(1.0).loss.double()
+        for d in (2.0 ** -126, 2.0 ** -100, 2.0 ** 100, 2.0 ** 127):
+            within(f(d).loss, (one / d).float().double(), 2 * U * (one / d).abs(), d)
+        for d in (0.0, 1e-50, 1e-40, -1.0, 3.5e38, float("nan"), float("inf")):
+            with pytest.raises(ValueError, match="denominator"):
+                f(d)
