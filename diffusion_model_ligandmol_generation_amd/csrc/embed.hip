@@ -510,10 +510,11 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void k_segment_join(SegIn a) {
 // in order; a row more takes the tokens without one.  The block joins its waves' tables and writes one part; k_table_join
 // adds the parts in order.  Four rows make one trip to LDS; read, add and write take a third of the time that LDS's float
 // atomics (29696 x 256 rows and 119 tokens: 52 us with atomics, 16 so, 20 sorted).  What bounds it at 119 rows, where one
-// block of four waves fits into a compute unit, is the instructions of its waves; many rows come at 4.2 TB/s.
+// block of four waves fits into a compute unit, is the instructions of its waves; many rows come at 3.9 to 4.2 TB/s.
 #define TABLE_ROWS 128
 #define TABLE_WAVES 4
 #define TABLE_U 16   // rows in flight, twice
+#define TABLE_CHAIN 1024   // rows a wave adds at most: as many additions of one 32-bit sum, if all are of one token
 struct TableIn {
   const void* d_out; int64_t d_stride;
   TokenView tok; int64_t n;
@@ -662,11 +663,14 @@ static int chunk_rows(int64_t n, int tiles) {
   while (r < 512 && n * tiles > (int64_t)r * 8192) r *= 2;
   return r;
 }
-// Blocks of the table sums: as many as the chip holds at once (a block takes rows + 1 KB of LDS), 32 rows a wave or more.
+// Blocks of the table sums: as many as the chip holds at once (a block takes rows + 1 KB of LDS), 32 rows a wave or more; whole
+// multiples of that many where a wave would add more than TABLE_CHAIN rows (600000 x 256 fp32: 143 -> 156 us, 400000 x 2048 702 ->
+// 791, the parts that the join reads; 8192 x 16448, where the chip was not full, 243 -> 199).
 static int64_t table_per_wave(int64_t n, int32_t rows, int32_t width) {
   const int64_t tiles = (width + 63) / 64, held = 256 * (rows <= 32 ? 4 : rows <= 64 ? 2 : 1);
-  const int64_t chunks = tiles < held ? held / tiles : 1, waves = chunks * TABLE_WAVES;
-  const int64_t per = (n + waves - 1) / waves;
+  const int64_t waves = (tiles < held ? held / tiles : 1) * TABLE_WAVES;
+  const int64_t rounds = (n + waves * TABLE_CHAIN - 1) / (waves * TABLE_CHAIN);
+  const int64_t per = rounds > 1 ? (n + waves * rounds - 1) / (waves * rounds) : (n + waves - 1) / waves;
   return per < 32 ? 32 : (per + 7) / 8 * 8;
 }
 static int64_t table_chunks(int64_t n, int32_t rows, int32_t width) {
@@ -674,7 +678,7 @@ static int64_t table_chunks(int64_t n, int32_t rows, int32_t width) {
   return (n + per - 1) / per;
 }
 // Measured against the sort (119 rows, us): 29 x 256 7 against 10, 29696 x 256 16 against 20, 29696 x 1024 32 against 39,
-// 600000 x 64 38 against 107, 600000 x 256 142 against 153; bf16 29696 x 1024 31 against 31.  (A batch's offsets are 32 bits.)
+// 600000 x 64 38 against 107, 600000 x 256 156 against 153; bf16 29696 x 1024 31 against 31.  (A batch's offsets are 32 bits.)
 static bool table_form(int64_t n, int32_t rows, int64_t d_stride) { return n > 0 && rows <= TABLE_ROWS && d_stride <= (1 << 24); }
 struct EmbedWs { uint32_t* key[2]; int32_t* pos[2]; int32_t* hist; int32_t* row_ptr; float* part; size_t bytes; };
 static EmbedWs embed_ws(void* base, int64_t n, int32_t rows, int32_t width) {

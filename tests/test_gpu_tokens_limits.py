@@ -1,5 +1,5 @@
 """GPU: the token operators where a value has no bound or a size has no room: infinite margins of the
-preference loss; derivatives that they do not have; sizes beyond 32 bits.  Against plain 64-bit forms; the tolerances of single values are
+preference loss; derivatives that they do not have; sizes beyond 32 bits; long sums.  Against plain 64-bit forms; the tolerances of single values are
 those of test_gpu_tokens.py (U half a step of fp32, LOGP the error of a log-probability)."""
 import pytest
 import torch
@@ -150,3 +150,20 @@ def test_denominators_at_the_ends(tk):
         for d in (0.0, 1e-50, 1e-40, -1.0, 3.5e38, float("nan"), float("inf")):
             with pytest.raises(ValueError, match="denominator"):
                 f(d)
+
+
+# ------------------------------------------------------------------------------------------------ long sums
+@pytest.mark.parametrize("T,V,D", [(65536, 119, 2048), (8192, 119, 16448), (24576, 20, 16448), (16384, 64, 16384), (70000, 300, 1000)])
+def test_long_sums_into_small_tables(tk, T, V, D):
+    """Every position has one token and the value 1 + 2^-14.  Sums of up to 1023 such values are exact in fp32; from 1024 on an
+    addition of one more loses its 2^-14, always to the same side, so that a running sum of 2048 is short by 3e-5.  Parts of
+    1024 at most cost one such step (u relative); they are joined four to a block, and the blocks' parts by 8 waves in turn."""
+    d = torch.full((T, D), 1 + 2.0 ** -14, device="cuda")
+    ids = torch.full((T,), V - 1, device="cuda")
+    ids[::97] = -1
+    n = int((ids >= 0).sum())
+    got = tk.embed_tokens_grad(d, ids, V)
+    adds = 1 + 4 + (T / 4096 + 8) + 8
+    within(got[V - 1], torch.full((D,), n * (1 + 2.0 ** -14), dtype=torch.float64, device="cuda"), adds * U * n, "sum")
+    assert not got[:V - 1].any()
+    assert torch.equal(got, tk.embed_tokens_grad(d, ids, V))
