@@ -314,6 +314,14 @@ __device__ __forceinline__ void exponentials(const TokenRows& a, u32x4 (&x)[NV],
     __builtin_amdgcn_sched_barrier(0);
   }
 }
+// A pack's exponentials added to a lane's sum.  Eight go by pairs: one after the other, 16 packs would be 128 additions to one
+// sum, twice those of a row of fp32.
+template <int N> __device__ __forceinline__ float add_pack(float s, const float (&e)[N]) {
+  if constexpr (N == 8) return s + (((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])));
+#pragma unroll
+  for (int j = 0; j < N; ++j) s += e[j];
+  return s;
+}
 // Half-precision rows that start between two 32-bit words (odd strides): packs across word borders come slower.  Where many
 // blocks of few lanes hold rows in registers it shows less (rows of 32003 bf16 127 us, of 32004 115); the kernel that streams
 // longer rows reads whole words, five a pack, and shifts them (another partition of the row would be another order of its sum,
@@ -433,8 +441,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, ROW_WAVES(NV * 4, MODE)) voi
     if (none) m = 0.f;
     float s = et = __builtin_amdgcn_exp2f(exponent(a, et, m));
     exponentials<T, NV, TPR>(a, x, nb, m, [&](int k, float (&e)[N]) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) s += e[j];
+      s = add_pack(s, e);
       if constexpr (KEEP) set_pack(x[k], e);
     });
     s = group_sum<GRP>(s);
@@ -597,7 +604,8 @@ __global__ __launch_bounds__(1024) void k_token_rows_long(TokenRows a, PolicyIn 
       }
       const float base = m == -__builtin_inff() ? 0.f : m;
 #pragma unroll
-      for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f(exponent(a, v[j], base));
+      for (int j = 0; j < N; ++j) v[j] = __builtin_amdgcn_exp2f(exponent(a, v[j], base));
+      s = add_pack(s, v);
     }
     const float wm = group_max<64>(m);
     s = group_sum<64>(s * part_factor(a, m, wm == -__builtin_inff() ? 0.f : wm));

@@ -167,3 +167,19 @@ def test_long_sums_into_small_tables(tk, T, V, D):
     within(got[V - 1], torch.full((D,), n * (1 + 2.0 ** -14), dtype=torch.float64, device="cuda"), adds * U * n, "sum")
     assert not got[:V - 1].any()
     assert torch.equal(got, tk.embed_tokens_grad(d, ids, V))
+
+
+@pytest.mark.parametrize("dtype,low", [(torch.bfloat16, -16.75), (torch.float16, -16.640625)])
+@pytest.mark.parametrize("V", [1024, 1536, 2048, 6144, 8192, 16384, 24576, 32768, 49152, 98304, 131072])
+def test_sums_that_start_with_the_largest(tk, dtype, low, V):
+    """One logit 0, all others ``low``: their exponentials are just below half a step of 1 (0.892 and 0.995 u), and each that is
+    added to the largest one alone is lost.  The sum is held to the 64 additions a lane and 40 of the tree, one u each, that a
+    row's tolerance counts; the other lanes' sums are exact to a few u of 1e-2 at most."""
+    x = torch.full((5, V), low, dtype=dtype, device="cuda")
+    x[:, 0] = 0
+    ids = torch.zeros(5, dtype=torch.int64, device="cuda")
+    want = -torch.log1p((V - 1) * torch.tensor(low, dtype=torch.float64, device="cuda").exp()).expand(5)
+    within(tk.token_logprobs(x, ids), want, 104 * U, "log-probabilities")
+    for T in (1, 5):
+        r = tk.policy_loss_and_grad(x[:T], ids[:T], None, torch.ones(1, device="cuda"), kl_coef=0.0)
+        within(r.logp, want[:T], 104 * U, "policy")
