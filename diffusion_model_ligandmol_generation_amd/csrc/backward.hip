@@ -20,8 +20,6 @@ struct BwdLayout {
   size_t dmod[LD_MAXL], b256a, b256b, b256c, b256d, b512, b2048, b8, bhid;
   size_t wt;   // transposed weight block of the dX GEMM in flight (<= 1536 x 256 elements, fp32 or split bf16: 6 bytes each)
   size_t wt_all, wt_all_floats;   // every weight block the input-gradient GEMMs need transposed, filled by ONE launch
-  size_t types;              // LIGDIFF_FWD_ATOM_TYPES: gradients of the per-type atom branch, [2][LD_A + 1, 256]
-  size_t sort, sort_bytes;   // and the workspace of the sums over equal types
   size_t pool, pool_bytes;   // single-use buffers: everything a weight-gradient launch on the side stream reads
   size_t total;
 };
@@ -29,12 +27,20 @@ struct BwdLayout {
 // out-projection 256 x 256, in-projection 768 x 256, adaLN 1536 x 256; per E(3) layer six 256 x 256 blocks and the
 // 128 x 256 coordinate gate; second time-MLP layer 256 x 512.
 #define WT_ALL_FLOATS(nl) (3 * 65536 + (nl) * (2 * 262144 + 65536 + 196608 + 393216) + (nl) * (6 * 65536 + 32768) + 131072)
+// The atom branch of the input embedding: a gradient row for each atom, or (LIGDIFF_FWD_ATOM_TYPES) two for each type and the
+// workspace of the sums over equal types, which is no larger from 10000 atoms on.
+#define TYPE_FLOATS ((LD_A + 1) * 256)
+static size_t type_sum_bytes(int64_t N) { return embed_grad_workspace(N, LD_A + 1, 256); }
+static int64_t atom_branch_floats(int64_t N) {
+  const int64_t types = 2 * TYPE_FLOATS + (int64_t)(type_sum_bytes(N) / 4);
+  return types > N * 256 ? types : N * 256;
+}
 // Bytes of the single-use pool: one buffer per use of every tensor that a weight-gradient launch reads (heads,
 // per attention layer, per E(3) layer, embeddings), each rounded like `take` below.
 static size_t bwd_pool_bytes(int64_t N, int64_t E, int nl) {
   const int64_t dit[] = {N * 256, N * 1024, N * 256, N * 768};
   const int64_t e3[] = {N * 256, N * 256, E * 128, E * 256, E * 256, E * 32, E * 32, E * 32, N * 512};
-  const int64_t once[] = {N * 512, N * 256, N * 256};
+  const int64_t once[] = {N * 512, atom_branch_floats(N), N * 256};
   size_t tot = 0;
   auto add = [&](int64_t nfloats) { tot += align_up((size_t)nfloats * 4 + 16, 256); };
   for (int l = 0; l < nl; ++l) {
@@ -57,9 +63,6 @@ static void bwd_layout(BwdLayout* L, int64_t N, int64_t E, int32_t B) {
   L->wt = take(1536 * 256 * 3 / 2);
   L->wt_all_floats = WT_ALL_FLOATS(nl);
   L->wt_all = take(L->wt_all_floats);
-  L->types = take(2 * (LD_A + 1) * 256);
-  L->sort_bytes = embed_grad_workspace(N, LD_A + 1, 256);
-  L->sort = take(L->sort_bytes / 4);
   L->pool = off;
   L->pool_bytes = bwd_pool_bytes(N, E, nl);
   off += L->pool_bytes;
@@ -602,12 +605,12 @@ extern "C" int ligdiff_backward_train(const float* const* w, float* const* gr, c
   // ------------------------------------------------------------------ embeddings (model1.py:709-718)
   {
     if (flags & LIGDIFF_FWD_ATOM_TYPES) {
-      // all atoms of a type share the branch's input: sum their gradients by sorted types, then LayerNorm and weights on
+      // all atoms of a type share the branch's input: sum their gradients by type, then LayerNorm and weights on
       // LD_A + 1 rows
-      float* dt = T(L.types);
-      float* du = dt + (LD_A + 1) * 256;
+      float* dt = fresh(atom_branch_floats(N));
+      float* du = dt + TYPE_FLOATS;
       const EmbedGrad eg{dxa, LIGDIFF_F32, 256, TokenView{x, 4, LD_A}, N, LD_A + 1, 256, 1.0f, dt, LIGDIFF_F32, 256, false};
-      embed_grad(eg, T(L.sort), s);
+      embed_grad(eg, du + TYPE_FLOATS, s);
       ln_bwd<0, 1>(A(F.type_pre), 256, w[W_ATOM_G], w[W_ATOM_BE], 1e-5f, dt, 256, nullptr, 0, nullptr, du, 256, gr[W_ATOM_G],
                    gr[W_ATOM_BE], LD_A + 1, s);
       type_embed_dw(du, gr[W_ATOM_W], gr[W_ATOM_B], s);

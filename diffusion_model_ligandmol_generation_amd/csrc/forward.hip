@@ -334,7 +334,8 @@ void fwd_layout(FwdLayout* L, int64_t N, int64_t E, int32_t B, int flags) {
   L->pooled = take((size_t)B * 256); L->ph = take((size_t)B * 256);
   L->save = save ? 1 : 0;
   if (save) {
-    L->t1_pre = take(Bt * 512); L->ua = take(N * 256);
+    L->t1_pre = take(Bt * 512);
+    if (!(flags & LIGDIFF_FWD_ATOM_TYPES)) L->ua = take(N * 256);
     L->pen_pre = take((size_t)B * 512); L->pg_pre = take((size_t)B * 256);
     L->pz = take((size_t)B * 8); L->pw = take((size_t)B * 8);
     for (int l = 0; l < nl; ++l) {
