@@ -47,6 +47,7 @@ __device__ __forceinline__ double log_of_sum(float s) {
 }
 
 // exp(q) - 1 and exp(q) - 1 - q without cancellation (the second is ~q^2 / 2): Taylor for |q| < 1/2, eight terms leave 2e-9.
+// In 32 bits: see row_epilogue.
 __device__ __forceinline__ void kl_terms(float q, float& em1, float& kl) {
   if (fabsf(q) < 0.5f) {
     float p = 1.0f / 362880.0f;
@@ -117,6 +118,9 @@ template <int MODE> __device__ __forceinline__ RowScalars row_scalars(const Toke
 
 // What a row contributes once its maximum M and sum S are known, the same in every lane of the row; returns the gradient's
 // factor d loss / d logp * grad_scale / temperature.
+// logp is in 64 bits up to its differences with old_logp and ref_logp, which are rounded once to 32; ratio, clip bounds, gain, KL
+// term and slope are in 32 bits from there on: the softmax sum under them is (its error, up to 1e-7, reaches all of them), and
+// a row of 119 logits has as much work in these few numbers as in its exponentials.  Their sums are in 64 bits again.
 template <int MODE>
 __device__ __forceinline__ float row_epilogue(const TokenRows& a, const PolicyIn& p, const RowOut& o, int64_t t, const RowScalars& c,
                                               float xt, float M, float S, float inv_s, bool writer, float A, double w, double* acc) {
@@ -323,7 +327,7 @@ template <int N> __device__ __forceinline__ float add_pack(float s, const float 
   return s;
 }
 // Half-precision rows that start between two 32-bit words (odd strides): packs across word borders come slower.  Where many
-// blocks of few lanes hold rows in registers it shows less (rows of 32003 bf16 127 us, of 32004 115); the kernel that streams
+// blocks of few lanes hold rows in registers it shows less (6007 rows of 32003 bf16 92 us, of 32004 75); the kernel that streams
 // longer rows reads whole words, five a pack, and shifts them (another partition of the row would be another order of its sum,
 // which would then change with the stride).  The halves before and behind the pack that come with the words lie in words of
 // the row's own ends.  (Log-probabilities of 1601 rows of 120001 bf16 94 us without, 86 with them.)
@@ -516,7 +520,7 @@ template <typename T, int TPR>
 __device__ __forceinline__ void row_gradient(const TokenRows& a, const T* row, T* d, int id, int r, float M, float inv_s, float g) {
   constexpr int N = Pack<T>::N;
   // long rows: packs from the first cache line of the gradient on, which a wave then writes whole; the elements before and
-  // behind them go to a lane each (preference of 6007 rows of 32003 bf16 284 -> 276 us, 20000 of 8201 fp32 415 -> 403)
+  // behind them go to a lane each (preference loss of 6007 rows of 32003 bf16 284 -> 274 us, 20000 of 8201 fp32 408 -> 400)
   const int V = a.V, head = TPR >= 256 ? uniform((int)(-reinterpret_cast<uintptr_t>(d) & 127) / (int)sizeof(T)) : 0;
   const int shift = head < V ? head : V, nb = (V - shift) / N, edges = V - nb * N;
   const bool off = g == 0.f || inv_s == 0.f;
@@ -643,7 +647,8 @@ __global__ __launch_bounds__(256) void k_token_grad(TokenRows a, LossTail f, con
   T* const mine = stage + (FLAT ? (threadIdx.x >> 6) * ROWS * FLAT_V : 0);
   for (int64_t from = (int64_t)blockIdx.x * RPB; from < a.n; from += (int64_t)blocks * RPB) {
     // long rows from the last one back: a preference step has just read them, and the last ones may still be in the last-level
-    // cache (6007 rows of 32003 bf16 251 us against 259; without effect on batches many times its size)
+    // cache (a logits buffer that is used again and again: 6007 rows of 32003 bf16 266 us against 270, 3000 of 32000 fp32 231
+    // against 234; several buffers in turn: no more than 1 % either way)
     const int64_t base = TPR == 256 ? a.n - 1 - from : from;
     const int64_t t = base + threadIdx.x / TPR;
     if (t < a.n) {
@@ -873,7 +878,7 @@ __device__ __forceinline__ double pair_loss(const PrefIn& a, int64_t pr, double 
   return loss;
 }
 // Pairs: sequence p is preferred over sequence P + p.  A wave joins the parts of both (a margin is what two long sums leave:
-// 64 bits); 64 pairs a wave at a time when the batch is one chunk and every sequence has one part.  5 us for 512 pairs.
+// 64 bits).  5 us for 512 pairs.
 __global__ __launch_bounds__(256) void k_preference(PrefIn a) {
   __shared__ double red[4];
   double total = 0.0;
@@ -887,7 +892,8 @@ __global__ __launch_bounds__(256) void k_preference(PrefIn a) {
   total = block_sum<256>(total, red);
   if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
 }
-// A batch of one chunk: rows -> sequences, pairs and the loss in one launch of one block.
+// A batch of one chunk, where every sequence is one part: rows -> sequences, pairs (a thread each) and the loss in one launch
+// of one block.
 __global__ __launch_bounds__(256) void k_preference_small(SegRows g, PrefIn a) {
   __shared__ SegShared<true> sh;
   __shared__ double red[4];

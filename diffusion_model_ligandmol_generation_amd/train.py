@@ -387,10 +387,11 @@ class ResearchAccurateTrainer:
     def policy_step(self, batch, draws, advantage, old_logp=None, ref_logp=None, advantage_per="sequence", clip_low=0.2,
                     clip_high=0.2, kl_coef=0.0, aggregate="token", temperature=1.0, lr=None):
         """One optimiser step on rewards (``tokens.policy_loss`` on ``atom_pred`` and ``batch.atom_types``): ``advantage`` has
-        one value for each molecule (or atom), ``old_logp`` are the log-probabilities under the policy that chose the
-        types, ``ref_logp`` those under the reference, both from ``atom_type_logprobs`` with the same ``draws``.  Under data
-        parallelism the mean goes over all ranks' atoms / molecules.  ``lr`` as in ``preference_step``.  Returns
-        tokens.PolicyGrad (this rank's share)."""
+        one value for each molecule (or atom), ``old_logp`` are the log-probabilities that an earlier policy gives to
+        ``batch.atom_types`` (None: this one), ``ref_logp`` those of the reference, both from ``atom_type_logprobs`` with the same
+        ``draws``.  (The samplers take the argmax of ``atom_pred``, which has no probability: types that are to count as that
+        policy's own are drawn from its softmax at these draws.)  Under data parallelism the mean goes over all ranks' atoms /
+        molecules.  ``lr`` as in ``preference_step``.  Returns tokens.PolicyGrad (this rank's share)."""
         from .tokens import _policy_inputs, policy_loss_and_grad
         draws, inputs = dict(draws or {}), []
 

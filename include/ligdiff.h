@@ -593,8 +593,10 @@ int ligdiff_validity_gate(const float* x, const float* pos, const int32_t* mol_p
  * in the reference, which takes one-hot types and has no loss on atom_pred's distribution.
  * Ids are int32 or int64 (token_bytes 4 or 8).  An id outside [0, vocab) is an ignored position (padding), not an
  * error: it looks up a row of zeros, has log-probability 0 and takes no part in a loss or gradient.  Sums, softmax
- * statistics and gradients are formed in 32 bits or more and rounded once to the element type.  Nothing is accumulated
- * by atomics: results do not change from run to run.
+ * statistics and gradients are formed in 32 bits or more and rounded once to the element type.  Of the losses, logarithms,
+ * sums over positions and margins are in 64 bits; a position's difference to ref_logp or old_logp is rounded to 32, and the
+ * policy loss's ratio, clip bounds and KL term are in 32.  Nothing is accumulated by atomics: results do not change from
+ * run to run.
  * ------------------------------------------------------------------------------- */
 enum ligdiff_dtype { LIGDIFF_F32 = 0, LIGDIFF_BF16 = 1, LIGDIFF_F16 = 2 };
 
