@@ -831,12 +831,12 @@ __device__ __forceinline__ void join_parts(const int32_t* __restrict__ seq_ptr, 
 }
 __global__ __launch_bounds__(256) void k_sequence_lengths(const int32_t* __restrict__ seq_ptr, int64_t n, int32_t S,
                                                           const int32_t* __restrict__ part_len, int32_t* __restrict__ seq_len) {
-  const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (s >= S) return;
-  double sum;
-  int len;
-  join_parts<false>(seq_ptr, n, s, nullptr, part_len, sum, len);
-  if ((threadIdx.x & 63) == 0) seq_len[s] = len;
+  for (int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); s < S; s += (int64_t)gridDim.x * 4) {
+    double sum;
+    int len;
+    join_parts<false>(seq_ptr, n, s, nullptr, part_len, sum, len);
+    if ((threadIdx.x & 63) == 0) seq_len[s] = len;
+  }
 }
 
 struct PrefIn {
@@ -1185,7 +1185,7 @@ extern "C" int ligdiff_policy_loss(const ligdiff_token_args* args, const ligdiff
                        SegRows{a.tok, a.n, q->seq_ptr, q->n_seq, nullptr, w.seq_of, nullptr, per_seq ? w.part_len : nullptr, w.chunk_len});
   // (in a batch of one chunk a sequence is its one part)
   if (per_seq && !small && chunks > 1)
-    hipLaunchKernelGGL(k_sequence_lengths, dim3(ceil_div(q->n_seq, 4)), dim3(256), 0, s, q->seq_ptr, a.n, q->n_seq, w.part_len, w.seq_len);
+    hipLaunchKernelGGL(k_sequence_lengths, dim3(row_grid(((int64_t)q->n_seq + 3) / 4, 1 << 20)), dim3(256), 0, s, q->seq_ptr, a.n, q->n_seq, w.part_len, w.seq_len);
   PolicyIn p;
   p.seq_of = w.seq_of; p.seq_len = chunks > 1 ? w.seq_len : w.part_len; p.chunk_len = w.chunk_len; p.n_chunks = chunks;
   p.denom = (double)q->denominator; p.n_seq = q->n_seq; p.per_seq_mean = per_seq;

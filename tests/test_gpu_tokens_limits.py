@@ -183,3 +183,19 @@ def test_sums_that_start_with_the_largest(tk, dtype, low, V):
     for T in (1, 5):
         r = tk.policy_loss_and_grad(x[:T], ids[:T], None, torch.ones(1, device="cuda"), kl_coef=0.0)
         within(r.logp, want[:T], 104 * U, "policy")
+
+
+def test_more_sequences_than_one_launch_holds(tk):
+    """A wave for each of 68 million sequences would be more than the 2^32 threads of a launch.  Nearly all are empty."""
+    g = gen(36)
+    T, S = 1500, 68_000_000
+    x, ids = torch.randn(T, 9, device="cuda", generator=g), ids_of(T, 9, g, 0.1)
+    few = torch.tensor([0, 400, 1100, T], device="cuda", dtype=torch.int32)
+    ptr = torch.zeros(S + 1, dtype=torch.int32, device="cuda")
+    ptr[S // 2:], ptr[-2:], ptr[-1:] = 400, 1100, T        # the last three are not empty
+    ptr[S - 2] = 400
+    adv = torch.zeros(S, device="cuda")
+    adv[S // 2 - 1], adv[-2:] = 0.3, torch.tensor([-1.2, 0.7], device="cuda")
+    got = tk.policy_loss_and_grad(x, ids, ptr, adv, kl_coef=0.0, aggregate="sequence", denominator=3)
+    want = tk.policy_loss_and_grad(x, ids, few, torch.tensor([0.3, -1.2, 0.7], device="cuda"), kl_coef=0.0, aggregate="sequence")
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and bool(got.d_logits.any())
