@@ -812,6 +812,19 @@ void embed_grad(const EmbedGrad& g, void* workspace, hipStream_t s) {
   else { if (wide) segment_sums<f16_t, float>(a, s); else segment_sums<f16_t, f16_t>(a, s); }
 }
 
+// A launch holds fewer than 2^32 threads: 2^29 rows of a table that is sorted for, 2^29 columns over the rows of a small one.
+static bool launches_fit(const EmbedGrad& g) {
+  const int64_t most = 0xffffffffLL;
+  if (table_form(g.n, g.rows, g.d_stride)) {
+    const int64_t tiles = ((int64_t)g.width + 63) / 64;
+    return table_chunks(g.n, g.rows, g.width) * tiles * TABLE_WAVES * 64 <= most && g.rows * tiles * 512 <= most;
+  }
+  const int64_t columns = 64 * (g.dtype == LIGDIFF_F32 ? Pack<float>::N : Pack<bf16_t>::N), tiles = (g.width + columns - 1) / columns;
+  const int64_t per = (int64_t)chunk_rows(g.n, (int)tiles) * SUM_WAVES, chunks = (g.n + per - 1) / per;
+  return (((int64_t)g.rows + ZERO_ROWS - 1) / ZERO_ROWS + chunks * tiles) * SUM_WAVES * 64 <= most &&
+         chunks * (((int64_t)g.width + 255) / 256) * JOIN_WAVES * 64 <= most;
+}
+
 extern "C" size_t ligdiff_embed_grad_workspace_bytes(int64_t n_tokens, int64_t n_rows, int32_t width) {
   if (bad_embed(LIGDIFF_F32, n_rows, width, 4, n_tokens)) return 0;
   return embed_grad_workspace(n_tokens, (int32_t)n_rows, width);
@@ -825,9 +838,10 @@ extern "C" int ligdiff_embed_grad(const void* d_out, int32_t dtype, int64_t d_st
       d_stride < width || table_stride < width || !d_table || !workspace)
     return LIGDIFF_ERR_ARG;
   if (n_tokens > 0 && (!d_out || !tokens)) return LIGDIFF_ERR_ARG;
-  if (workspace_bytes < embed_grad_workspace(n_tokens, (int32_t)n_rows, width)) return LIGDIFF_ERR_WORKSPACE;
-  EmbedGrad g{d_out, dtype, d_stride, TokenView{tokens, token_bytes, (int32_t)n_rows}, n_tokens, (int32_t)n_rows, width, scale,
+  const EmbedGrad g{d_out, dtype, d_stride, TokenView{tokens, token_bytes, (int32_t)n_rows}, n_tokens, (int32_t)n_rows, width, scale,
               d_table, grad_dtype, table_stride, accumulate != 0};
+  if (!launches_fit(g)) return LIGDIFF_ERR_ARG;
+  if (workspace_bytes < embed_grad_workspace(n_tokens, (int32_t)n_rows, width)) return LIGDIFF_ERR_WORKSPACE;
   embed_grad(g, workspace, (hipStream_t)stream);
   LD_CHECK_LAUNCH();
   return LIGDIFF_OK;

@@ -609,7 +609,8 @@ int ligdiff_embed(const void* table, int32_t dtype, int64_t n_rows, int32_t widt
 /* d_table[v, :] = scale * sum of d_out[i, :] over the positions with tokens[i] == v, zeros where there is none (with
  * accumulate != 0 the sums are added to d_table and other rows left alone).  Sums are in 32 bits and in an order that depends
  * on the sizes, strides, types and tokens only: the same call gives the same bits.  No sum runs over more than 1024 positions
- * one by one; beyond that it is a sum of such parts.  grad_dtype: dtype or LIGDIFF_F32. */
+ * one by one; beyond that it is a sum of such parts.  Tables beyond what a launch holds are refused
+ * (LIGDIFF_ERR_ARG): from 2^29 rows on, or from 2^29 elements on for up to 128 rows.  grad_dtype: dtype or LIGDIFF_F32. */
 size_t ligdiff_embed_grad_workspace_bytes(int64_t n_tokens, int64_t n_rows, int32_t width);
 int ligdiff_embed_grad(const void* d_out, int32_t dtype, int64_t d_stride, const void* tokens, int32_t token_bytes,
                        int64_t n_tokens, int64_t n_rows, int32_t width, float scale, void* d_table,
