@@ -142,7 +142,7 @@ __device__ __forceinline__ void chain_tall(const ChainLane& cl, unsigned off, f3
       [&](auto J) -> f32x16& { return out[decltype(J)::value >> 2]; });
 }
 
-// SiLU of an accumulator tile, two elements per packed instruction where the ISA has one
+// SiLU of an accumulator tile, two elements at a time
 __device__ __forceinline__ void silu_tile(f32x16& u) {
 #pragma unroll
   for (int k = 0; k < 16; k += 2) {

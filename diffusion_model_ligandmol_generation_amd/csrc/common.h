@@ -24,9 +24,8 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // erf with absolute error <= 3e-7 (Abramowitz & Stegun 7.1.28):
 //   1 - (1 + a1 t + ... + a6 t^6)^-16,  t = |x|.
 // Six FMAs, four squarings and ONE reciprocal, no exponential: the transcendental unit runs at
-// a quarter of the FMA rate, and GELU sits inside GEMM epilogues that are VALU-bound.  The
-// two-wide form keeps the polynomial on packed fp32 instructions (v_pk_fma_f32: two lanes of
-// work per issue).  For |x| > ~9 the power overflows to +inf and the reciprocal gives 0.
+// a quarter of the FMA rate, and GELU sits inside GEMM epilogues that are VALU-bound.  Two
+// values at a time are two independent chains of the polynomial.  For |x| > ~9 the power overflows to +inf and the reciprocal gives 0.
 __device__ __forceinline__ f32x2 erf_fast2(f32x2 x) {
   const f32x2 t = __builtin_elementwise_abs(x);
   f32x2 p = t * 0.0000430638f + 0.0002765672f;

@@ -232,7 +232,7 @@ struct EpiBiasAct {
   }
   // Column-split form (NW accumulators per wave: columns [32 NW half, 32 NW (half + 1)) of the block).
   // The optional outputs are a template switch so that the row loop has no per-element branch, and
-  // GELU runs two columns at a time on packed fp32 instructions.
+  // GELU runs two columns at a time.
   template <bool PRE, int NW, class MB>
   __device__ __forceinline__ void cs_body(f32x16 (&acc)[NW], int row0, int by, int half, int lane, const MB&) const {
     const int c0 = half * 32 * NW + (lane & 31);

@@ -1,6 +1,6 @@
 // Stand-alone check and timing of the fused feed-forward kernel against the two-launch path
 // (developer tool, not part of the library).
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -o chain_bench chain_bench.hip
+// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -o chain_bench chain_bench.hip
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>

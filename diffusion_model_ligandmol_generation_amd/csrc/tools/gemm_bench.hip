@@ -1,5 +1,5 @@
 // Stand-alone timing harness for the row-slab GEMM kernels (developer tool, not part of the
-// library).  Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -o gemm_bench gemm_bench.hip
+// library).  Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -o gemm_bench gemm_bench.hip
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>

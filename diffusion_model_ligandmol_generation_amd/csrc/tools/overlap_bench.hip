@@ -32,7 +32,6 @@ __global__ void k_roles(float* out, int mfma_iters, int valu_iters, int mfma_wav
         for (int v = 0; v < 8; ++v) {
           if (KIND == 0) asm volatile("v_fma_f32 %0, %0, %1, %1" : "+v"(x[v]) : "v"(b));
           if (KIND == 1) asm volatile("v_or_b32 %0, %0, %1" : "+v"(x[v]) : "v"(b));
-          if (KIND == 2) asm volatile("v_pk_fma_f32 %0, %0, %1, %1" : "+v"(*(double*)&x[v & 6]) : "v"(*(double*)&x[(v & 6)]));
         }
       }
     }
@@ -91,9 +90,6 @@ int main() {
     float t_v = time_it([&] { hipLaunchKernelGGL((k_roles<1, 1>), dim3(256), dim3(512), 0, 0, out, 0, vi, 1, 1); }, 5);
     float t_b = time_it([&] { hipLaunchKernelGGL((k_roles<1, 1>), dim3(256), dim3(512), 0, 0, out, mi, vi, 1, 1); }, 5);
     printf("cross-wave v_or_b32   (%6d VALU/wave): VALU only %7.1f us, both %7.1f us\n", vi * 256, t_v, t_b);
-    t_v = time_it([&] { hipLaunchKernelGGL((k_roles<1, 2>), dim3(256), dim3(512), 0, 0, out, 0, vi, 1, 1); }, 5);
-    t_b = time_it([&] { hipLaunchKernelGGL((k_roles<1, 2>), dim3(256), dim3(512), 0, 0, out, mi, vi, 1, 1); }, 5);
-    printf("cross-wave v_pk_fma   (%6d VALU/wave): VALU only %7.1f us, both %7.1f us\n", vi * 256, t_v, t_b);
   }
   {
     float t2 = time_it([&] { hipLaunchKernelGGL((k_roles<1, 0>), dim3(256), dim3(512), 0, 0, out, mi, 0, 2, 0); }, 5);

@@ -1,5 +1,5 @@
 // Where the split-operand GEMM's time goes: copies of its main loop with parts removed (results are garbage).
-// Developer tool, not part of the library.  Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -o split_ablate split_ablate.hip
+// Developer tool, not part of the library.  Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -o split_ablate split_ablate.hip
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
