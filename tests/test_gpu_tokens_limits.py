@@ -1,6 +1,6 @@
-"""GPU: the token operators where a value has no bound or a size has no room: infinite margins of the
-preference loss; derivatives that they do not have; sizes beyond 32 bits; long sums.  Against plain 64-bit forms; the tolerances of single values are
-those of test_gpu_tokens.py (U half a step of fp32, LOGP the error of a log-probability)."""
+"""GPU: the token operators where a value has no bound or a size has no room: infinite margins of the preference loss,
+derivatives that they do not have, sizes beyond 32 bits, long sums.  Against plain 64-bit forms; the tolerances of single values
+are those of test_gpu_tokens.py (U half a step of fp32, LOGP the error of a log-probability)."""
 import pytest
 import torch
 
